@@ -353,6 +353,52 @@ int mxfa_varlen_fwd_exact_launch(const void* q, const void* k, const void* v, co
                                  int total_q, int total_k, int HQ, int HKV, int D, int causal, int bf16,
                                  float scale, void* stream);
 
+/* ------------------------------------------- ragged batch over a paged cache
+ *
+ * Packed tokens [T, heads, D]: sequence b owns rows cu[b] .. cu[b+1] (int32
+ * [B + 1] on the device), the LAST of the seqlens[b] tokens its cache holds
+ * once the call's tokens are in it: packed row t is position
+ * seqlens[b] - cu[b+1] + t.  Rows past cu[B] are padding and left alone.
+ * Caches are paged [P, PS, HKV, D] with a block table int32 [B, BTW]; D in
+ * {64, 128}.  Quantised caches (k_scales and v_scales given) hold e4m3 codes
+ * and one e8m0 byte per token and KV head, [P, HKV, PS]: value = code *
+ * 2^(byte - 127).  Out-of-range pages and positions are skipped and flagged.
+ * No reference counterpart: the reference appends and attends uniform
+ * blocks (mxflashattn/reference.py:88-139) and has no quantised cache. */
+
+/* Write packed k, v [T, HKV, D] (strides in elements; D contiguous) into the
+ * caches: a bit-exact copy, or with scales quantised -- the scale is the
+ * smallest power of two s >= 2^-126 with max |x| <= 448 s over the row's
+ * finite values, the code e4m3(x / s) to nearest even, saturating (an
+ * infinity becomes +-448 s, a NaN stays NaN). */
+int mxfa_kvcache_append_varlen_launch(const void* k, const void* v, void* k_cache, void* v_cache,
+                                      void* k_scales, void* v_scales, const int32_t* cu_seqlens,
+                                      const int32_t* seqlens, const int32_t* block_table, int total,
+                                      int B, int HKV, int D, int PS, int BTW, int num_pages,
+                                      size_t k_token_stride, size_t k_head_stride,
+                                      size_t v_token_stride, size_t v_head_stride, int bf16,
+                                      void* stream);
+
+/* Read the packed tokens back: k_out, v_out [T, HKV, D] contiguous, code *
+ * scale rounded once to the output type (16-bit caches are copied). */
+int mxfa_kvcache_gather_varlen_launch(const void* k_cache, const void* v_cache, const void* k_scales,
+                                      const void* v_scales, const int32_t* cu_seqlens,
+                                      const int32_t* seqlens, const int32_t* block_table, void* k_out,
+                                      void* v_out, int total, int B, int HKV, int D, int PS, int BTW,
+                                      int num_pages, int bf16, void* stream);
+
+/* Attention of packed queries q [T, HQ, D] (strides in elements, multiples
+ * of 8) over each sequence's seqlens[b] cached tokens; causal: the query at
+ * position p sees keys 0 .. p.  out [T, HQ, D]; lse optional f32 [T, HQ]
+ * (natural log).  A row that sees no key outputs 0 and LSE -inf. */
+int mxfa_kvcache_varlen_attention_launch(const void* q, const void* k_cache, const void* v_cache,
+                                         const void* k_scales, const void* v_scales,
+                                         const int32_t* cu_seqlens_q, const int32_t* seqlens,
+                                         const int32_t* block_table, void* out, float* lse, int total_q,
+                                         int B, int HQ, int HKV, int D, int PS, int BTW, int num_pages,
+                                         size_t q_token_stride, size_t q_head_stride, int causal,
+                                         int bf16, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

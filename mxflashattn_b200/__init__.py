@@ -10,6 +10,8 @@ record, validation and policy objects.
 from .accuracy import ErrorSummary, summarize_error
 from .api import flash_attn_func, flash_attn_varlen_func, flash_attn_with_kvcache, kvcache_length_order
 from .dispatch import BACKEND_LABEL, BackendUnavailableError, DispatchInfo, get_last_dispatch_info
+from .varlen_cache import (KvChunkPlan, flash_attn_varlen_with_kvcache, kvcache_append_varlen, kvcache_chunk_plan,
+                           kvcache_gather_varlen)
 from .policy import AdaptiveDispatchPolicy, DispatchDecision, DispatchPolicyConfig, WorkloadShape
 
 __all__ = [
@@ -18,9 +20,14 @@ __all__ = [
     "DispatchInfo",
     "flash_attn_func",
     "flash_attn_varlen_func",
+    "flash_attn_varlen_with_kvcache",
     "flash_attn_with_kvcache",
     "get_last_dispatch_info",
+    "kvcache_append_varlen",
+    "kvcache_chunk_plan",
+    "kvcache_gather_varlen",
     "kvcache_length_order",
+    "KvChunkPlan",
     "AdaptiveDispatchPolicy",
     "DispatchDecision",
     "DispatchPolicyConfig",

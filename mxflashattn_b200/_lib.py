@@ -79,6 +79,13 @@ SIGNATURES = {
     "mxfa_lse_merge_launch": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "mxfa_kv_append_launch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "mxfa_seqlens_add_launch": (_i, [_vp, _i, _i, _i, _vp]),
+    "mxfa_kvcache_append_varlen_launch": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _sz, _sz, _sz, _sz, _i, _vp]),
+    "mxfa_kvcache_gather_varlen_launch": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "mxfa_kvcache_varlen_attention_launch": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _sz, _sz, _i, _i, _f,
+             _vp]),
     "mxfa_varlen_fwd_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp]),
     "mxfa_varlen_fwd_exact_launch": (

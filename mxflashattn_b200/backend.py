@@ -383,6 +383,64 @@ def kvcache_attention_packed(q, k_cache, v_cache, cache_seqlens, block_table, so
     return out
 
 
+# ------------------------------------ a ragged batch over a paged cache
+
+def _rows16(t):
+    """``t`` with unit stride along D and 16-byte rows: itself, or a packed copy."""
+    s = t.stride()
+    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def kvcache_append_varlen(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, k_scales, v_scales) -> None:
+    """Packed k/v [T, HKV, D] into their pages, copied or quantised (no length update)."""
+    k = k if k.stride(2) == 1 else k.contiguous()
+    v = v if v.stride(2) == 1 else v.contiguous()
+    cu, seq, bt = _i32(cu_seqlens), _i32(cache_seqlens), _i32(block_table)
+    T, HKV, D = k.shape
+    ks, vs = k.stride(), v.stride()
+    with _on(k):
+        rc = _L().mxfa_kvcache_append_varlen_launch(
+            k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales),
+            _lib.ptr(v_scales), cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), T, seq.shape[0], HKV, D,
+            k_cache.shape[1], bt.shape[1], k_cache.shape[0], ks[0], ks[1], vs[0], vs[1], _bf16(k), _stream(k))
+    _lib.check(rc, "mxfa_kvcache_append_varlen_launch")
+
+
+def kvcache_gather_varlen(k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, k_scales, v_scales, k, v) -> None:
+    """Packed k/v [T, HKV, D] (written) from their pages."""
+    cu, seq, bt = _i32(cu_seqlens), _i32(cache_seqlens), _i32(block_table)
+    T, HKV, D = k.shape
+    with _on(k):
+        rc = _L().mxfa_kvcache_gather_varlen_launch(
+            k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales), cu.data_ptr(),
+            seq.data_ptr(), bt.data_ptr(), k.data_ptr(), v.data_ptr(), T, seq.shape[0], HKV, D, k_cache.shape[1],
+            bt.shape[1], k_cache.shape[0], _bf16(k), _stream(k))
+    _lib.check(rc, "mxfa_kvcache_gather_varlen_launch")
+
+
+def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q,
+                                   max_seqlen_k, softmax_scale, causal, k_scales=None, v_scales=None, plan=None,
+                                   out=None, return_lse: bool = False):
+    """Packed q [Tq, HQ, D] over paged caches, 16-bit or e4m3 with scales (see varlen_cache.py)."""
+    q = _rows16(q)
+    cu, seq, bt = _i32(cu_seqlens_q), _i32(cache_seqlens), _i32(block_table)
+    Tq, HQ, D = q.shape
+    if out is None:
+        out = torch.empty((Tq, HQ, D), device=q.device, dtype=q.dtype)
+    lse = torch.empty((Tq, HQ), device=q.device, dtype=torch.float32) if return_lse else None
+    PS, HKV = k_cache.shape[1], k_cache.shape[2]
+    with _on(q):
+        rc = _L().mxfa_kvcache_varlen_attention_launch(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales),
+            cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), out.data_ptr(), _lib.ptr(lse), Tq, seq.shape[0], HQ, HKV,
+            D, PS, bt.shape[1], k_cache.shape[0], q.stride(0), q.stride(1), int(causal), _bf16(q),
+            float(softmax_scale), _stream(q))
+    _lib.check(rc, "mxfa_kvcache_varlen_attention_launch")
+    return (out, lse) if return_lse else out
+
+
 # ------------------------------------------------------ combine / merge
 
 def split_combine(ows, mdws, rows: int, head_dim: int, num_splits: int, dtype, *, lse: bool = False,

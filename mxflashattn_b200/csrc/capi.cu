@@ -19,6 +19,7 @@
 #include <cstdlib>
 
 #include "decode.cuh"
+#include "paged_varlen.cuh"
 #include "prefill_sm100.cuh"
 
 namespace mxfa {
@@ -1187,3 +1188,5 @@ extern "C" int mxfa_kvcache_attention_noalloc_launch(const void* q, const void* 
                                        scratch ? MXFA_NOALLOC_SCRATCH_BYTES : 0, B, Sq, HQ, HKV, D, PS, BTW,
                                        num_pages, append_len, num_splits, chunk_len, causal, bf16, scale, stream);
 }
+
+#include "capi_varlen.cuh"

@@ -1,0 +1,346 @@
+// paged_varlen.cuh -- a ragged batch over a paged cache: append, read-back, row attention.
+//
+// Every kernel here takes packed tokens [T, heads, D] whose sequence b owns
+// rows cu[b] .. cu[b+1], and seqlens[b], the tokens the cache holds for b
+// with those included: packed row t of sequence b is position
+// seqlens[b] - cu[b+1] + t of its block-table row.  No reference counterpart
+// (the reference appends a uniform block, mxflashattn/reference.py:108-122).
+//
+// Quantised caches hold e4m3 codes [P, PS, HKV, D] and one e8m0 byte per
+// (token, KV head), [P, HKV, PS]: value = code * 2^(byte - 127).  The scale
+// is the smallest power of two s >= 2^-126 with max |x| <= 448 s.  e4m3 is a
+// floating format, so a power of two costs no precision against max/448
+// (only the last binade of the subnormal range differs), and in return x / s
+// is exact before its one rounding, the scale is one byte, and code * s is
+// exact in bf16: reading back or multiplying through never rounds again.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace mxfa {
+
+// Sequence of packed token t (one warp): the number of entries cu[1..B] that
+// are <= t, every lane comparing its own; B when no sequence holds t.
+__device__ __forceinline__ int token_sequence(const int* __restrict__ cu, int B, int t, int lane) {
+  int n = 0;
+  for (int i = 0; i < B; i += 32) {
+    const bool before = i + lane < B && cu[1 + i + lane] <= t;
+    const int c = __popc(__ballot_sync(0xffffffffu, before));
+    n += c;
+    if (c < 32) break;  // the rest lie behind t
+  }
+  return n;
+}
+
+// Cache row (page * PS + offset) of position pos of sequence b, or -1 with
+// the flag raised when the table or the cache does not have it.
+__device__ __forceinline__ long long paged_row(const int* __restrict__ bt, int b, int pos, int PS, int BTW, int P) {
+  const int page = pos / PS;
+  if (pos < 0 || page >= BTW) {
+    raise_flag(MXFA_FLAG_TABLE_TOO_NARROW);
+    return -1;
+  }
+  const int phys = bt[static_cast<size_t>(b) * BTW + page];
+  if (phys < 0 || phys >= P) {
+    raise_flag(MXFA_FLAG_PAGE_OUT_OF_RANGE);
+    return -1;
+  }
+  return static_cast<long long>(phys) * PS + (pos - page * PS);
+}
+
+struct PagedVarlenParams {
+  const void* k;  // append: packed input; gather: packed output (written)
+  const void* v;
+  size_t k_tok, k_head, v_tok, v_head;  // strides of the packed tensors, elements
+  uint8_t* k_cache;  // [P, PS, HKV, D]
+  uint8_t* v_cache;
+  uint8_t* k_scales;  // [P, HKV, PS], quantised caches
+  uint8_t* v_scales;
+  const int* cu;       // [B+1]
+  const int* seqlens;  // [B]
+  const int* bt;       // [B, BTW]
+  int T, B, HKV, PS, BTW, P;
+  int tok_per_cta;
+};
+
+constexpr int kPvThreads = 256;
+constexpr int kPvMaxTok = 32;  // tokens of one CTA
+
+// The cache rows of this CTA's tokens, one warp per token: -1 not mapped.
+__device__ __forceinline__ void cta_token_rows(const PagedVarlenParams& p, int t0, int n, long long* rows) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = warp; i < n; i += kPvThreads / 32) {
+    const int t = t0 + i;
+    const int b = token_sequence(p.cu, p.B, t, lane);
+    if (lane == 0)
+      rows[i] = b < p.B ? paged_row(p.bt, b, p.seqlens[b] - p.cu[b + 1] + t, p.PS, p.BTW, p.P) : -1;
+  }
+}
+
+// Exponent k of the row scale 2^k for the largest finite magnitude amax:
+// amax = 1.m * 2^E, 448 = 1.75 * 2^8.
+__device__ __forceinline__ int scale_exponent(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  const int E = static_cast<int>(bits >> 23) - 127;
+  const int k = E - ((bits & 0x7fffffu) > 0x600000u ? 7 : 8);
+  return max(k, -126);
+}
+
+// Append: a group of D/8 lanes moves one (token, KV head) row of K or V,
+// eight values a lane.  HBM-bound: each value is read once and its code (or
+// itself) written once; a group reduces its row's maximum by shuffles, so
+// nothing is staged.  kVec: the rows allow 16-byte loads.
+template <typename T, int HD, bool kQuant, bool kVec>
+__global__ void __launch_bounds__(kPvThreads) append_varlen_kernel(const PagedVarlenParams p) {
+  constexpr int kGroup = HD / 8;
+  __shared__ long long s_rows[kPvMaxTok];
+  const int t0 = blockIdx.x * p.tok_per_cta;
+  const int n = min(p.tok_per_cta, p.T - t0);
+  cta_token_rows(p, t0, n, s_rows);
+  __syncthreads();
+  const int sub = threadIdx.x % kGroup;
+  const int per_tok = 2 * p.HKV;  // K heads, then V heads
+  const int total = n * per_tok;
+  // every lane of a warp runs the same number of rounds: the shuffles below
+  // need all of them
+  for (int base = 0; base < total; base += kPvThreads / kGroup) {
+    const int idx = base + threadIdx.x / kGroup;
+    const int i = idx / per_tok;
+    const int kv = (idx - i * per_tok) / p.HKV;
+    const int h = idx - i * per_tok - kv * p.HKV;
+    const long long row = idx < total ? s_rows[i] : -1;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (row >= 0) {
+      const T* src = kv ? static_cast<const T*>(p.v) + static_cast<size_t>(t0 + i) * p.v_tok + h * p.v_head
+                        : static_cast<const T*>(p.k) + static_cast<size_t>(t0 + i) * p.k_tok + h * p.k_head;
+      src += sub * 8;
+      if constexpr (kVec) {
+        raw = *reinterpret_cast<const uint4*>(src);
+      } else {
+        const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
+        raw.x = s16[0] | (static_cast<uint32_t>(s16[1]) << 16);
+        raw.y = s16[2] | (static_cast<uint32_t>(s16[3]) << 16);
+        raw.z = s16[4] | (static_cast<uint32_t>(s16[5]) << 16);
+        raw.w = s16[6] | (static_cast<uint32_t>(s16[7]) << 16);
+      }
+    }
+    uint8_t* cache = kv ? p.v_cache : p.k_cache;
+    if constexpr (!kQuant) {
+      if (row >= 0) *reinterpret_cast<uint4*>(cache + ((row * p.HKV + h) * HD + sub * 8) * 2) = raw;
+    } else {
+      const float2 a = Elem<T>::unpack(raw.x), b = Elem<T>::unpack(raw.y);
+      const float2 c = Elem<T>::unpack(raw.z), d = Elem<T>::unpack(raw.w);
+      const float x[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+      // the maximum is over finite values: an infinity saturates to 448 s and
+      // a NaN stays a NaN, and neither costs the rest of its row
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float m = fabsf(x[j]);
+        amax = m < INFINITY ? fmaxf(amax, m) : amax;
+      }
+#pragma unroll
+      for (int sh = kGroup / 2; sh > 0; sh >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
+      const int k = scale_exponent(amax);
+      const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+      uint32_t q[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * j] * inv, x[4 * j + 1] * inv), __NV_SATFINITE,
+                                                     __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * j + 2] * inv, x[4 * j + 3] * inv),
+                                                     __NV_SATFINITE, __NV_E4M3);
+        q[j] = lo | (hi << 16);
+      }
+      if (row >= 0) {
+        *reinterpret_cast<uint2*>(cache + (row * p.HKV + h) * HD + sub * 8) = make_uint2(q[0], q[1]);
+        if (sub == 0) {
+          const long long page = row / p.PS;
+          (kv ? p.v_scales : p.k_scales)[(page * p.HKV + h) * p.PS + (row - page * p.PS)] =
+              static_cast<uint8_t>(k + 127);
+        }
+      }
+    }
+  }
+}
+
+// 2^(byte - 127) as a float (byte 0 is 2^-127, a subnormal; 255 is NaN).
+__device__ __forceinline__ float e8m0_to_float(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fffffffu : byte << 23);
+}
+
+// Eight e4m3 codes times one scale, as eight floats.
+__device__ __forceinline__ void dequant8(uint2 codes, float s, float (&x)[8]) {
+  uint32_t h[4];
+  e4m3x4_to_f16x2x2(codes.x, h[0], h[1]);
+  e4m3x4_to_f16x2x2(codes.y, h[2], h[3]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = Elem<__half>::unpack(h[j]);
+    x[2 * j] = f.x * s;
+    x[2 * j + 1] = f.y * s;
+  }
+}
+
+// Read-back: the append's mirror; packed rows of tokens that are not mapped
+// (or that no sequence holds) are zero.  HBM-bound, each code read once and
+// each value written once.
+template <typename T, int HD, bool kQuant>
+__global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVarlenParams p) {
+  constexpr int kGroup = HD / 8;
+  __shared__ long long s_rows[kPvMaxTok];
+  const int t0 = blockIdx.x * p.tok_per_cta;
+  const int n = min(p.tok_per_cta, p.T - t0);
+  cta_token_rows(p, t0, n, s_rows);
+  __syncthreads();
+  const int sub = threadIdx.x % kGroup;
+  const int per_tok = 2 * p.HKV;
+  const int total = n * per_tok;
+  for (int idx = threadIdx.x / kGroup; idx < total; idx += kPvThreads / kGroup) {
+    const int i = idx / per_tok;
+    const int kv = (idx - i * per_tok) / p.HKV;
+    const int h = idx - i * per_tok - kv * p.HKV;
+    const long long row = s_rows[i];
+    const uint8_t* cache = kv ? p.v_cache : p.k_cache;
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (row >= 0) {
+      if constexpr (!kQuant) {
+        out = *reinterpret_cast<const uint4*>(cache + ((row * p.HKV + h) * HD + sub * 8) * 2);
+      } else {
+        const uint2 codes = *reinterpret_cast<const uint2*>(cache + (row * p.HKV + h) * HD + sub * 8);
+        const long long page = row / p.PS;
+        const float s =
+            e8m0_to_float((kv ? p.v_scales : p.k_scales)[(page * p.HKV + h) * p.PS + (row - page * p.PS)]);
+        float x[8];
+        dequant8(codes, s, x);
+        out = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
+                         Elem<T>::pack(x[6], x[7]));
+      }
+    }
+    T* dst = static_cast<T*>(const_cast<void*>(kv ? p.v : p.k)) +
+             (static_cast<size_t>(t0 + i) * p.HKV + h) * HD + sub * 8;
+    *reinterpret_cast<uint4*>(dst) = out;
+  }
+}
+
+// ------------------------------------------------------------- row attention
+
+struct VarlenAttnParams {
+  const void* q;  // [T, HQ, D], strides q_tok / q_head
+  size_t q_tok, q_head;
+  const uint8_t* k;  // [P, PS, HKV, D]
+  const uint8_t* v;
+  const uint8_t* k_scales;  // [P, HKV, PS], quantised caches
+  const uint8_t* v_scales;
+  const int* cu;
+  const int* seqlens;
+  const int* bt;
+  void* out;   // [T, HQ, D]
+  float* lse;  // optional [T, HQ]
+  int T, B, HQ, HKV, GQ, PS, BTW, P;
+  int causal;
+  float scale_log2;
+};
+
+// One warp per (token, query head): 32 keys a round, a key per lane for the
+// scores, D/32 columns per lane for P.V.  Every K and V row is read by each
+// of its query rows, so this form is for what the tiled kernel does not
+// take.  All arithmetic is fp32; P is never rounded.
+template <typename T, int HD, bool kQuant>
+__global__ void __launch_bounds__(128) varlen_rows_kernel(const VarlenAttnParams p) {
+  constexpr int kPer = HD / 32;
+  __shared__ float s_q[4][HD];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long r = static_cast<long long>(blockIdx.x) * 4 + warp;
+  if (r >= static_cast<long long>(p.T) * p.HQ) return;
+  const int t = static_cast<int>(r / p.HQ);
+  const int h = static_cast<int>(r - static_cast<long long>(t) * p.HQ);
+  const int hk = h / p.GQ;
+  const int b = token_sequence(p.cu, p.B, t, lane);
+  if (b >= p.B) return;  // a padding row: nothing is written
+  const T* qr = static_cast<const T*>(p.q) + static_cast<size_t>(t) * p.q_tok + h * p.q_head;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) s_q[warp][j * 32 + lane] = static_cast<float>(qr[j * 32 + lane]);
+  __syncwarp();
+  const int total = p.seqlens[b];
+  const int pos = total - p.cu[b + 1] + t;
+  const int end = p.causal ? min(total, pos + 1) : total;
+  float m = -INFINITY, l = 0.f, acc[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
+  for (int k0 = 0; k0 < end; k0 += 32) {
+    long long row = -1;
+    float vs = 1.f, s = -INFINITY;
+    if (k0 + lane < end) row = paged_row(p.bt, b, k0 + lane, p.PS, p.BTW, p.P);
+    if (row >= 0) {
+      s = 0.f;
+      if constexpr (kQuant) {
+        const long long page = row / p.PS;
+        const long long at = (page * p.HKV + hk) * p.PS + (row - page * p.PS);
+        vs = e8m0_to_float(p.v_scales[at]);
+        const float ks = e8m0_to_float(p.k_scales[at]);
+        const uint8_t* kr = p.k + (row * p.HKV + hk) * HD;
+        for (int c = 0; c < HD; c += 8) {
+          float x[8];
+          dequant8(*reinterpret_cast<const uint2*>(kr + c), ks, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s = fmaf(s_q[warp][c + j], x[j], s);
+        }
+      } else {
+        const uint8_t* kr = p.k + (row * p.HKV + hk) * HD * 2;
+        for (int c = 0; c < HD; c += 8) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(kr + c * 2);
+          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = Elem<T>::unpack(w[j]);
+            s = fmaf(s_q[warp][c + 2 * j], f.x, s);
+            s = fmaf(s_q[warp][c + 2 * j + 1], f.y, s);
+          }
+        }
+      }
+      s *= p.scale_log2;
+    }
+    float mx = s;
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+    const float m_new = fmaxf(m, mx);
+    // nothing visible yet; a NaN score (which the maximum ignores) goes on
+    if (m_new == -INFINITY && !__any_sync(0xffffffffu, s != s)) continue;
+    const float alpha = fast_exp2(m - m_new);
+    const float pr = row >= 0 ? fast_exp2(s - m_new) : 0.f;
+    m = m_new;
+    float sum = pr;
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
+    l = l * alpha + sum;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) acc[j] *= alpha;
+    const int n = min(32, end - k0);
+    for (int i = 0; i < n; ++i) {
+      const long long vrow = __shfl_sync(0xffffffffu, row, i);
+      const float w = __shfl_sync(0xffffffffu, pr * vs, i);
+      if (vrow < 0) continue;
+      if constexpr (kQuant) {
+        const uint8_t* vr = p.v + (vrow * p.HKV + hk) * HD + lane * kPer;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          acc[j] = fmaf(w, __half2float(__half(__nv_cvt_fp8_to_halfraw(vr[j], __NV_E4M3))), acc[j]);
+      } else {
+        const T* vr = reinterpret_cast<const T*>(p.v + (vrow * p.HKV + hk) * HD * 2) + lane * kPer;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) acc[j] = fmaf(w, static_cast<float>(vr[j]), acc[j]);
+      }
+    }
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;  // a NaN sum stays one
+  T* orow = static_cast<T*>(p.out) + (static_cast<size_t>(t) * p.HQ + h) * HD + lane * kPer;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) orow[j] = Elem<T>::from_float(acc[j] * inv);
+  if (p.lse != nullptr && lane == 0)
+    p.lse[static_cast<size_t>(t) * p.HQ + h] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+}  // namespace mxfa

@@ -1,0 +1,385 @@
+"""GPU parity of the ragged paged-cache operators (append, read-back, attention) against 64-bit definitions."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from helpers import host
+from mxflashattn_b200 import synthetic as syn
+from varlen_oracle import assert_attention, make_batch, quantise64
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _flags_stay_clear(cuda_device):
+    import torch
+
+    from mxflashattn_b200 import _lib
+
+    _lib.read_error_flags()
+    yield
+    torch.cuda.synchronize()
+    assert _lib.read_error_flags() == 0
+
+
+# ------------------------------------------------------------------------------------------------- append, read-back
+
+def _append_inputs(seed, T, hkv, d, dtype, layout, dev):
+    import torch
+
+    rng = np.random.default_rng(seed)
+    k = rng.standard_normal((T, hkv, d), dtype=np.float32) * np.exp(rng.standard_normal((T, hkv, 1))).astype(np.float32)
+    v = rng.standard_normal((T, hkv, d), dtype=np.float32)
+    if T > 2:
+        k[1, 0] = 0.0                       # an all-zero row
+        k[2, 0] *= 1e-30 if dtype == "bf16" else 1e-7
+        v[1, 0, :] = 7.0                    # max / 448 is an exact power of two
+        v[2, 0, 0] = 448.0
+    k, v = syn.round_dtype(k, dtype), syn.round_dtype(v, dtype)
+    tdt = syn.torch_dtype(dtype)
+    kt, vt = torch.from_numpy(k).to(dev, tdt), torch.from_numpy(v).to(dev, tdt)
+    if layout == "fused":    # slices of one projection
+        qkv = torch.zeros((T, 3 + 2 * hkv, d), device=dev, dtype=tdt)
+        qkv[:, 3:3 + hkv], qkv[:, 3 + hkv:] = kt, vt
+        kt, vt = qkv[:, 3:3 + hkv], qkv[:, 3 + hkv:]
+    elif layout == "odd":    # rows that start two bytes past a 16-byte boundary
+        pad = torch.zeros((T, hkv, 2 * d + 3), device=dev, dtype=tdt)
+        pad[:, :, 1:1 + d], pad[:, :, 2 + d:2 + 2 * d] = kt, vt
+        kt, vt = pad[:, :, 1:1 + d], pad[:, :, 2 + d:2 + 2 * d]
+    elif layout == "heads_first":
+        kt, vt = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (kt, vt))
+    elif layout == "d_strided":
+        kt, vt = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (kt, vt))
+    return k, v, kt, vt
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 64), ("bf16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("layout", ["packed", "fused", "odd", "heads_first", "d_strided"])
+def test_append_writes_the_defined_codes_and_only_them(quant, dtype, d, layout, cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    new, total, page, hkv = [1, 0, 37, 16, 5], [1, 9, 300, 16, 40], 16, 3
+    b = make_batch(11, new, total, hkv=hkv, hq=hkv, d=d, page=page, dtype=dtype)
+    T = int(b.cu[-1])
+    k, v, kt, vt = _append_inputs(12, T, hkv, d, dtype, layout, cuda_device)
+    pages = b.k.shape[0]
+    tdt = syn.torch_dtype(dtype)
+    store = torch.float8_e4m3fn if quant else tdt
+    caches = [torch.full((pages, page, hkv, d), 1.5, device=cuda_device).to(store) for _ in range(2)]
+    scales = [torch.full((pages, hkv, page), 3, device=cuda_device, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+              for _ in range(2)] if quant else [None, None]
+    cu, lens, table = (torch.from_numpy(np.asarray(x)).to(cuda_device) for x in (b.cu, np.array(total), b.table))
+    fa.kvcache_append_varlen(kt, vt, caches[0], caches[1], cu, lens, table, k_scales=scales[0], v_scales=scales[1])
+    torch.cuda.synchronize()
+    rows = np.concatenate([b.slots(i, t - n, t) for i, (n, t) in enumerate(zip(new, total))])
+    for x, cache, scale in ((k, caches[0], scales[0]), (v, caches[1], scales[1])):
+        want = np.full((pages * page, hkv, d), 1.5)
+        if quant:
+            codes, s = quantise64(x)
+            want[rows] = codes
+            want_s = np.full((pages * page, hkv), 2.0 ** (3 - 127))
+            want_s[rows] = s
+            got_s = scale.float().cpu().numpy().astype(np.float64).transpose(0, 2, 1).reshape(-1, hkv)
+            assert np.array_equal(got_s, want_s)
+        else:
+            want[rows] = x
+        assert np.array_equal(host(cache).reshape(-1, hkv, d).astype(np.float64), want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_append_keeps_nan_saturates_infinity_and_their_row_stays_usable(dtype, cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    x = syn.round_dtype(np.random.default_rng(3).standard_normal((4, 1, 128), dtype=np.float32), dtype)
+    x[0, 0, 5], x[1, 0, 7], x[2, 0, 9], x[3, 0, :] = np.nan, np.inf, -np.inf, np.inf
+    xt = torch.from_numpy(x).to(cuda_device, syn.torch_dtype(dtype))
+    kc, vc = (torch.zeros((1, 16, 1, 128), device=cuda_device).to(torch.float8_e4m3fn) for _ in range(2))
+    ks, vs = (torch.zeros((1, 1, 16), device=cuda_device, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+              for _ in range(2))
+    fa.kvcache_append_varlen(xt, xt, kc, vc, torch.tensor([0, 4], device=cuda_device),
+                             torch.tensor([4], device=cuda_device),
+                             torch.zeros((1, 1), device=cuda_device, dtype=torch.int32), k_scales=ks, v_scales=vs)
+    codes, scale = quantise64(x)
+    got = host(kc)[0, :4].astype(np.float64)
+    assert np.array_equal(np.isnan(got), np.isnan(x.astype(np.float64)))
+    assert np.array_equal(got[~np.isnan(got)], codes[~np.isnan(codes)])
+    assert np.array_equal(ks.float().cpu().numpy()[0, :, :4].T.astype(np.float64), scale)
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("dtype,d,page", [("bf16", 128, 16), ("fp16", 64, 8), ("bf16", 64, 5), ("fp16", 128, 24)])
+def test_gather_returns_the_cached_values(quant, dtype, d, page, cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    new, total = [0, 1, 100, 7, 33], [20, 1, 100, 64, 57]
+    b = make_batch(21, new, total, d=d, page=page, dtype=dtype, quant=quant, poison=np.nan)
+    t = b.device(cuda_device)
+    T = int(b.cu[-1])
+    k, v = fa.kvcache_gather_varlen(t["kc"], t["vc"], t["cu"], t["lens"], t["table"], T + 3, k_scales=t["ks"],
+                                    v_scales=t["vs"], dtype=syn.torch_dtype(dtype))
+    rows = np.concatenate([b.slots(i, x - n, x) for i, (n, x) in enumerate(zip(new, total))])
+    for got, want in ((k, b.k), (v, b.v)):
+        want = want.reshape(-1, b.hkv, d)[rows]
+        want = want.astype(np.float16).astype(np.float64) if dtype == "fp16" else want  # e4m3 * 2^k is exact in bf16
+        assert np.array_equal(host(got)[:T].astype(np.float64), want)
+        assert not host(got)[T:].any()
+
+
+def test_append_then_gather_returns_the_quantised_values(cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    new, total = [5, 129, 1], [5, 200, 33]
+    b = make_batch(31, new, total, quant=True)
+    t = b.device(cuda_device)
+    T = int(b.cu[-1])
+    rng = np.random.default_rng(5)
+    x = syn.round_dtype(rng.standard_normal((2, T, b.hkv, b.d), dtype=np.float32), "bf16")
+    kt, vt = torch.from_numpy(x).to(cuda_device, torch.bfloat16)
+    fa.kvcache_append_varlen(kt, vt, t["kc"], t["vc"], t["cu"], t["lens"], t["table"], k_scales=t["ks"],
+                             v_scales=t["vs"])
+    k, v = fa.kvcache_gather_varlen(t["kc"], t["vc"], t["cu"], t["lens"], t["table"], T, k_scales=t["ks"],
+                                    v_scales=t["vs"])
+    for got, src in ((k, x[0]), (v, x[1])):
+        codes, scale = quantise64(src)
+        assert np.array_equal(host(got).astype(np.float64), codes * scale[..., None])
+
+
+# ------------------------------------------------------------------------------------------------------- attention
+
+def _attend(b, dev, causal, scale=None, index_dtype=None, plan=False, **kw):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    t = b.device(dev, index_dtype)
+    scale = b.d ** -0.5 if scale is None else scale
+    if plan:
+        kw["plan"] = fa.kvcache_chunk_plan(t["cu"], t["lens"], t["q"].shape[0], max(b.new), q_heads=b.hq,
+                                           kv_heads=b.hkv, causal=causal)
+    out, lse = fa.flash_attn_varlen_with_kvcache(t["q"], t["kc"], t["vc"], t["cu"], t["lens"], t["table"], max(b.new),
+                                                 max(b.total), softmax_scale=scale, causal=causal, k_scales=t["ks"],
+                                                 v_scales=t["vs"], return_softmax_lse=True, **kw)
+    torch.cuda.synchronize()
+    return host(out), host(lse), scale
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 128), ("bf16", 64), ("fp16", 64)])
+@pytest.mark.parametrize("hq,hkv", [(4, 4), (6, 2), (8, 2), (8, 1), (5, 1), (32, 2)])
+def test_ragged_pieces_match_the_definition(quant, dtype, d, hq, hkv, cuda_device):
+    b = make_batch(100 + hq + d, [1, 0, 37, 130, 3, 64], [1, 50, 37, 300, 257, 128], hq=hq, hkv=hkv, d=d, dtype=dtype,
+                   quant=quant, poison=np.nan)
+    out, lse, scale = _attend(b, cuda_device, True, plan=hq == 8)
+    assert_attention(out, lse, b, scale, True, f"hq{hq} hkv{hkv} d{d} {dtype} quant{quant}")
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("page", [1, 5, 8, 16, 24, 48, 64, 128, 256])
+def test_pages_that_end_inside_a_tile(quant, page, cuda_device):
+    b = make_batch(200 + page, [3, 70, 1], [131, 70, 257], page=page, quant=quant, poison=np.nan)
+    out, lse, scale = _attend(b, cuda_device, True)
+    assert_attention(out, lse, b, scale, True, f"page{page}")
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new,total", [([1], [1]), ([1], [0]), ([5], [3]), ([0, 2], [4, 0]), ([128], [128]), ([129], [129]),
+                                       ([127], [255]), ([200, 5], [100, 2]), ([32], [1000]), ([33], [1024]),
+                                       ([2], [4097]), ([1, 1, 1], [1, 5000, 128])])
+def test_lengths_that_leave_rows_empty_and_edges_of_tiles(quant, causal, new, total, cuda_device):
+    b = make_batch(300 + len(new) + total[0], new, total, quant=quant, poison=np.nan)
+    out, lse, scale = _attend(b, cuda_device, causal)
+    assert_attention(out, lse, b, scale, causal, f"new{new} total{total} causal{causal}")
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("d,dtype", [(128, "bf16"), (64, "fp16")])
+def test_single_tokens_of_many_sequences(quant, d, dtype, cuda_device):
+    rng = np.random.default_rng(7)
+    total = [int(x) for x in rng.integers(1, 700, size=40)]
+    b = make_batch(400, [1] * 40, total, d=d, dtype=dtype, quant=quant, poison=np.nan)
+    for plan in (False, True):
+        out, lse, scale = _attend(b, cuda_device, True, plan=plan)
+        assert_attention(out, lse, b, scale, True, f"singles plan{plan}")
+
+
+@pytest.mark.parametrize("quant", [True, False])
+def test_prompt_piece_mixed_with_decodes(quant, cuda_device):
+    new = [200] + [1] * 9 + [0] + [17]
+    total = [900, 1, 2, 127, 128, 129, 500, 16, 17, 1300, 40, 17]
+    b = make_batch(500, new, total, hq=16, hkv=4, quant=quant, poison=np.nan)
+    for plan in (False, True):
+        out, lse, scale = _attend(b, cuda_device, True, plan=plan)
+        assert_attention(out, lse, b, scale, True, f"mixed plan{plan}")
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("scale", [0.0, -0.05, 1.5])
+def test_scales_zero_negative_and_sharp(quant, scale, cuda_device):
+    b = make_batch(600, [40, 3], [300, 260], quant=quant, spread=0.1)
+    out, lse, _ = _attend(b, cuda_device, True, scale=scale)
+    assert_attention(out, lse, b, scale, True, f"scale {scale}")
+
+
+@pytest.mark.parametrize("quant", [True, False])
+def test_rescales_when_late_keys_tower_over_early_ones(quant, cuda_device):
+    b = make_batch(610, [40, 1], [700, 900], spread=0.0)
+    flat = b.k.reshape(-1, b.hkv, b.d)
+    for s, t in enumerate(b.total):
+        for lo in range(0, t, 130):
+            flat[b.slots(s, lo, min(lo + 3, t))] *= 1.0 + lo / 40.0
+    b.k = syn.round_dtype(b.k.astype(np.float32), "bf16").astype(np.float64)
+    if quant:
+        b.quant = True
+        b.k_codes, b.k_scale = quantise64(b.k)
+        b.v_codes, b.v_scale = quantise64(b.v)
+        b.k, b.v = b.k_codes * b.k_scale[..., None], b.v_codes * b.v_scale[..., None]
+    out, lse, scale = _attend(b, cuda_device, True)
+    assert_attention(out, lse, b, scale, True, "late large keys")
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_a_later_tokens_bad_values_reach_no_earlier_query(quant, value, cuda_device):
+    """A non-finite K or V row of token j is seen by queries at positions >= j only."""
+    if quant and not np.isnan(value):
+        pytest.skip("e4m3 codes have no infinity")
+    b = make_batch(700, [60, 5], [200, 5], quant=quant)
+    for s, bad in ((0, 170), (1, 2)):
+        slot = int(b.slots(s, bad, bad + 1)[0])
+        for x in (b.v.reshape(-1, b.hkv, b.d),) + ((b.v_codes.reshape(-1, b.hkv, b.d),) if quant else ()):
+            x[slot, :, 3] = value
+        for x in (b.k.reshape(-1, b.hkv, b.d),) + ((b.k_codes.reshape(-1, b.hkv, b.d),) if quant else ()):
+            x[slot, :, 3] = np.nan
+    out, lse, scale = _attend(b, cuda_device, True)
+    clean = [i for s, (n, t, bad) in enumerate(zip(b.new, b.total, (170, 2)))
+             for i in range(int(b.cu[s]), int(b.cu[s]) + n) if t - n + i - int(b.cu[s]) < bad]
+    dirty = sorted(set(range(int(b.cu[-1]))) - set(clean))
+    good = make_batch(700, [60, 5], [200, 5], quant=quant)
+    from varlen_oracle import attention64
+
+    want, want_lse, _, _ = attention64(good, scale, True)
+    assert np.isfinite(out[clean]).all() and np.isfinite(lse[clean]).all()
+    assert np.abs(out[clean] - want[clean]).max() < 3e-2 and np.abs(lse[clean] - want_lse[clean]).max() < 1e-3
+    assert np.isnan(out[dirty]).all() and np.isnan(lse[dirty]).all()
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_a_bad_value_in_v_reaches_its_column_of_the_queries_that_see_it(value, cuda_device):
+    b = make_batch(710, [60, 5], [200, 5])
+    for s, bad in ((0, 170), (1, 2)):
+        b.v.reshape(-1, b.hkv, b.d)[int(b.slots(s, bad, bad + 1)[0]), :, 3] = value
+    out, lse, scale = _attend(b, cuda_device, True)
+    assert np.isfinite(lse).all()
+    for s, (n, t, bad) in enumerate(zip(b.new, b.total, (170, 2))):
+        for i in range(n):
+            row = out[int(b.cu[s]) + i]
+            assert np.isfinite(np.delete(row, 3, axis=1)).all()
+            seen = t - n + i >= bad
+            got = row[:, 3]
+            assert np.isfinite(got).all() if not seen else np.isnan(got).all() if np.isnan(value) else (got == value).all()
+
+
+@pytest.mark.parametrize("quant", [True, False])
+def test_padding_rows_strided_queries_int64_indices_and_out(quant, cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    b = make_batch(800, [9, 40], [100, 41], quant=quant)
+    t = b.device(cuda_device, torch.int64)
+    T = int(b.cu[-1])
+    fused = torch.zeros((T + 5, b.hq + 4, b.d), device=cuda_device, dtype=torch.bfloat16)
+    fused[:T, 2:2 + b.hq] = t["q"]
+    q = fused[:, 2:2 + b.hq]
+    out = torch.full((T + 5, b.hq, b.d), 9.0, device=cuda_device, dtype=torch.bfloat16)
+    scale = b.d ** -0.5
+    got, lse = fa.flash_attn_varlen_with_kvcache(q, t["kc"], t["vc"], t["cu"], t["lens"], t["table"], 40, causal=True,
+                                                 k_scales=t["ks"], v_scales=t["vs"], out=out, return_softmax_lse=True)
+    assert got is out
+    assert (host(out)[T:] == 9.0).all()
+    assert_attention(host(out)[:T], host(lse)[:T], b, scale, True, "strided")
+    odd = torch.zeros((T, b.hq, b.d + 1), device=cuda_device, dtype=torch.bfloat16)[:, :, 1:]
+    odd.copy_(t["q"])
+    again = fa.flash_attn_varlen_with_kvcache(odd, t["kc"], t["vc"], t["cu"], t["lens"], t["table"], 40, causal=True,
+                                              k_scales=t["ks"], v_scales=t["vs"])
+    assert torch.equal(again, out[:T])
+
+
+def test_results_do_not_change_from_call_to_call_nor_on_another_stream(cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    b = make_batch(900, [1, 64, 1, 2], [3000, 700, 129, 2500], quant=True)
+    t = b.device(cuda_device)
+    args = (t["q"], t["kc"], t["vc"], t["cu"], t["lens"], t["table"], 64)
+    kw = dict(causal=True, k_scales=t["ks"], v_scales=t["vs"])
+    first = fa.flash_attn_varlen_with_kvcache(*args, **kw)
+    for _ in range(3):
+        assert torch.equal(fa.flash_attn_varlen_with_kvcache(*args, **kw), first)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = fa.flash_attn_varlen_with_kvcache(*args, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, first)
+
+
+def test_replay_in_a_cuda_graph_follows_the_lengths(cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    b = make_batch(910, [1, 1, 1], [200, 33, 150], quant=True)
+    t = b.device(cuda_device)
+    run = lambda: fa.flash_attn_varlen_with_kvcache(t["q"], t["kc"], t["vc"], t["cu"], t["lens"], t["table"], 1,  # noqa: E731
+                                                    causal=True, k_scales=t["ks"], v_scales=t["vs"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    t["lens"].copy_(torch.tensor([100, 5, 150], dtype=torch.int32))
+    graph.replay()
+    b.total = [100, 5, 150]
+    assert_attention(host(out), None, b, b.d ** -0.5, True, "replay")
+
+
+def test_bad_pages_and_short_tables_are_flagged_not_read(cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+    from mxflashattn_b200 import _lib
+
+    b = make_batch(920, [4], [200], quant=True)
+    t = b.device(cuda_device)
+    kw = dict(k_scales=t["ks"], v_scales=t["vs"])
+    bad = t["table"].clone()
+    bad[0, 3] = 10_000
+    for table, lens, flag in ((bad, t["lens"], _lib.FLAG_PAGE_OUT_OF_RANGE),
+                              (t["table"][:, :5].contiguous(), t["lens"], _lib.FLAG_TABLE_TOO_NARROW)):
+        fa.flash_attn_varlen_with_kvcache(t["q"], t["kc"], t["vc"], t["cu"], lens, table, 4, causal=True, **kw)
+        torch.cuda.synchronize()
+        assert _lib.read_error_flags() & flag
+    x = torch.zeros((4, b.hkv, b.d), device=cuda_device, dtype=torch.bfloat16)
+    before = t["kc"].view(torch.uint8).clone()
+    fa.kvcache_append_varlen(x, x, t["kc"], t["vc"], t["cu"], torch.tensor([2], device=cuda_device), t["table"], **kw)
+    torch.cuda.synchronize()
+    assert _lib.read_error_flags() & _lib.FLAG_TABLE_TOO_NARROW
+    changed = (t["kc"].view(torch.uint8) != before).any(dim=-1).any(dim=-1).sum().item()
+    assert changed <= 2
