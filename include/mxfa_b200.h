@@ -40,7 +40,8 @@ extern "C" {
 #define MXFA_FLAG_TABLE_TOO_NARROW 0x2u   /* sequence longer than block_table width * page size */
 #define MXFA_FLAG_WAIT_TIMEOUT 0x4u       /* a bounded pipeline wait gave up */
 #define MXFA_FLAG_DENSE_OVERFLOW 0x8u     /* dense-cache append past the cache capacity */
-#define MXFA_FLAG_BAD_ORDER 0x10u         /* a length order entry outside [0, B) (that row ran its own index) */
+#define MXFA_FLAG_BAD_ORDER 0x10u         /* a length order entry outside [0, B) (that row ran its own index), or
+                                           * query offsets that decrease (the chunk plan is then empty) */
 
 /* Library identity.  No reference counterpart (the reference's pybind
  * modules expose no version); used by the ctypes loader. */
@@ -387,15 +388,35 @@ int mxfa_kvcache_gather_varlen_launch(const void* k_cache, const void* v_cache, 
                                       void* v_out, int total, int B, int HKV, int D, int PS, int BTW,
                                       int num_pages, int bf16, void* stream);
 
+/* The division of a step's attention into items, written to `plan` (device,
+ * mxfa_chunk_plan_bytes, 16-byte aligned) from the lengths, once per step
+ * for every layer.  A plan belongs to the lengths, head counts and causal
+ * flag it was made for. */
+size_t mxfa_chunk_plan_bytes(int total_q, int B, int HQ, int HKV);
+int mxfa_kvcache_chunk_plan_launch(const int32_t* cu_seqlens_q, const int32_t* seqlens, void* plan,
+                                   size_t plan_bytes, int total_q, int B, int HQ, int HKV, int causal,
+                                   void* stream);
+
+/* Workspace of one attention call (partial states of split tiles; may be
+ * shared by launches ordered on one stream), and its counters, which the
+ * caller zeroes once and every launch leaves zero. */
+size_t mxfa_chunk_workspace_bytes(int HKV, int D);
+size_t mxfa_chunk_counter_bytes(int HKV);
+
 /* Attention of packed queries q [T, HQ, D] (strides in elements, multiples
  * of 8) over each sequence's seqlens[b] cached tokens; causal: the query at
  * position p sees keys 0 .. p.  out [T, HQ, D]; lse optional f32 [T, HQ]
- * (natural log).  A row that sees no key outputs 0 and LSE -inf. */
+ * (natural log).  A row that sees no key outputs 0 and LSE -inf.  Plan,
+ * workspace and counters are needed for page sizes that are multiples of 8
+ * and up to 128 query heads per KV head (the tensor-core path); other calls
+ * run a slower row kernel and ignore them. */
 int mxfa_kvcache_varlen_attention_launch(const void* q, const void* k_cache, const void* v_cache,
                                          const void* k_scales, const void* v_scales,
                                          const int32_t* cu_seqlens_q, const int32_t* seqlens,
-                                         const int32_t* block_table, void* out, float* lse, int total_q,
-                                         int B, int HQ, int HKV, int D, int PS, int BTW, int num_pages,
+                                         const int32_t* block_table, const void* plan, size_t plan_bytes,
+                                         void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                         unsigned* counters, int total_q, int B, int HQ, int HKV, int D,
+                                         int PS, int BTW, int num_pages,
                                          size_t q_token_stride, size_t q_head_stride, int causal,
                                          int bf16, float scale, void* stream);
 

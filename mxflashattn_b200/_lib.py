@@ -83,8 +83,12 @@ SIGNATURES = {
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _sz, _sz, _sz, _sz, _i, _vp]),
     "mxfa_kvcache_gather_varlen_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "mxfa_chunk_plan_bytes": (_sz, [_i, _i, _i, _i]),
+    "mxfa_chunk_workspace_bytes": (_sz, [_i, _i]),
+    "mxfa_chunk_counter_bytes": (_sz, [_i]),
+    "mxfa_kvcache_chunk_plan_launch": (_i, [_vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _vp]),
     "mxfa_kvcache_varlen_attention_launch": (
-        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _sz, _sz, _i, _i, _f,
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _sz, _sz, _i, _i, _f,
              _vp]),
     "mxfa_varlen_fwd_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp]),

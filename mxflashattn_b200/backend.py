@@ -388,7 +388,7 @@ def kvcache_attention_packed(q, k_cache, v_cache, cache_seqlens, block_table, so
 def _rows16(t):
     """``t`` with unit stride along D and 16-byte rows: itself, or a packed copy."""
     s = t.stride()
-    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0:
+    if s[2] == 1 and s[0] and s[1] and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
@@ -420,6 +420,39 @@ def kvcache_gather_varlen(k_cache, v_cache, cu_seqlens, cache_seqlens, block_tab
     _lib.check(rc, "mxfa_kvcache_gather_varlen_launch")
 
 
+_CHUNK_SIZES: dict[tuple, tuple[int, int]] = {}
+
+
+def _chunk_sizes(kv_heads: int, head_dim: int) -> tuple[int, int]:
+    """(workspace bytes, counter bytes) of the tiled attention on the current device (cached)."""
+    key = (torch.cuda.current_device() if (_CUDA_OK or torch.cuda.is_available()) else -1, kv_heads, head_dim)
+    sizes = _CHUNK_SIZES.get(key)
+    if sizes is None:
+        lib = _L()
+        sizes = _CHUNK_SIZES[key] = (int(lib.mxfa_chunk_workspace_bytes(kv_heads, head_dim)),
+                                     int(lib.mxfa_chunk_counter_bytes(kv_heads)))
+    return sizes
+
+
+_MAX_GROUP = 128  # query heads of one KV head that the tiled kernel takes
+
+
+def kvcache_chunk_plan(cu_seqlens_q, cache_seqlens, total_q: int, q_heads: int, kv_heads: int, causal: bool):
+    """The items of a step's ragged attention (int32, on the device), or None where no tiled call needs them."""
+    B = cache_seqlens.numel()
+    if total_q == 0 or B == 0 or q_heads // kv_heads > _MAX_GROUP:
+        return None
+    cu, seq = _i32(cu_seqlens_q), _i32(cache_seqlens)
+    lib = _L()
+    with _on(cu):
+        nbytes = int(lib.mxfa_chunk_plan_bytes(total_q, B, q_heads, kv_heads))
+        table = torch.empty((nbytes // 4,), device=cu.device, dtype=torch.int32)
+        rc = lib.mxfa_kvcache_chunk_plan_launch(cu.data_ptr(), seq.data_ptr(), table.data_ptr(), nbytes, total_q, B,
+                                                q_heads, kv_heads, int(causal), _stream(cu))
+    _lib.check(rc, "mxfa_kvcache_chunk_plan_launch")
+    return table
+
+
 def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q,
                                    max_seqlen_k, softmax_scale, causal, k_scales=None, v_scales=None, plan=None,
                                    out=None, return_lse: bool = False):
@@ -431,12 +464,22 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
         out = torch.empty((Tq, HQ, D), device=q.device, dtype=q.dtype)
     lse = torch.empty((Tq, HQ), device=q.device, dtype=torch.float32) if return_lse else None
     PS, HKV = k_cache.shape[1], k_cache.shape[2]
+    lib = _L()
     with _on(q):
-        rc = _L().mxfa_kvcache_varlen_attention_launch(
+        stream = _stream(q)
+        table = ws = counters = None
+        ws_bytes = 0
+        if Tq and seq.shape[0] and PS % 8 == 0 and HQ // HKV <= _MAX_GROUP:
+            table = kvcache_chunk_plan(cu, seq, Tq, HQ, HKV, causal) if plan is None else plan.table
+            ws_bytes, counter_bytes = _chunk_sizes(HKV, D)
+            ws = torch.empty((ws_bytes // 4,), device=q.device, dtype=torch.float32)
+            counters = split_counters(q.device, stream, counter_bytes)
+        rc = lib.mxfa_kvcache_varlen_attention_launch(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales),
-            cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), out.data_ptr(), _lib.ptr(lse), Tq, seq.shape[0], HQ, HKV,
-            D, PS, bt.shape[1], k_cache.shape[0], q.stride(0), q.stride(1), int(causal), _bf16(q),
-            float(softmax_scale), _stream(q))
+            cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), _lib.ptr(table), 0 if table is None else table.numel() * 4,
+            out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), ws_bytes, _lib.ptr(counters), Tq, seq.shape[0], HQ, HKV, D,
+            PS, bt.shape[1], k_cache.shape[0], q.stride(0), q.stride(1), int(causal), _bf16(q), float(softmax_scale),
+            stream)
     _lib.check(rc, "mxfa_kvcache_varlen_attention_launch")
     return (out, lse) if return_lse else out
 

@@ -19,7 +19,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB_NAME = "libmxfa_b200.so"
 LIB_PATH = os.path.join(PKG, LIB_NAME)
 SOURCES = ["capi.cu"]
-HEADERS = ["common.cuh", "decode.cuh", "paged_varlen.cuh", "prefill_sm100.cuh", "capi_varlen.cuh"]
+HEADERS = ["common.cuh", "decode.cuh", "paged_varlen.cuh", "prefill_sm100.cuh", "chunk_sm100.cuh",
+           "capi_varlen.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -18,6 +18,7 @@
 
 #include <cstdlib>
 
+#include "chunk_sm100.cuh"
 #include "decode.cuh"
 #include "paged_varlen.cuh"
 #include "prefill_sm100.cuh"

@@ -1,0 +1,904 @@
+// chunk_sm100.cuh -- attention of a ragged batch over a paged cache on the
+// 5th-generation tensor cores, and the plan that divides it.
+//
+// A tile is 128 query rows of one KV head: 128 / GQ tokens of one sequence
+// times the GQ query heads that share the head (row r = token r / GQ, head
+// r % GQ).  Packing heads with tokens reads each K/V row once per 128 query
+// rows whatever GQ is, fills the tile from 128 / GQ tokens on, and keeps the
+// causal diagonal of a tile 128 / GQ keys wide.
+//
+// An item is a tile and a range of 128-key tiles.  chunk_plan_kernel writes
+// the items of a step once (every layer uses them): tiles whose keys exceed
+// a CTA's fair share are split, and items go out longest first.  A split
+// tile's parts leave (O, m, l) in a workspace, and the part that finishes
+// last merges them in split order.
+//
+// The pipeline of one item is prefill_sm100.cuh's: score and P.V products
+// from two issuing threads, three score buffers and one O in tensor memory,
+// two softmax groups on alternating key tiles that share a running maximum.
+// What differs:
+//  - K and V come through the block table: one TMA box per page piece (the
+//    largest power of two that divides page size and tile, 8 rows at least),
+//    each lane of a producer warp resolving and issuing its own box.  A box
+//    lands as [8-row group][64-column block][8 rows][128 B], so any mix of
+//    boxes makes one tile with a constant 8-row group stride.
+//  - Keys that some row of the tile does not see have P = 0, but 0 * NaN is
+//    NaN: V rows past the last visible key are zeroed in shared memory, and a
+//    non-finite V element that only some rows see is zeroed and put into
+//    those rows' output at the end.
+//  - Quantised caches: a converter warpgroup turns the e4m3 tiles that TMA
+//    lands into 16-bit tiles, times each row's scale.  code * 2^k is exact in
+//    bf16, so the products are those of the cached values; fp16 saturates at
+//    65504 and rounds below 2^-14.
+#pragma once
+
+#include "paged_varlen.cuh"
+#include "prefill_sm100.cuh"
+
+namespace mxfa {
+
+// ------------------------------------------------------------------- plan
+
+struct ChunkItem {
+  int b, row0, ntok, pos0;     // sequence, packed row of the first token, tokens, position of the first token
+  int total, kt0, kt1, nsplit; // cached tokens, key tiles [kt0, kt1), parts of this tile
+  int split, part0, group, pad;
+};
+constexpr int kPlanHeader = 16;  // ints before the items: [0] items
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBuckets = 256;
+
+struct ChunkPlanParams {
+  const int* cu;
+  const int* seqlens;
+  int* plan;     // header, items, then B + 1 tile offsets
+  int T, B, tok; // tok: tokens per tile
+  int items_cap, parts_cap;
+  int share;     // CTA slots per KV head that the step's work is divided by
+  int min_part;  // key tiles a part holds at least
+  int causal;
+};
+
+__device__ __forceinline__ int chunk_tiles_of(const ChunkPlanParams& p, int b) {
+  const int lo = min(max(p.cu[b], 0), p.T), hi = min(max(p.cu[b + 1], lo), p.T);
+  return (hi - lo + p.tok - 1) / p.tok;
+}
+
+// Item fields of tile i (its sequence by binary search in the tile offsets),
+// and the key tiles it covers (at least one: a tile without keys still
+// writes its rows).
+__device__ __forceinline__ int chunk_tile(const ChunkPlanParams& p, const int* off, int i, ChunkItem& it) {
+  int lo = 0, hi = p.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (off[mid] <= i)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int b = lo;
+  const int q0 = min(max(p.cu[b], 0), p.T);
+  const int n = min(max(p.cu[b + 1], q0), p.T) - q0;
+  const int t0 = (i - off[b]) * p.tok;
+  it.b = b;
+  it.row0 = q0 + t0;
+  it.ntok = min(p.tok, n - t0);
+  it.total = max(p.seqlens[b], 0);
+  it.pos0 = it.total - n + t0;
+  it.pad = 0;
+  const int k_end = p.causal ? min(max(it.pos0 + it.ntok, 0), it.total) : it.total;
+  return max(1, (k_end + kTcKeys - 1) / kTcKeys);
+}
+
+// One block.  The work is counted in key tiles; parts hold at most
+// max(work / share, min_part) of them, which bounds the items by tiles +
+// share and the parts of split tiles by 2 * share.  Buckets of equal length
+// order the items; which item of a bucket comes first is left to the
+// atomics, since the order only schedules.
+__global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const ChunkPlanParams p) {
+  __shared__ int s_scan[kPlanThreads / 32];
+  __shared__ unsigned long long s_work;
+  __shared__ int s_max, s_parts, s_groups, s_hist[kPlanBuckets];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  ChunkItem* items = reinterpret_cast<ChunkItem*>(p.plan + kPlanHeader);
+  int* off = p.plan + kPlanHeader + p.items_cap * static_cast<int>(sizeof(ChunkItem) / 4);
+  if (tid == 0) {
+    s_work = 0;
+    s_max = s_parts = s_groups = 0;
+  }
+  for (int i = tid; i < kPlanBuckets; i += kPlanThreads) s_hist[i] = 0;
+  // tile offsets: block-wide exclusive scan over the sequences
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int n = b < p.B ? chunk_tiles_of(p, b) : 0;
+    int x = n;
+#pragma unroll
+    for (int sh = 1; sh < 32; sh <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, sh);
+      if (lane >= sh) x += y;
+    }
+    if (lane == 31) s_scan[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+      int w = s_scan[lane];
+#pragma unroll
+      for (int sh = 1; sh < 32; sh <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, w, sh);
+        if (lane >= sh) w += y;
+      }
+      s_scan[lane] = w;
+    }
+    __syncthreads();
+    if (b < p.B) off[b] = base + x - n + (warp > 0 ? s_scan[warp - 1] : 0);
+    base += s_scan[kPlanThreads / 32 - 1];
+    __syncthreads();
+  }
+  int tiles = base;
+  if (tiles > p.T / p.tok + min(p.B, p.T)) {  // more than any cu_seqlens that never decreases has
+    if (tid == 0) raise_flag(MXFA_FLAG_BAD_ORDER);
+    tiles = 0;
+  }
+  if (tid == 0) off[p.B] = tiles;
+  __syncthreads();  // off (global, this block's own writes) and the counters are visible
+
+  unsigned long long work = 0;
+  int longest = 0;
+  for (int i = tid; i < tiles; i += kPlanThreads) {
+    ChunkItem it;
+    const int n = chunk_tile(p, off, i, it);
+    work += n;
+    longest = max(longest, n);
+  }
+  atomicAdd(&s_work, work);
+  atomicMax(&s_max, longest);
+  __syncthreads();
+  const long long fair = (static_cast<long long>(s_work) + p.share - 1) / p.share;
+  const int limit = static_cast<int>(min(max(fair, static_cast<long long>(p.min_part)), 1ll << 30));
+  const int top = min(s_max, limit);
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int i = tid; i < tiles; i += kPlanThreads) {
+      ChunkItem it;
+      const int n = chunk_tile(p, off, i, it);
+      const int parts = (n + limit - 1) / limit;
+      const int per = (n + parts - 1) / parts;
+      const int bucket =
+          kPlanBuckets - 1 - static_cast<int>(static_cast<long long>(per) * (kPlanBuckets - 1) / max(top, 1));
+      if (pass == 0) {
+        atomicAdd(&s_hist[bucket], parts);
+        continue;
+      }
+      const int at = atomicAdd(&s_hist[bucket], parts);
+      it.nsplit = parts;
+      it.part0 = it.group = -1;
+      if (parts > 1) {
+        it.part0 = atomicAdd(&s_parts, parts);
+        it.group = atomicAdd(&s_groups, 1);
+      }
+      for (int s = 0; s < parts; ++s) {
+        it.split = s;
+        it.kt0 = min(s * per, n);
+        it.kt1 = min((s + 1) * per, n);
+        if (at + s < p.items_cap) items[at + s] = it;
+      }
+    }
+    __syncthreads();
+    if (pass == 0 && warp == 0) {  // exclusive scan of the buckets, longest first
+      int run = 0;
+      for (int b0 = 0; b0 < kPlanBuckets; b0 += 32) {
+        const int n = s_hist[b0 + lane];
+        int x = n;
+#pragma unroll
+        for (int sh = 1; sh < 32; sh <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, sh);
+          if (lane >= sh) x += y;
+        }
+        s_hist[b0 + lane] = run + x - n;
+        run += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (lane == 0) p.plan[0] = min(run, p.items_cap);
+    }
+    __syncthreads();
+  }
+}
+
+// --------------------------------------------------------------- attention
+
+struct ChunkParams {
+  const int* plan;
+  const int* bt;
+  void* out;   // [T, HQ, HD]
+  float* lse;  // optional [T, HQ]
+  const uint8_t* k_scales;  // [P, HKV, PS], quantised caches
+  const uint8_t* v_scales;
+  float* part_o;    // [HKV][parts_cap][128][HD]
+  float* part_ml;   // [HKV][parts_cap][128][2]
+  unsigned* counters;  // [HKV][parts_cap / 2 + 1], zero on entry and on exit
+  int parts_cap;
+  int HQ, HKV, GQ, PS, BTW, P;
+  int box;       // rows of one TMA box: divides PS and 128, a multiple of 8
+  int causal;
+  float scale_log2;
+};
+
+template <int HD, bool kQuant>
+struct ChunkCfg {
+  static constexpr int kThreads = kQuant ? 512 : 384;
+  static constexpr int kDBlk = HD / 64;
+  static constexpr int kStages = kQuant ? 2 : 3;
+  static constexpr int kGroupBytes = kDBlk * 1024;        // 8 rows of a K or V tile
+  static constexpr int kQBlk = 128 * 128;                 // one 64-column block of the Q tile
+  static constexpr int kTile = 128 * HD * 2;
+  static constexpr int kRawSlots = kQuant ? 3 : 0;
+  static constexpr int kRawTile = 128 * HD;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + kTile;
+  static constexpr int kV = kK + kStages * kTile;
+  static constexpr int kRaw = kV + kStages * kTile;
+  static constexpr int kMl = kQ;                          // epilogue exchange over Q once every product is done
+  static constexpr int kMPub = kRaw + kRawSlots * kRawTile;  // [2][128] running maxima
+  static constexpr int kScale = kMPub + 2 * kTcRows * 4;  // [3][K|V][128] row scales (quantised)
+  static constexpr int kBad = kScale + (kQuant ? 3 * 2 * 128 * 4 : 0);  // [HD] first keys with a non-finite V
+  static constexpr int kBar = kBad + HD * 4;
+  static constexpr int kNumBars = 40;
+  static constexpr int kSmemBytes = kBar + kNumBars * 8 + 32 + 1024;
+  static constexpr uint32_t kTmemCols = 512;
+  static constexpr uint32_t kTmemO = 3 * kTcKeys;
+  static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
+};
+
+struct ChunkBars {
+  uint64_t q_full, k_full[3], v_full[3], raw_full[3], raw_empty[3];
+  uint64_t s_full[3], p_full[3], pv_done[3];
+  uint64_t m_ready[2][4];
+  uint64_t v_ok[2];  // 16-bit caches: the guarded V tiles (the last two at most) are clean
+  uint64_t all_done;
+};
+static_assert(sizeof(ChunkBars) <= 40 * 8, "barrier block");
+
+// Pairs of 16-bit values with an exponent of all ones.
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite(uint4 v) {
+  constexpr uint32_t e = std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = std::is_same_v<T, __half> ? 0x04000400u : 0x00800080u;
+  // adding one unit of exponent carries into the (masked) sign exactly when all its bits are set
+  const uint32_t x = (((v.x & e) + one) | ((v.y & e) + one) | ((v.z & e) + one) | ((v.w & e) + one)) & 0x80008000u;
+  return x != 0;
+}
+
+// First keys (relative to the first guarded tile, under 256) whose V is NaN,
+// +inf and -inf in one column: three 10-bit fields, kNoKey where there is none.
+constexpr unsigned kNoKey = 0x3ffu;
+constexpr unsigned kNoBad = kNoKey | (kNoKey << 10) | (kNoKey << 20);
+
+// A 16-byte chunk of V of key `rel` (columns d0 .. d0+7): zero its
+// non-finite elements and note the key in their columns.
+template <typename T>
+__device__ __noinline__ uint4 strip_nonfinite(uint4 v, unsigned rel, unsigned* bad, volatile int* any_bad) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Elem<T>::unpack(w[i]);
+    const float x[2] = {f.x, f.y};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (!(fabsf(x[j]) < INFINITY)) {
+        const int at = 10 * (x[j] != x[j] ? 0 : x[j] > 0.f ? 1 : 2);
+        unsigned old = bad[2 * i + j];
+        while (((old >> at) & kNoKey) > rel) {
+          const unsigned seen = atomicCAS(&bad[2 * i + j], old, (old & ~(kNoKey << at)) | (rel << at));
+          if (seen == old) break;
+          old = seen;
+        }
+        *any_bad = 1;
+        w[i] &= j ? 0x0000ffffu : 0xffff0000u;
+      }
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Two floats to T, fp16 saturating at its largest value (NaN stays NaN).
+template <typename T>
+__device__ __forceinline__ uint32_t pack_sat(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  } else {
+    return Elem<T>::pack(lo, hi);
+  }
+}
+
+template <typename T, int HD, bool kQuant>
+__global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
+    chunk_attn_kernel(const ChunkParams p, const __grid_constant__ CUtensorMap tmq,
+                      const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
+  using Cfg = ChunkCfg<HD, kQuant>;
+  constexpr int NS = Cfg::kStages;
+  constexpr int NB = 3;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  ChunkBars* bars = reinterpret_cast<ChunkBars*>(sm + Cfg::kBar);
+  float* ml = reinterpret_cast<float*>(sm + Cfg::kMl);
+  float* mpub = reinterpret_cast<float*>(sm + Cfg::kMPub);
+  unsigned* bad = reinterpret_cast<unsigned*>(sm + Cfg::kBad);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Cfg::kBar + Cfg::kNumBars * 8);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* any_bad = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  int* s_last = reinterpret_cast<int*>(tmem_slot + 3);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = blockIdx.x;
+  if (static_cast<int>(blockIdx.y) >= p.plan[0]) return;
+  const ChunkItem it = reinterpret_cast<const ChunkItem*>(p.plan + kPlanHeader)[blockIdx.y];
+  // keys the block table can hold; a longer sequence is flagged and cut
+  const int k_lim = min(it.total, p.BTW * p.PS);
+  if (threadIdx.x == 0 && it.total > k_lim) raise_flag(MXFA_FLAG_TABLE_TOO_NARROW);
+  const int k_end = p.causal ? min(max(it.pos0 + it.ntok, 0), k_lim) : k_lim;    // keys some row sees
+  const int vis_first = p.causal ? min(max(it.pos0 + 1, 0), k_lim) : k_lim;      // keys every row sees
+  const int nkt = max(0, min(it.kt1, (k_end + kTcKeys - 1) / kTcKeys) - it.kt0);  // key tiles of this item
+  const int key_base = it.kt0 * kTcKeys;
+  const int nrows = it.ntok * p.GQ;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&bars->k_full[i], kQuant ? 4 : 1);
+      mbar_init(&bars->v_full[i], kQuant ? 4 : 1);
+      mbar_init(&bars->raw_full[i], 1);
+      mbar_init(&bars->raw_empty[i], 4);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], kTcGroupWarps);
+      mbar_init(&bars->pv_done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      for (int qd = 0; qd < 4; ++qd) mbar_init(&bars->m_ready[i][qd], 32);
+      mbar_init(&bars->v_ok[i], 1);
+    }
+    mbar_init(&bars->all_done, 1);
+    *abort = 0;
+    *any_bad = 0;
+    fence_mbar_init();
+  }
+  for (int i = threadIdx.x; i < HD; i += Cfg::kThreads) bad[i] = kNoBad;
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Row of the cache (in units of `unit` rows) of the box at position pos, or past the end of the cache
+  // (TMA fills zeros and reads nothing) when the table names no page for it.
+  auto box_row = [&](int pos, int unit) -> int {
+    const int page = pos / p.PS;
+    int phys = p.bt[static_cast<size_t>(it.b) * p.BTW + page];
+    if (phys < 0 || phys >= p.P) {
+      raise_flag(MXFA_FLAG_PAGE_OUT_OF_RANGE);
+      return static_cast<int>(static_cast<long long>(p.P) * p.PS / unit);
+    }
+    return static_cast<int>((static_cast<long long>(phys) * p.PS + (pos - page * p.PS)) / unit);
+  };
+  // first tile (of this item) that some row does not see in full
+  const int guard0 = max(0, vis_first / kTcKeys - it.kt0);
+  const int guard_key = key_base + guard0 * kTcKeys;
+
+  if (nkt > 0 && (warp == 0 || (warp == 3 && !kQuant))) {
+    // ------------------------------------------------------------ producers
+    // 16-bit: warp 0 loads Q and K, warp 3 loads V.  Quantised: warp 0 loads
+    // Q and the e4m3 tiles in the converter's order.  Lane i owns box i of a
+    // tile; the block-table entries of the next tile are read ahead.
+    const int nbox = kTcKeys / p.box;
+    const bool for_v = warp == 3;
+    if (lane == 0 && !for_v) {
+      prefetch_tensormap(&tmq);
+      mbar_arrive_expect_tx(&bars->q_full, Cfg::kDBlk * (kTcRows / p.GQ) * p.GQ * 128);
+#pragma unroll
+      for (int db = 0; db < Cfg::kDBlk; ++db)
+        tma_load_3d(sm + Cfg::kQ + db * Cfg::kQBlk, &tmq, &bars->q_full, db * 64, hk * p.GQ, it.row0);
+    }
+    auto row_of = [&](int t) -> int {  // this lane's box of tile t, -1 when there is none
+      const int pos = key_base + t * kTcKeys + lane * p.box;
+      return (t < nkt && lane < nbox && pos < k_lim) ? box_row(pos, kQuant ? 1 : 8) : -1;
+    };
+    bool ok = true;
+    int filled = 0;
+    if constexpr (!kQuant) {
+      int row = row_of(0);
+      for (int t = 0; t < nkt; ++t) {
+        const int next = row_of(t + 1);
+        const int st = t % NS, use = t / NS;
+        uint64_t* full = for_v ? &bars->v_full[st] : &bars->k_full[st];
+        const int n = __popc(__ballot_sync(0xffffffffu, row >= 0));
+        if (lane == 0) {
+          // K stage: free once S_{t-3} is done; V stage: once P.V_{t-3} is
+          if (use > 0) ok = tc_wait(for_v ? &bars->pv_done[st] : &bars->s_full[st], (use - 1) & 1, abort);
+          if (ok) mbar_arrive_expect_tx(full, n * p.box * HD * 2);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        filled = t + 1;
+        uint8_t* dst = sm + (for_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile + lane * (p.box / 8) * Cfg::kGroupBytes;
+        if (row >= 0) tma_load_5d(dst, for_v ? &tmv : &tmk, full, 0, hk, 0, 0, row);
+        row = next;
+      }
+      if (for_v) {
+        // V guard: keys [vis_first, end of tile) of the last tiles
+        for (int t = guard0; t < nkt && ok; ++t) {
+          ok = __all_sync(0xffffffffu, tc_wait(&bars->v_full[t % NS], (t / NS) & 1, abort));
+          if (!ok) break;
+          uint8_t* vt = sm + Cfg::kV + (t % NS) * Cfg::kTile;
+          const int key0 = key_base + t * kTcKeys;
+          constexpr int kCh = HD / 8;
+          for (int c = max(0, vis_first - key0) * kCh + lane; c < kTcKeys * kCh; c += 32) {
+            const int r = c / kCh, ch = c % kCh;
+            uint4* at = reinterpret_cast<uint4*>(vt + (r >> 3) * Cfg::kGroupBytes + (ch >> 3) * 1024 +
+                                                 swz128(r & 7, ch & 7));
+            if (key0 + r >= k_end) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else if (any_nonfinite<T>(*at)) {
+              *at = strip_nonfinite<T>(*at, key0 + r - guard_key, bad + ch * 8, any_bad);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->v_ok[t - guard0]);
+        }
+      }
+      if (*abort) {  // leave no copy in flight
+        if (lane == 0)
+          for (int t = max(0, filled - NS); t < filled; ++t)
+            mbar_wait(for_v ? &bars->v_full[t % NS] : &bars->k_full[t % NS], (t / NS) & 1);
+      }
+    } else {
+      // order: K_0, then per tile K_{t+1} and V_t
+      int u = 0;
+      auto emit = [&](int row, const CUtensorMap* map) {
+        const int slot = u % 3;
+        const int n = __popc(__ballot_sync(0xffffffffu, row >= 0));
+        if (lane == 0) {
+          if (u >= 3) ok = tc_wait(&bars->raw_empty[slot], (u / 3 - 1) & 1, abort);
+          if (ok) mbar_arrive_expect_tx(&bars->raw_full[slot], n * p.box * HD);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) return;
+        if (row >= 0)
+          tma_load_3d(sm + Cfg::kRaw + slot * Cfg::kRawTile + lane * p.box * HD, map, &bars->raw_full[slot], 0, hk, row);
+        filled = ++u;
+      };
+      int r0 = row_of(0), r1 = row_of(1);  // boxes of tiles t and t+1
+      emit(r0, &tmk);
+      for (int t = 0; t < nkt && ok; ++t) {
+        const int r2 = row_of(t + 2);
+        if (t + 1 < nkt) emit(r1, &tmk);
+        if (ok) emit(r0, &tmv);
+        r0 = r1;
+        r1 = r2;
+      }
+      if (*abort) {
+        if (lane == 0)
+          for (int u = max(0, filled - 3); u < filled; ++u) mbar_wait(&bars->raw_full[u % 3], (u / 3) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (nkt > 0 && (warp == 1 || warp == 2)) {
+    // ------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = umma_idesc<T>(kTcRows, kTcKeys, false);
+      constexpr uint32_t idesc_o = umma_idesc<T>(kTcRows, HD, true);
+      constexpr int kS = HD / 16;
+      constexpr int kP = kTcKeys / 16;
+      if (warp == 2) {
+        uint64_t qd[kS];
+        {
+          const uint64_t base = smem_desc(smem_u32(sm + Cfg::kQ), 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < kS; ++kk) qd[kk] = base + (kk >> 2) * (Cfg::kQBlk >> 4) + (kk & 3) * 2;
+        }
+        bool ok = tc_wait(&bars->q_full, 0, abort);
+        for (int t = 0; t < nkt && ok; ++t) {
+          const int buf = t % NB, ks = t % NS;
+          uint64_t kd[kS];
+          {
+            const uint64_t base = smem_desc(smem_u32(sm + Cfg::kK + ks * Cfg::kTile), 16, Cfg::kGroupBytes);
+#pragma unroll
+            for (int kk = 0; kk < kS; ++kk) kd[kk] = base + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2;
+          }
+          pin_regs(kd);
+          if (t >= NB && !tc_wait(&bars->pv_done[buf], ((t - NB) / NB) & 1, abort)) break;  // buffer free
+          if (!tc_wait(&bars->k_full[ks], (t / NS) & 1, abort)) break;
+          tc_fence_after();
+          umma_ss_chain(tmem + buf * kTcKeys, qd, kd, idesc_s);
+          umma_commit(&bars->s_full[buf]);
+        }
+      } else {
+        for (int j = 0; j < nkt; ++j) {
+          const int buf = j % NB, vs = j % NS;
+          uint64_t vd[kP];
+          uint32_t pa[kP];
+          {
+            const uint64_t vbase = smem_desc(smem_u32(sm + Cfg::kV + vs * Cfg::kTile), 1024, Cfg::kGroupBytes);
+#pragma unroll
+            for (int kk = 0; kk < kP; ++kk) {
+              vd[kk] = vbase + kk * (2 * Cfg::kGroupBytes >> 4);
+              pa[kk] = tmem + buf * kTcKeys + kk * 8;
+            }
+          }
+          pin_regs(vd);
+          pin_regs(pa);
+          if (!tc_wait(&bars->v_full[vs], (j / NS) & 1, abort)) break;
+          if (!kQuant && j >= guard0 && !tc_wait(&bars->v_ok[j - guard0], 0, abort)) break;
+          if (!tc_wait(&bars->p_full[buf], (j / NB) & 1, abort)) break;
+          tc_fence_after();
+          umma_ts_chain(tmem + Cfg::kTmemO, pa, vd, idesc_o, j > 0 ? 1u : 0u);
+          umma_commit(&bars->pv_done[buf]);
+          if (j == nkt - 1) umma_commit(&bars->all_done);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (kQuant && nkt > 0 && warp >= 12) {
+    // ------------------------------------------------------------ converter
+    // Four warps turn each e4m3 tile into a 16-bit tile: a thread takes the
+    // 16-byte chunk tid % (HD/16) of rows apart by 128 / (HD/16).  Scales of
+    // the next tile are read (through the table) while this one converts.
+    const int tid = threadIdx.x - 384;
+    float* sc = reinterpret_cast<float*>(sm + Cfg::kScale);  // [3][K|V][128]
+    auto page_of = [&](int t) -> int {  // physical page of key row tid of tile t, -1 when there is none
+      const int pos = key_base + t * kTcKeys + tid;
+      if (t >= nkt || pos >= k_lim) return -1;
+      const int phys = p.bt[static_cast<size_t>(it.b) * p.BTW + pos / p.PS];
+      return phys < 0 || phys >= p.P ? -1 : phys;
+    };
+    uint32_t kb = 127, vb = 127;
+    auto load_scales = [&](int t, int phys) {
+      kb = vb = 127;
+      if (phys >= 0) {
+        const int pos = key_base + t * kTcKeys + tid;
+        const size_t at = (static_cast<size_t>(phys) * p.HKV + hk) * p.PS + pos % p.PS;
+        kb = p.k_scales[at];
+        vb = p.v_scales[at];
+      }
+    };
+    auto store_scales = [&](int t) {
+      sc[(t % 3) * 256 + tid] = e8m0_to_float(kb);
+      sc[(t % 3) * 256 + 128 + tid] = e8m0_to_float(vb);
+    };
+    constexpr int kCh = HD / 16;
+    constexpr int kRowStep = 128 / kCh;
+    const int c = tid % kCh, r0 = tid / kCh;
+    auto convert = [&](int u, int t, bool is_v) -> bool {
+      const int slot = u % 3, st = t % NS;
+      // the 16-bit stage is free once the product that read it is done
+      bool ready = t < NS ||
+                   tc_wait(is_v ? &bars->pv_done[(t - NS) % NB] : &bars->s_full[(t - NS) % NB], ((t - NS) / NB) & 1, abort);
+      ready = ready && tc_wait(&bars->raw_full[slot], (u / 3) & 1, abort);
+      if (!__all_sync(0xffffffffu, ready)) return false;  // every lane leaves together
+      const uint8_t* raw = sm + Cfg::kRaw + slot * Cfg::kRawTile;
+      uint8_t* dst = sm + (is_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile;
+      const float* scale = sc + (t % 3) * 256 + (is_v ? 128 : 0);
+      const int key0 = key_base + t * kTcKeys;
+      const bool guard = is_v && t >= guard0;
+#pragma unroll 4
+      for (int i = 0; i < kCh; ++i) {
+        const int r = r0 + i * kRowStep;
+        const uint4 x = *reinterpret_cast<const uint4*>(raw + r * HD + c * 16);
+        const float s = scale[r];
+        float f[8];
+        uint4 lo, hi;
+        dequant8(make_uint2(x.x, x.y), s, f);
+        lo = make_uint4(pack_sat<T>(f[0], f[1]), pack_sat<T>(f[2], f[3]), pack_sat<T>(f[4], f[5]),
+                        pack_sat<T>(f[6], f[7]));
+        dequant8(make_uint2(x.z, x.w), s, f);
+        hi = make_uint4(pack_sat<T>(f[0], f[1]), pack_sat<T>(f[2], f[3]), pack_sat<T>(f[4], f[5]),
+                        pack_sat<T>(f[6], f[7]));
+        if (guard && key0 + r >= vis_first) {
+          if (key0 + r >= k_end) {
+            lo = hi = make_uint4(0, 0, 0, 0);
+          } else {
+            if (any_nonfinite<T>(lo)) lo = strip_nonfinite<T>(lo, key0 + r - guard_key, bad + c * 16, any_bad);
+            if (any_nonfinite<T>(hi)) hi = strip_nonfinite<T>(hi, key0 + r - guard_key, bad + c * 16 + 8, any_bad);
+          }
+        }
+        uint8_t* row = dst + (r >> 3) * Cfg::kGroupBytes + (c >> 2) * 1024;
+        const int ch = (c & 3) * 2;
+        *reinterpret_cast<uint4*>(row + swz128(r & 7, ch)) = lo;
+        *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + 1)) = hi;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(is_v ? &bars->v_full[st] : &bars->k_full[st]);
+        mbar_arrive(&bars->raw_empty[slot]);
+      }
+      return true;
+    };
+    load_scales(0, page_of(0));
+    store_scales(0);
+    int phys = page_of(1);
+    load_scales(1, phys);
+    phys = page_of(2);
+    named_barrier_sync(2, 128);
+    bool ok = convert(0, 0, false);
+    for (int t = 0; t < nkt; ++t) {
+      // scales of tile t+1 go in (their slot was last read for tile t-2), and the loads for t+2 go out
+      store_scales(t + 1);
+      load_scales(t + 2, phys);
+      phys = page_of(t + 3);
+      named_barrier_sync(2, 128);
+      if (ok && t + 1 < nkt) ok = convert(2 * t + 1, t + 1, false);
+      if (ok) ok = convert(t + 1 < nkt ? 2 * t + 2 : 2 * t + 1, t, true);
+      // every converter warp keeps the barrier's count until the loop ends, aborted or not
+    }
+  } else if (warp >= 4 && warp < 12) {
+    // ------------------------------------------------------------ softmax
+    const int g = (warp - 4) >> 2;
+    const int quad = warp & 3;
+    const int r = quad * 32 + lane;
+    const uint32_t lane_base = tmem + ((static_cast<uint32_t>(quad) * 32u) << 16);
+    const uint32_t o_base = lane_base + Cfg::kTmemO;
+    const bool warp_live = quad * 32 < nrows;  // some row of this warp exists
+    const bool row_live = r < nrows;
+    const int pos = it.pos0 + r / p.GQ;
+    // keys [0, vis_end) are visible; rows that do not exist see everything
+    const int vis_end = !row_live ? 0x7fffffff : p.causal ? min(k_lim, max(pos + 1, 0)) : k_lim;
+    const float sc = p.scale_log2;
+    float m_own = -INFINITY, l_own = 0.f;
+    bool ok = true;
+    for (int j = g; j < nkt; j += 2) {
+      const int buf = j % NB;
+      if (!__all_sync(0xffffffffu, tc_wait(&bars->s_full[buf], (j / NB) & 1, abort))) {
+        ok = false;
+        break;
+      }
+      if (!warp_live) {  // P of rows that do not exist is never read back
+        if (lane == 0) mbar_arrive(&bars->p_full[buf]);
+        continue;
+      }
+      tc_fence_after();
+      const uint32_t sbuf = lane_base + buf * kTcKeys;
+      const int key0 = key_base + j * kTcKeys;
+      const bool all_full = __all_sync(0xffffffffu, key0 + kTcKeys <= vis_end);
+      const bool pos_scale = sc >= 0.f;
+      const float ext0 = pos_scale ? -INFINITY : INFINITY;
+      float ext = ext0;
+      uint32_t ra[32], rb[32];
+      if (all_full) {
+        float e[4] = {ext0, ext0, ext0, ext0};
+        tmem_ld32_async(sbuf, ra);
+        tmem_wait_ld(ra);
+        tmem_ld32_async(sbuf + 32, rb);
+        ext_chunk32(ra, pos_scale, e);
+        tmem_wait_ld(rb);
+        tmem_ld32_async(sbuf + 64, ra);
+        ext_chunk32(rb, pos_scale, e);
+        tmem_wait_ld(ra);
+        tmem_ld32_async(sbuf + 96, rb);
+        ext_chunk32(ra, pos_scale, e);
+        tmem_wait_ld(rb);
+        tmem_ld32_async(sbuf, ra);
+        ext_chunk32(rb, pos_scale, e);
+        ext = pos_scale ? fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) : fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < kTcKeys; c += 16) {
+          uint32_t raw[16];
+          tmem_ld16(sbuf + c, raw);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float v = __uint_as_float(raw[i]);
+            const bool vis = key0 + c + i < vis_end;
+            ext = vis ? (pos_scale ? fmaxf(ext, v) : fminf(ext, v)) : ext;
+          }
+        }
+      }
+      const float mx = (ext == INFINITY || ext == -INFINITY) ? -INFINITY : ext * sc;
+      float m_in = -INFINITY;
+      if (j > 0) {
+        const int pj = j - 1;
+        if (!__all_sync(0xffffffffu, tc_wait(&bars->m_ready[pj & 1][quad], (pj >> 1) & 1, abort))) {
+          ok = false;
+          break;
+        }
+        m_in = mpub[(pj & 1) * kTcRows + r];
+      }
+      const float m_j = mx > m_in + kRescaleThreshold ? mx : m_in;
+      mpub[(j & 1) * kTcRows + r] = m_j;
+      mbar_arrive(&bars->m_ready[j & 1][quad]);
+      if (m_j != m_own) {
+        l_own *= fast_exp2(m_own - m_j);
+        m_own = m_j;
+      }
+      const bool grow = j > 0 && m_j != m_in;
+      if (__any_sync(0xffffffffu, grow)) {
+        const int pj = j - 1;
+        if (!__all_sync(0xffffffffu, tc_wait(&bars->pv_done[pj % NB], (pj / NB) & 1, abort))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const float alpha = grow ? fast_exp2(m_in - m_j) : 1.f;
+        if (all_full) tmem_wait_ld(ra);  // the first chunk's load must not stay open across the ones below
+#pragma unroll
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_base + c, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(o_base + c, o);
+        }
+      }
+      float rs = 0.f;
+      const float neg_m = -m_j;
+      if (all_full) {
+        const uint64_t sc2 = f2_pack(sc, sc), nm2 = f2_pack(neg_m, neg_m);
+        uint64_t acc0 = 0, acc1 = 0;
+        uint32_t pk3[16], pka[16], pkb[16];
+        exp2_chunk32<T>(rb, sc2, nm2, acc0, acc1, pk3);
+        tmem_wait_ld(ra);
+        tmem_ld32_async(sbuf + 32, rb);
+        exp2_chunk32<T>(ra, sc2, nm2, acc0, acc1, pka);
+        tmem_st16_async(sbuf, pka);
+        tmem_wait_ld(rb);
+        tmem_ld32_async(sbuf + 64, ra);
+        exp2_chunk32<T>(rb, sc2, nm2, acc0, acc1, pkb);
+        tmem_st16_async(sbuf + 16, pkb);
+        tmem_st16_async(sbuf + 48, pk3);
+        tmem_wait_ld(ra);
+        tmem_wait_st();
+        exp2_chunk32<T>(ra, sc2, nm2, acc0, acc1, pka);
+        tmem_st16_async(sbuf + 32, pka);
+        tmem_wait_st();
+        float a, bb;
+        f2_unpack(f2_add(acc0, acc1), a, bb);
+        rs = a + bb;
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < kTcKeys; c += 16) {
+          uint32_t raw[16];
+          tmem_ld16(sbuf + c, raw);
+          uint32_t packed[8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const bool v0 = key0 + c + i < vis_end;
+            const bool v1 = key0 + c + i + 1 < vis_end;
+            const float p0 = v0 ? fast_exp2(fmaf(__uint_as_float(raw[i]), sc, neg_m)) : 0.f;
+            const float p1 = v1 ? fast_exp2(fmaf(__uint_as_float(raw[i + 1]), sc, neg_m)) : 0.f;
+            rs += p0 + p1;
+            packed[i >> 1] = Elem<T>::pack(p0, p1);
+          }
+          tmem_st8(sbuf + (c >> 1), packed);
+        }
+      }
+      l_own += rs;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->p_full[buf]);
+    }
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");  // a load left in flight by an aborted tile
+
+    // ---------------------------------------------------------- merge + store
+    const bool done_ok =
+        nkt == 0 || __all_sync(0xffffffffu, ok && tc_wait(&bars->all_done, 0, abort));
+    fence_proxy_async_smem();
+    ml[(g * 2) * kTcRows + r] = m_own;
+    ml[(g * 2 + 1) * kTcRows + r] = l_own;
+    named_barrier_sync(1, 256);
+    tc_fence_after();
+    const float m0 = ml[r], m1 = ml[2 * kTcRows + r];
+    const float M = fmaxf(m0, m1);
+    // a sum at maximum -inf is 0, or NaN when every score it saw was
+    float L = ml[kTcRows + r] * (m0 == -INFINITY ? 1.f : fast_exp2(m0 - M));
+    L += ml[3 * kTcRows + r] * (m1 == -INFINITY ? 1.f : fast_exp2(m1 - M));
+    const bool split = it.nsplit > 1;
+    const float inv = split ? 1.f : (L != 0.f ? 1.f / L : 0.f);
+    const int head = hk * p.GQ + r % p.GQ;
+    const size_t R = static_cast<size_t>(it.row0 + r / p.GQ) * p.HQ + head;
+    const size_t prow = (static_cast<size_t>(hk) * p.parts_cap + it.part0 + it.split) * kTcRows + r;
+    T* orow = static_cast<T*>(p.out) + R * HD;
+    if (warp_live && done_ok) {
+      const bool patch = *any_bad != 0;
+      for (int c = g * 32; c < HD; c += 64) {
+        uint32_t o[32];
+        if (nkt > 0)
+          tmem_ld32(o_base + c, o);
+        else
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        if (patch) {
+          // non-finite V elements taken out of the products go into the rows that see their key
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const unsigned b3 = bad[c + i];
+            const int seen = vis_end - guard_key;  // relative keys below it are visible
+            const int kn = b3 & kNoKey, kp = (b3 >> 10) & kNoKey, km = (b3 >> 20) & kNoKey;
+            const bool n = kn != kNoKey && kn < seen, pi = kp != kNoKey && kp < seen, mi = km != kNoKey && km < seen;
+            if (n || (pi && mi))
+              o[i] = 0x7fffffffu;
+            else if (pi || mi)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) + (pi ? INFINITY : -INFINITY));
+          }
+        }
+        if (row_live && split) {
+          float* dst = p.part_o + prow * HD + c;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else if (row_live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 v;
+            v.x = Elem<T>::pack(__uint_as_float(o[i + 0]) * inv, __uint_as_float(o[i + 1]) * inv);
+            v.y = Elem<T>::pack(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+            v.z = Elem<T>::pack(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+            v.w = Elem<T>::pack(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+            *reinterpret_cast<uint4*>(orow + c + i) = v;
+          }
+        }
+        __syncwarp();
+      }
+    }
+    if (g == 0 && row_live && done_ok) {
+      if (split)
+        *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(M, L);
+      else if (p.lse != nullptr)
+        p.lse[R] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+    }
+    if (split) {
+      // publish this part; the last one of the tile merges them all, in split order
+      __threadfence();
+      named_barrier_sync(1, 256);
+      unsigned* counter = p.counters + static_cast<size_t>(hk) * (p.parts_cap / 2 + 1) + it.group;
+      const int tid = threadIdx.x - 128;
+      if (tid == 0) *s_last = atomicAdd(counter, 1u) == static_cast<unsigned>(it.nsplit) - 1u;
+      named_barrier_sync(1, 256);
+      if (*s_last) {
+        __threadfence();
+        const size_t first = (static_cast<size_t>(hk) * p.parts_cap + it.part0) * kTcRows;
+        constexpr int kQuads = HD / 4;
+        for (int idx = tid; idx < nrows * kQuads; idx += 256) {
+          const int rr = idx / kQuads, d4 = (idx % kQuads) * 4;
+          const float* po = p.part_o + (first + rr) * HD + d4;
+          const float* pm = p.part_ml + (first + rr) * 2;
+          float Mx = -INFINITY;
+          for (int z = 0; z < it.nsplit; ++z) Mx = fmaxf(Mx, __ldcg(pm + static_cast<size_t>(z) * kTcRows * 2));
+          float Ls = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int z = 0; z < it.nsplit; ++z) {
+            const float2 s = __ldcg(reinterpret_cast<const float2*>(pm + static_cast<size_t>(z) * kTcRows * 2));
+            if (s.x == -INFINITY && s.y == 0.f) continue;  // a part that saw no key
+            const float w = s.x == -INFINITY ? 1.f : fast_exp2(s.x - Mx);
+            const float4 o4 = __ldcg(reinterpret_cast<const float4*>(po + static_cast<size_t>(z) * kTcRows * HD));
+            Ls = fmaf(s.y, w, Ls);
+            acc.x = fmaf(o4.x, w, acc.x);
+            acc.y = fmaf(o4.y, w, acc.y);
+            acc.z = fmaf(o4.z, w, acc.z);
+            acc.w = fmaf(o4.w, w, acc.w);
+          }
+          const float iv = Ls != 0.f ? 1.f / Ls : 0.f;
+          const size_t RR = static_cast<size_t>(it.row0 + rr / p.GQ) * p.HQ + hk * p.GQ + rr % p.GQ;
+          uint2 v;
+          v.x = Elem<T>::pack(acc.x * iv, acc.y * iv);
+          v.y = Elem<T>::pack(acc.z * iv, acc.w * iv);
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + RR * HD + d4) = v;
+          if (d4 == 0 && p.lse != nullptr) p.lse[RR] = Ls != 0.f ? (Mx + log2f(Ls)) * kLn2 : -INFINITY;
+        }
+        if (tid == 0) *counter = 0u;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::kTmemCols);
+  }
+}
+
+}  // namespace mxfa

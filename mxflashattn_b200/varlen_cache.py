@@ -192,7 +192,10 @@ def kvcache_gather_varlen(
 
 @dataclass(frozen=True)
 class KvChunkPlan:
-    """How one step's ragged batch is divided (``kvcache_chunk_plan``); every layer of the step uses it."""
+    """How one step's ragged batch is divided (``kvcache_chunk_plan``); every layer of the step uses it.
+
+    ``table`` lists the items of the tiled kernel on the device.
+    """
 
     total_q: int
     batch: int
@@ -200,6 +203,7 @@ class KvChunkPlan:
     q_heads: int
     kv_heads: int
     causal: bool
+    table: torch.Tensor | None
 
 
 def kvcache_chunk_plan(
@@ -214,14 +218,22 @@ def kvcache_chunk_plan(
 ) -> KvChunkPlan:
     """The division of a step's ragged batch for ``flash_attn_varlen_with_kvcache(..., plan=)``.
 
+    One small kernel reads the lengths and writes the plan on the device.
     Call it once per step, after the lengths are final, and pass the result
-    to every layer; a call without a plan makes its own.
+    to every layer of that step; a call without a plan makes its own.  A plan
+    belongs to the lengths it was made from: after they change, make another.
     """
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cache_seqlens", cache_seqlens)):
+        _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor", TypeError)
+    _require(cu_seqlens_q.device.type == "cuda", "cu_seqlens_q must be on a CUDA device")
     batch = _validate_batch(cu_seqlens_q, cache_seqlens, None, cu_seqlens_q.device, "cu_seqlens_q")
     _require(int(total_q) >= 0 and int(max_seqlen_q) >= 0, "total_q and max_seqlen_q must be non-negative")
     _require(q_heads > 0 and kv_heads > 0 and q_heads % kv_heads == 0,
              "q heads must be a positive multiple of kv heads")
-    return KvChunkPlan(int(total_q), batch, int(max_seqlen_q), int(q_heads), int(kv_heads), bool(causal))
+    from . import backend
+
+    table = backend.kvcache_chunk_plan(cu_seqlens_q, cache_seqlens, int(total_q), q_heads, kv_heads, causal)
+    return KvChunkPlan(int(total_q), batch, int(max_seqlen_q), int(q_heads), int(kv_heads), bool(causal), table)
 
 
 def flash_attn_varlen_with_kvcache(

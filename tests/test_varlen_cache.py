@@ -151,6 +151,9 @@ def test_attention_refusals():
         _attend(a, max_seqlen_k=-1)
     with pytest.raises(ValueError, match="softmax_scale"):
         _attend(a, softmax_scale=float("nan"))
+    other = fa.KvChunkPlan(6, 2, 4, 16, 2, False, None)
+    with pytest.raises(ValueError, match="another batch"):
+        _attend(a, plan=other)
     with pytest.raises(ValueError, match="out must be"):
         _attend(a, out=torch.zeros(6, 8, 64, dtype=torch.bfloat16))
     with pytest.raises(TypeError, match="kvcache_chunk_plan"):
@@ -234,7 +237,8 @@ def _guard_args(name, **over):
                 cu_seqlens_q=4096, seqlens=4096, block_table=4096, k_out=4096, v_out=4096, out=4096, lse=None, total=4,
                 total_q=4, B=2, HQ=8, HKV=2, D=128, PS=16, BTW=4, num_pages=8, k_token_stride=256, k_head_stride=128,
                 v_token_stride=256, v_head_stride=128, q_token_stride=1024, q_head_stride=128, causal=1, bf16=1,
-                scale=0.1, stream=None, plan=None, plan_bytes=0, workspace=None, workspace_bytes=0, max_q=4, max_k=64)
+                scale=0.1, stream=None, plan=4096, plan_bytes=1 << 20, workspace=4096,
+                workspace_bytes=1 << 30, counters=4096)
     base.update(over)
     return [base[n] for n in NAMES[name]]
 
@@ -258,5 +262,27 @@ def test_entries_refuse_before_any_device_work(lib, name, over, status):
 
 def test_attention_entry_refuses_bad_queries(lib):
     name = "mxfa_kvcache_varlen_attention_launch"
-    for over in (dict(q=None), dict(out=None), dict(q=4104), dict(q_token_stride=1025), dict(HQ=7)):
+    for over in (dict(q=None), dict(out=None), dict(q=4104), dict(q_token_stride=1025), dict(HQ=7), dict(plan=None),
+                 dict(plan_bytes=64), dict(workspace=None), dict(workspace_bytes=64), dict(counters=None)):
         assert getattr(lib, name)(*_guard_args(name, **over)) == _lib.MXFA_ERR_INVALID, over
+
+
+def test_plan_entry_refuses_and_sizes_are_host_only(lib):
+    name = "mxfa_kvcache_chunk_plan_launch"
+    assert getattr(lib, name)(*_guard_args(name, HQ=7)) == _lib.MXFA_ERR_INVALID
+    assert getattr(lib, name)(*_guard_args(name, seqlens=None)) == _lib.MXFA_ERR_INVALID
+    assert getattr(lib, name)(*_guard_args(name, plan_bytes=32)) == _lib.MXFA_ERR_INVALID
+    assert getattr(lib, name)(*_guard_args(name, HQ=258)) == _lib.MXFA_ERR_UNSUPPORTED
+    assert getattr(lib, name)(*_guard_args(name, total_q=0, plan=None)) == _lib.MXFA_OK
+    small, large = lib.mxfa_chunk_plan_bytes(1, 1, 32, 8), lib.mxfa_chunk_plan_bytes(4096, 64, 32, 8)
+    assert 0 < small < large and lib.mxfa_chunk_plan_bytes(0, 1, 32, 8) == 0
+    assert lib.mxfa_chunk_workspace_bytes(8, 128) > lib.mxfa_chunk_workspace_bytes(8, 64) > 0
+    assert lib.mxfa_chunk_counter_bytes(8) > 0
+
+
+def test_plan_refuses_tensors_that_are_not_on_a_device():
+    a = _args()
+    with pytest.raises(ValueError, match="CUDA device"):
+        fa.kvcache_chunk_plan(a["cu"], a["lens"], 6, 4, q_heads=8, kv_heads=2)
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        fa.kvcache_chunk_plan(a["cu"], [1, 2], 6, 4, q_heads=8, kv_heads=2)
