@@ -26,7 +26,7 @@
 //    NaN: V rows past the last visible key are zeroed in shared memory, and a
 //    non-finite V element that only some rows see is zeroed and put into
 //    those rows' output at the end.
-//  - Quantised caches: a converter warpgroup turns the e4m3 tiles that TMA
+//  - Quantised caches: two converter warpgroups turn the e4m3 tiles that TMA
 //    lands into 16-bit tiles, times each row's scale.  code * 2^k is exact in
 //    bf16, so the products are those of the cached values; fp16 saturates at
 //    65504 and rounds below 2^-14.
@@ -225,7 +225,7 @@ struct ChunkParams {
 
 template <int HD, bool kQuant>
 struct ChunkCfg {
-  static constexpr int kThreads = kQuant ? 512 : 384;
+  static constexpr int kThreads = kQuant ? 640 : 384;
   static constexpr int kDBlk = HD / 64;
   static constexpr int kStages = kQuant ? 2 : 3;
   static constexpr int kGroupBytes = kDBlk * 1024;        // 8 rows of a K or V tile
@@ -239,8 +239,8 @@ struct ChunkCfg {
   static constexpr int kRaw = kV + kStages * kTile;
   static constexpr int kMl = kQ;                          // epilogue exchange over Q once every product is done
   static constexpr int kMPub = kRaw + kRawSlots * kRawTile;  // [2][128] running maxima
-  static constexpr int kScale = kMPub + 2 * kTcRows * 4;  // [3][K|V][128] row scales (quantised)
-  static constexpr int kBad = kScale + (kQuant ? 3 * 2 * 128 * 4 : 0);  // [HD] first keys with a non-finite V
+  static constexpr int kScale = kMPub + 2 * kTcRows * 4;  // [K|V][2][128] row scales (quantised)
+  static constexpr int kBad = kScale + (kQuant ? 2 * 2 * 128 * 4 : 0);  // [HD] first keys with a non-finite V
   static constexpr int kBar = kBad + HD * 4;
   static constexpr int kNumBars = 40;
   static constexpr int kSmemBytes = kBar + kNumBars * 8 + 32 + 1024;
@@ -312,6 +312,40 @@ __device__ __forceinline__ uint32_t pack_sat(float lo, float hi) {
   }
 }
 
+// Eight e4m3 codes times one scale, packed to T.
+template <typename T>
+__device__ __forceinline__ uint4 dequant8_pack(uint2 codes, float s) {
+  uint32_t h[4], w[4];
+  e4m3x4_to_f16x2x2(codes.x, h[0], h[1]);
+  e4m3x4_to_f16x2x2(codes.y, h[2], h[3]);
+  const uint64_t s2 = f2_pack(s, s);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = Elem<__half>::unpack(h[j]);
+    float a, b;
+    f2_unpack(f2_mul(f2_pack(f.x, f.y), s2), a, b);
+    w[j] = pack_sat<T>(a, b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Register shares of the quantised kernel's five warpgroups (launched with
+// 96 each): producers, issuers and converters give theirs to the softmax.
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+constexpr int kRegsIssue = 48, kRegsSoftmax = 152, kRegsConvert = 64;
+static_assert(kRegsIssue + 2 * kRegsSoftmax + 2 * kRegsConvert <= 5 * 96, "the launch's registers");
+
+__device__ __forceinline__ void named_barrier_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 template <typename T, int HD, bool kQuant>
 __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     chunk_attn_kernel(const ChunkParams p, const __grid_constant__ CUtensorMap tmq,
@@ -373,22 +407,29 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Row of the cache (in units of `unit` rows) of the box at position pos, or past the end of the cache
-  // (TMA fills zeros and reads nothing) when the table names no page for it.
-  auto box_row = [&](int pos, int unit) -> int {
-    const int page = pos / p.PS;
-    int phys = p.bt[static_cast<size_t>(it.b) * p.BTW + page];
+  // Physical page of position pos as the table has it (-1 past the keys).
+  // The value is not looked at before it is used, a tile later: a compare
+  // beside the load would wait out its latency.
+  auto page_entry = [&](int pos, bool want) -> int {
+    return want && pos < k_lim ? p.bt[static_cast<size_t>(it.b) * p.BTW + pos / p.PS] : -1;
+  };
+  // Cache row (in units of `unit` rows) of position pos on page phys; the
+  // first row past the cache, where TMA fills zeros and reads nothing, for
+  // an entry that names no page.
+  auto box_row = [&](int pos, int phys, int unit) -> int {
     if (phys < 0 || phys >= p.P) {
       raise_flag(MXFA_FLAG_PAGE_OUT_OF_RANGE);
       return static_cast<int>(static_cast<long long>(p.P) * p.PS / unit);
     }
-    return static_cast<int>((static_cast<long long>(phys) * p.PS + (pos - page * p.PS)) / unit);
+    return static_cast<int>((static_cast<long long>(phys) * p.PS + pos % p.PS) / unit);
   };
   // first tile (of this item) that some row does not see in full
   const int guard0 = max(0, vis_first / kTcKeys - it.kt0);
   const int guard_key = key_base + guard0 * kTcKeys;
 
-  if (nkt > 0 && (warp == 0 || (warp == 3 && !kQuant))) {
+  if (warp < 4) {
+   if constexpr (kQuant) regs_dec<kRegsIssue>();
+   if (nkt > 0 && (warp == 0 || (warp == 3 && !kQuant))) {
     // ------------------------------------------------------------ producers
     // 16-bit: warp 0 loads Q and K, warp 3 loads V.  Quantised: warp 0 loads
     // Q and the e4m3 tiles in the converter's order.  Lane i owns box i of a
@@ -402,19 +443,20 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       for (int db = 0; db < Cfg::kDBlk; ++db)
         tma_load_3d(sm + Cfg::kQ + db * Cfg::kQBlk, &tmq, &bars->q_full, db * 64, hk * p.GQ, it.row0);
     }
-    auto row_of = [&](int t) -> int {  // this lane's box of tile t, -1 when there is none
-      const int pos = key_base + t * kTcKeys + lane * p.box;
-      return (t < nkt && lane < nbox && pos < k_lim) ? box_row(pos, kQuant ? 1 : 8) : -1;
-    };
+    const int lane_pos = key_base + lane * p.box;  // this lane's box of tile 0
+    auto entry_of = [&](int t) { return page_entry(lane_pos + t * kTcKeys, t < nkt && lane < nbox); };
+    auto has_box = [&](int t) { return lane < nbox && lane_pos + t * kTcKeys < k_lim; };
     bool ok = true;
     int filled = 0;
     if constexpr (!kQuant) {
-      int row = row_of(0);
+      int entry = entry_of(0);
       for (int t = 0; t < nkt; ++t) {
-        const int next = row_of(t + 1);
+        const int next = entry_of(t + 1);
         const int st = t % NS, use = t / NS;
         uint64_t* full = for_v ? &bars->v_full[st] : &bars->k_full[st];
-        const int n = __popc(__ballot_sync(0xffffffffu, row >= 0));
+        const bool has = has_box(t);
+        const int n = __popc(__ballot_sync(0xffffffffu, has));
+        const int row = has ? box_row(lane_pos + t * kTcKeys, entry, 8) : 0;
         if (lane == 0) {
           // K stage: free once S_{t-3} is done; V stage: once P.V_{t-3} is
           if (use > 0) ok = tc_wait(for_v ? &bars->pv_done[st] : &bars->s_full[st], (use - 1) & 1, abort);
@@ -424,8 +466,8 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         if (!ok) break;
         filled = t + 1;
         uint8_t* dst = sm + (for_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile + lane * (p.box / 8) * Cfg::kGroupBytes;
-        if (row >= 0) tma_load_5d(dst, for_v ? &tmv : &tmk, full, 0, hk, 0, 0, row);
-        row = next;
+        if (has) tma_load_5d(dst, for_v ? &tmv : &tmk, full, 0, hk, 0, 0, row);
+        entry = next;
       }
       if (for_v) {
         // V guard: keys [vis_first, end of tile) of the last tiles
@@ -458,27 +500,32 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     } else {
       // order: K_0, then per tile K_{t+1} and V_t
       int u = 0;
-      auto emit = [&](int row, const CUtensorMap* map) {
+      auto emit = [&](int t, int row, const CUtensorMap* map) {
         const int slot = u % 3;
-        const int n = __popc(__ballot_sync(0xffffffffu, row >= 0));
+        const bool has = has_box(t);
+        const int n = __popc(__ballot_sync(0xffffffffu, has));
         if (lane == 0) {
           if (u >= 3) ok = tc_wait(&bars->raw_empty[slot], (u / 3 - 1) & 1, abort);
           if (ok) mbar_arrive_expect_tx(&bars->raw_full[slot], n * p.box * HD);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) return;
-        if (row >= 0)
+        if (has)
           tma_load_3d(sm + Cfg::kRaw + slot * Cfg::kRawTile + lane * p.box * HD, map, &bars->raw_full[slot], 0, hk, row);
         filled = ++u;
       };
-      int r0 = row_of(0), r1 = row_of(1);  // boxes of tiles t and t+1
-      emit(r0, &tmk);
+      auto row_of = [&](int t, int entry) { return has_box(t) ? box_row(lane_pos + t * kTcKeys, entry, 1) : 0; };
+      const int e0 = entry_of(0);
+      int e1 = entry_of(1);
+      int r0 = row_of(0, e0);
+      emit(0, r0, &tmk);
       for (int t = 0; t < nkt && ok; ++t) {
-        const int r2 = row_of(t + 2);
-        if (t + 1 < nkt) emit(r1, &tmk);
-        if (ok) emit(r0, &tmv);
+        const int e2 = entry_of(t + 2);
+        const int r1 = t + 1 < nkt ? row_of(t + 1, e1) : 0;
+        if (t + 1 < nkt) emit(t + 1, r1, &tmk);
+        if (ok) emit(t, r0, &tmv);
         r0 = r1;
-        r1 = r2;
+        e1 = e2;
       }
       if (*abort) {
         if (lane == 0)
@@ -486,7 +533,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (nkt > 0 && (warp == 1 || warp == 2)) {
+   } else if (nkt > 0 && (warp == 1 || warp == 2)) {
     // ------------------------------------------------------------ MMA issue
     if (lane == 0) {
       constexpr uint32_t idesc_s = umma_idesc<T>(kTcRows, kTcKeys, false);
@@ -542,100 +589,94 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (kQuant && nkt > 0 && warp >= 12) {
-    // ------------------------------------------------------------ converter
-    // Four warps turn each e4m3 tile into a 16-bit tile: a thread takes the
-    // 16-byte chunk tid % (HD/16) of rows apart by 128 / (HD/16).  Scales of
-    // the next tile are read (through the table) while this one converts.
-    const int tid = threadIdx.x - 384;
-    float* sc = reinterpret_cast<float*>(sm + Cfg::kScale);  // [3][K|V][128]
-    auto page_of = [&](int t) -> int {  // physical page of key row tid of tile t, -1 when there is none
-      const int pos = key_base + t * kTcKeys + tid;
-      if (t >= nkt || pos >= k_lim) return -1;
-      const int phys = p.bt[static_cast<size_t>(it.b) * p.BTW + pos / p.PS];
-      return phys < 0 || phys >= p.P ? -1 : phys;
-    };
-    uint32_t kb = 127, vb = 127;
-    auto load_scales = [&](int t, int phys) {
-      kb = vb = 127;
-      if (phys >= 0) {
-        const int pos = key_base + t * kTcKeys + tid;
-        const size_t at = (static_cast<size_t>(phys) * p.HKV + hk) * p.PS + pos % p.PS;
-        kb = p.k_scales[at];
-        vb = p.v_scales[at];
-      }
-    };
-    auto store_scales = [&](int t) {
-      sc[(t % 3) * 256 + tid] = e8m0_to_float(kb);
-      sc[(t % 3) * 256 + 128 + tid] = e8m0_to_float(vb);
+   }
+   if (warp == 1) {  // tensor memory goes back once the softmax warps have read it
+     named_barrier_sync(3, 256 + 32);
+     tc_fence_after();
+     tmem_dealloc(tmem, Cfg::kTmemCols);
+   }
+  } else if (kQuant && warp >= 12) {
+   if constexpr (kQuant) regs_dec<kRegsConvert>();
+   if (nkt > 0) {
+    // ----------------------------------------------------------- converters
+    // Warps 12-15 turn the e4m3 K tiles into 16-bit tiles, warps 16-19 the V
+    // tiles: a thread takes the 16-byte chunk tid % (HD/16) of rows apart by
+    // 128 / (HD/16).  The raw slot is free again once it is in registers, so
+    // all three slots are loads in flight nearly all the time.  Scales of the
+    // next tile are read (through the table) while this one converts.
+    const bool is_v = warp >= 16;
+    const int tid = (threadIdx.x - 384) & 127;
+    float* sc = reinterpret_cast<float*>(sm + Cfg::kScale) + (is_v ? 256 : 0);  // [2][128]
+    const uint8_t* scales = is_v ? p.v_scales : p.k_scales;
+    const int row_pos = key_base + tid;  // the key whose scale this thread reads, tile 0
+    auto entry_of = [&](int t) { return page_entry(row_pos + t * kTcKeys, t < nkt); };
+    auto scale_of = [&](int t, int phys) -> uint32_t {
+      if (phys < 0 || phys >= p.P) return 127;
+      return scales[(static_cast<size_t>(phys) * p.HKV + hk) * p.PS + (row_pos + t * kTcKeys) % p.PS];
     };
     constexpr int kCh = HD / 16;
     constexpr int kRowStep = 128 / kCh;
     const int c = tid % kCh, r0 = tid / kCh;
-    auto convert = [&](int u, int t, bool is_v) -> bool {
+    int entry = entry_of(0);
+    uint32_t byte = scale_of(0, entry);
+    entry = entry_of(1);
+    for (int t = 0; t < nkt; ++t) {
+      float* sct = sc + (t & 1) * 128;
+      sct[tid] = e8m0_to_float(byte);
+      byte = scale_of(t + 1, entry);
+      entry = entry_of(t + 2);
+      named_barrier_sync(is_v ? 4 : 2, 128);  // also: every thread is done with the scales of tile t-2's slot
+      // position in the producer's order: K_0, then K_{t+1}, V_t
+      const int u = is_v ? (t + 1 < nkt ? 2 * t + 2 : 2 * t + 1) : (t == 0 ? 0 : 2 * t - 1);
       const int slot = u % 3, st = t % NS;
-      // the 16-bit stage is free once the product that read it is done
-      bool ready = t < NS ||
-                   tc_wait(is_v ? &bars->pv_done[(t - NS) % NB] : &bars->s_full[(t - NS) % NB], ((t - NS) / NB) & 1, abort);
-      ready = ready && tc_wait(&bars->raw_full[slot], (u / 3) & 1, abort);
-      if (!__all_sync(0xffffffffu, ready)) return false;  // every lane leaves together
-      const uint8_t* raw = sm + Cfg::kRaw + slot * Cfg::kRawTile;
-      uint8_t* dst = sm + (is_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile;
-      const float* scale = sc + (t % 3) * 256 + (is_v ? 128 : 0);
       const int key0 = key_base + t * kTcKeys;
-      const bool guard = is_v && t >= guard0;
-#pragma unroll 4
+      bool ready = !*abort && tc_wait(&bars->raw_full[slot], (u / 3) & 1, abort);
+      uint4 x[kCh];
+      {
+        const uint8_t* raw = sm + Cfg::kRaw + slot * Cfg::kRawTile + r0 * HD + c * 16;
+#pragma unroll
+        for (int i = 0; i < kCh; ++i) x[i] = *reinterpret_cast<const uint4*>(raw + i * kRowStep * HD);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->raw_empty[slot]);
+      // the 16-bit stage is free once the product that read it is done
+      if (t >= NS)
+        ready = tc_wait(is_v ? &bars->pv_done[(t - NS) % NB] : &bars->s_full[(t - NS) % NB], ((t - NS) / NB) & 1, abort) &&
+                ready;
+      if (!__all_sync(0xffffffffu, ready)) continue;  // aborted: only the barrier above still counts
+      uint8_t* dst = sm + (is_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile + (c >> 2) * 1024;
+      const int ch = (c & 3) * 2, odd = c >> 2;
+#pragma unroll
       for (int i = 0; i < kCh; ++i) {
         const int r = r0 + i * kRowStep;
-        const uint4 x = *reinterpret_cast<const uint4*>(raw + r * HD + c * 16);
-        const float s = scale[r];
-        float f[8];
-        uint4 lo, hi;
-        dequant8(make_uint2(x.x, x.y), s, f);
-        lo = make_uint4(pack_sat<T>(f[0], f[1]), pack_sat<T>(f[2], f[3]), pack_sat<T>(f[4], f[5]),
-                        pack_sat<T>(f[6], f[7]));
-        dequant8(make_uint2(x.z, x.w), s, f);
-        hi = make_uint4(pack_sat<T>(f[0], f[1]), pack_sat<T>(f[2], f[3]), pack_sat<T>(f[4], f[5]),
-                        pack_sat<T>(f[6], f[7]));
-        if (guard && key0 + r >= vis_first) {
-          if (key0 + r >= k_end) {
-            lo = hi = make_uint4(0, 0, 0, 0);
-          } else {
-            if (any_nonfinite<T>(lo)) lo = strip_nonfinite<T>(lo, key0 + r - guard_key, bad + c * 16, any_bad);
-            if (any_nonfinite<T>(hi)) hi = strip_nonfinite<T>(hi, key0 + r - guard_key, bad + c * 16 + 8, any_bad);
-          }
+        const float s = sct[r];
+        const uint4 lo = dequant8_pack<T>(make_uint2(x[i].x, x[i].y), s);
+        const uint4 hi = dequant8_pack<T>(make_uint2(x[i].z, x[i].w), s);
+        // the two halves of a thread's 32 bytes swap their order in the
+        // second 64-column block, so eight lanes hit eight 16-byte banks
+        uint8_t* row = dst + (r >> 3) * Cfg::kGroupBytes;
+        *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + odd)) = odd ? hi : lo;
+        *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + 1 - odd)) = odd ? lo : hi;
+      }
+      if (is_v && t >= guard0) {  // V guard, each thread over its own chunks
+#pragma unroll 1
+        for (int i = 0; i < 2 * kCh; ++i) {
+          const int r = r0 + (i >> 1) * kRowStep, e = c * 2 + (i & 1), key = key0 + r;
+          if (key < vis_first) continue;
+          uint4* at = reinterpret_cast<uint4*>(dst + (r >> 3) * Cfg::kGroupBytes + swz128(r & 7, e & 7));
+          if (key >= k_end)
+            *at = make_uint4(0, 0, 0, 0);
+          else if (any_nonfinite<T>(*at))
+            *at = strip_nonfinite<T>(*at, key - guard_key, bad + e * 8, any_bad);
         }
-        uint8_t* row = dst + (r >> 3) * Cfg::kGroupBytes + (c >> 2) * 1024;
-        const int ch = (c & 3) * 2;
-        *reinterpret_cast<uint4*>(row + swz128(r & 7, ch)) = lo;
-        *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + 1)) = hi;
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(is_v ? &bars->v_full[st] : &bars->k_full[st]);
-        mbar_arrive(&bars->raw_empty[slot]);
-      }
-      return true;
-    };
-    load_scales(0, page_of(0));
-    store_scales(0);
-    int phys = page_of(1);
-    load_scales(1, phys);
-    phys = page_of(2);
-    named_barrier_sync(2, 128);
-    bool ok = convert(0, 0, false);
-    for (int t = 0; t < nkt; ++t) {
-      // scales of tile t+1 go in (their slot was last read for tile t-2), and the loads for t+2 go out
-      store_scales(t + 1);
-      load_scales(t + 2, phys);
-      phys = page_of(t + 3);
-      named_barrier_sync(2, 128);
-      if (ok && t + 1 < nkt) ok = convert(2 * t + 1, t + 1, false);
-      if (ok) ok = convert(t + 1 < nkt ? 2 * t + 2 : 2 * t + 1, t, true);
-      // every converter warp keeps the barrier's count until the loop ends, aborted or not
+      if (lane == 0) mbar_arrive(is_v ? &bars->v_full[st] : &bars->k_full[st]);
     }
-  } else if (warp >= 4 && warp < 12) {
+   }
+  } else {
+    if constexpr (kQuant) regs_inc<kRegsSoftmax>();
     // ------------------------------------------------------------ softmax
     const int g = (warp - 4) >> 2;
     const int quad = warp & 3;
@@ -849,6 +890,8 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       else if (p.lse != nullptr)
         p.lse[R] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
     }
+    tc_fence_before();
+    named_barrier_arrive(3, 256 + 32);  // tensor memory is read
     if (split) {
       // publish this part; the last one of the tile merges them all, in split order
       __threadfence();
@@ -891,13 +934,6 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         if (tid == 0) *counter = 0u;
       }
     }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, Cfg::kTmemCols);
   }
 }
 
