@@ -27,9 +27,10 @@
 //    non-finite V element that only some rows see is zeroed and put into
 //    those rows' output at the end.
 //  - Quantised caches: two converter warpgroups turn the e4m3 tiles that TMA
-//    lands into 16-bit tiles, times each row's scale.  code * 2^k is exact in
-//    bf16, so the products are those of the cached values; fp16 saturates at
-//    65504 and rounds below 2^-14.
+//    lands into f16 tiles, times each row's scale relative to the tile's
+//    largest (see kRefShift); the tile's own power of two goes into the softmax
+//    in 32 bits.  bf16 queries become f16 the same way, row by row.  f16 needs
+//    two instructions per pair of codes; widening to bf16 took five.
 #pragma once
 
 #include "paged_varlen.cuh"
@@ -239,8 +240,13 @@ struct ChunkCfg {
   static constexpr int kRaw = kV + kStages * kTile;
   static constexpr int kMl = kQ;                          // epilogue exchange over Q once every product is done
   static constexpr int kMPub = kRaw + kRawSlots * kRawTile;  // [2][128] running maxima
-  static constexpr int kScale = kMPub + 2 * kTcRows * 4;  // [K|V][2][128] row scales (quantised)
-  static constexpr int kBad = kScale + (kQuant ? 2 * 2 * 128 * 4 : 0);  // [HD] first keys with a non-finite V
+  // quantised: [K|V][2][128] row factors (f16 pairs), [K|V][2][4] warp maxima,
+  // [8] (K, V) exponents of a tile, [128] factors of the query rows
+  static constexpr int kScale = kMPub + 2 * kTcRows * 4;
+  static constexpr int kTileMax = kScale + (kQuant ? 2 * 2 * 128 * 4 : 0);
+  static constexpr int kTileExp = kTileMax + (kQuant ? 2 * 16 * 4 : 0);
+  static constexpr int kQScale = kTileExp + (kQuant ? 8 * 8 : 0);
+  static constexpr int kBad = kQScale + (kQuant ? 128 * 4 : 0);  // [HD] first keys with a non-finite V
   static constexpr int kBar = kBad + HD * 4;
   static constexpr int kNumBars = 40;
   static constexpr int kSmemBytes = kBar + kNumBars * 8 + 32 + 1024;
@@ -250,7 +256,7 @@ struct ChunkCfg {
 };
 
 struct ChunkBars {
-  uint64_t q_full, k_full[3], v_full[3], raw_full[3], raw_empty[3];
+  uint64_t q_full, q_ready, k_full[3], v_full[3], raw_full[3], raw_empty[3];
   uint64_t s_full[3], p_full[3], pv_done[3];
   uint64_t m_ready[2][4];
   uint64_t v_ok[2];  // 16-bit caches: the guarded V tiles (the last two at most) are clean
@@ -300,33 +306,32 @@ __device__ __noinline__ uint4 strip_nonfinite(uint4 v, unsigned rel, unsigned* b
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Two floats to T, fp16 saturating at its largest value (NaN stays NaN).
-template <typename T>
-__device__ __forceinline__ uint32_t pack_sat(float lo, float hi) {
-  if constexpr (std::is_same_v<T, __half>) {
-    uint32_t r;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-  } else {
-    return Elem<T>::pack(lo, hi);
-  }
-}
+// Exponent bytes (e8m0) of a tile are taken relative to the tile's largest
+// one, ref: a 16-bit operand is code * 2^(byte - ref + 7), at most 448 * 2^7
+// < 65504, and exact in f16 for rows down to 2^-22 of the tile's largest
+// (smaller ones round at 2^-25 of a value of 2^15.8).  2^(ref - 127 - 7)
+// multiplies the products in 32 bits.  ref is kept from 2^-60 up, so that
+// 2^-ref and sums of it stay in range; values under 2^-75 vanish.
+constexpr int kRefShift = 7, kRefMin = 127 - 60;
 
-// Eight e4m3 codes times one scale, packed to T.
-template <typename T>
-__device__ __forceinline__ uint4 dequant8_pack(uint2 codes, float s) {
-  uint32_t h[4], w[4];
-  e4m3x4_to_f16x2x2(codes.x, h[0], h[1]);
-  e4m3x4_to_f16x2x2(codes.y, h[2], h[3]);
-  const uint64_t s2 = f2_pack(s, s);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = Elem<__half>::unpack(h[j]);
-    float a, b;
-    f2_unpack(f2_mul(f2_pack(f.x, f.y), s2), a, b);
-    w[j] = pack_sat<T>(a, b);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+// 2^e as an f16 pair for e <= 15; under 2^-24 it is 0.
+__device__ __forceinline__ uint32_t pow2_f16x2(int e) {
+  const uint32_t h = e >= -14 ? static_cast<uint32_t>(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+  return h | (h << 16);
+}
+__device__ __forceinline__ float pow2_f32(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// Eight e4m3 codes times a row's factor, as f16.
+__device__ __forceinline__ uint4 codes_to_f16(uint2 codes, uint32_t factor) {
+  uint4 h;
+  e4m3x4_to_f16x2x2(codes.x, h.x, h.y);
+  e4m3x4_to_f16x2x2(codes.y, h.z, h.w);
+  return make_uint4(mul_f16x2(h.x, factor), mul_f16x2(h.y, factor), mul_f16x2(h.z, factor), mul_f16x2(h.w, factor));
 }
 
 // Register shares of the quantised kernel's five warpgroups (launched with
@@ -353,6 +358,8 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   using Cfg = ChunkCfg<HD, kQuant>;
   constexpr int NS = Cfg::kStages;
   constexpr int NB = 3;
+  using MT = std::conditional_t<kQuant, __half, T>;              // tensor-core operand type
+  constexpr bool kConvertQ = kQuant && !std::is_same_v<T, __half>;  // bf16 queries become f16 in shared memory
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   ChunkBars* bars = reinterpret_cast<ChunkBars*>(sm + Cfg::kBar);
@@ -379,6 +386,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_ready, 4);
     for (int i = 0; i < 3; ++i) {
       mbar_init(&bars->k_full[i], kQuant ? 4 : 1);
       mbar_init(&bars->v_full[i], kQuant ? 4 : 1);
@@ -536,8 +544,8 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
    } else if (nkt > 0 && (warp == 1 || warp == 2)) {
     // ------------------------------------------------------------ MMA issue
     if (lane == 0) {
-      constexpr uint32_t idesc_s = umma_idesc<T>(kTcRows, kTcKeys, false);
-      constexpr uint32_t idesc_o = umma_idesc<T>(kTcRows, HD, true);
+      constexpr uint32_t idesc_s = umma_idesc<MT>(kTcRows, kTcKeys, false);
+      constexpr uint32_t idesc_o = umma_idesc<MT>(kTcRows, HD, true);
       constexpr int kS = HD / 16;
       constexpr int kP = kTcKeys / 16;
       if (warp == 2) {
@@ -547,7 +555,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < kS; ++kk) qd[kk] = base + (kk >> 2) * (Cfg::kQBlk >> 4) + (kk & 3) * 2;
         }
-        bool ok = tc_wait(&bars->q_full, 0, abort);
+        bool ok = tc_wait(kConvertQ ? &bars->q_ready : &bars->q_full, 0, abort);
         for (int t = 0; t < nkt && ok; ++t) {
           const int buf = t % NB, ks = t % NS;
           uint64_t kd[kS];
@@ -606,26 +614,98 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     // next tile are read (through the table) while this one converts.
     const bool is_v = warp >= 16;
     const int tid = (threadIdx.x - 384) & 127;
-    float* sc = reinterpret_cast<float*>(sm + Cfg::kScale) + (is_v ? 256 : 0);  // [2][128]
-    const uint8_t* scales = is_v ? p.v_scales : p.k_scales;
-    const int row_pos = key_base + tid;  // the key whose scale this thread reads, tile 0
-    auto entry_of = [&](int t) { return page_entry(row_pos + t * kTcKeys, t < nkt); };
-    auto scale_of = [&](int t, int phys) -> uint32_t {
-      if (phys < 0 || phys >= p.P) return 127;
-      return scales[(static_cast<size_t>(phys) * p.HKV + hk) * p.PS + (row_pos + t * kTcKeys) % p.PS];
+    const int kvi = is_v ? 1 : 0;
+    uint32_t* factors = reinterpret_cast<uint32_t*>(sm + Cfg::kScale) + kvi * 256;  // [2][128]
+    int* wmax = reinterpret_cast<int*>(sm + Cfg::kTileMax) + kvi * 16;              // K warps: [2][K|V][4]; V: [2][4]
+    int2* tile_exp = reinterpret_cast<int2*>(sm + Cfg::kTileExp);
+    if (kConvertQ && is_v) {
+      // Query row tid to f16, times the power of two that brings its largest
+      // finite element to [2^14, 2^15): exact for elements down to 2^-28 of it.
+      if (__all_sync(0xffffffffu, tc_wait(&bars->q_full, 0, abort))) {
+        float top = 0.f;
+#pragma unroll 4
+        for (int ch = 0; ch < HD / 8; ++ch) {
+          const uint4 v = *reinterpret_cast<const uint4*>(sm + Cfg::kQ + (ch >> 3) * Cfg::kQBlk + swz128(tid, ch & 7));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = Elem<T>::unpack(w[i]);
+            top = fabsf(f.x) < INFINITY ? fmaxf(top, fabsf(f.x)) : top;
+            top = fabsf(f.y) < INFINITY ? fmaxf(top, fabsf(f.y)) : top;
+          }
+        }
+        const int e = top > 0.f ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -100) : 0;
+        const float down = pow2_f32(-e);
+#pragma unroll 4
+        for (int ch = 0; ch < HD / 8; ++ch) {
+          uint4* at = reinterpret_cast<uint4*>(sm + Cfg::kQ + (ch >> 3) * Cfg::kQBlk + swz128(tid, ch & 7));
+          const uint4 v = *at;
+          const float2 a = Elem<T>::unpack(v.x), b = Elem<T>::unpack(v.y), cc = Elem<T>::unpack(v.z),
+                       d = Elem<T>::unpack(v.w);
+          *at = make_uint4(Elem<__half>::pack(a.x * down, a.y * down), Elem<__half>::pack(b.x * down, b.y * down),
+                           Elem<__half>::pack(cc.x * down, cc.y * down), Elem<__half>::pack(d.x * down, d.y * down));
+        }
+        reinterpret_cast<float*>(sm + Cfg::kQScale)[tid] = pow2_f32(e);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->q_ready);
+      }
+    }
+    // This thread's key row: table entry and exponent bytes, read ahead and
+    // not looked at before their tile (addresses stay in range instead).
+    const int row_pos = key_base + tid;
+    auto has_row = [&](int t) { return t < nkt && row_pos + t * kTcKeys < k_lim; };
+    auto entry_of = [&](int t) {
+      return p.bt[static_cast<size_t>(it.b) * p.BTW + min((row_pos + t * kTcKeys) / p.PS, p.BTW - 1)];
+    };
+    auto page_ok = [&](int t, int phys) { return has_row(t) && phys >= 0 && phys < p.P; };
+    auto byte_at = [&](int t, int phys) {
+      return (static_cast<size_t>(page_ok(t, phys) ? phys : 0) * p.HKV + hk) * p.PS + (row_pos + t * kTcKeys) % p.PS;
+    };
+    const uint8_t* own = is_v ? p.v_scales : p.k_scales;
+    // The K warps also follow V's exponents: the softmax of a tile needs its
+    // V exponent long before the tile's V is converted.
+    struct Bytes {
+      uint32_t k, v;
+      bool ok;
+    };
+    auto bytes_of = [&](int t, int phys) -> Bytes {
+      const size_t at = byte_at(t, phys);
+      return {own[at], is_v ? 0u : p.v_scales[at], page_ok(t, phys)};
+    };
+    auto known = [](uint32_t byte, bool ok) { return ok && byte < 255 ? static_cast<int>(byte) : 0; };
+    auto put_max = [&](int t, const Bytes& x) {
+      const int mk = __reduce_max_sync(0xffffffffu, known(x.k, x.ok));
+      const int mv = __reduce_max_sync(0xffffffffu, known(x.v, x.ok));
+      if (lane == 0) {
+        wmax[(t & 1) * 8 + (warp & 3)] = mk;
+        if (!is_v) wmax[(t & 1) * 8 + 4 + (warp & 3)] = mv;
+      }
+    };
+    auto get_max = [&](int t, int which) {
+      const int* w = wmax + (t & 1) * 8 + which * 4;
+      return max(max(max(w[0], w[1]), max(w[2], w[3])), kRefMin);
     };
     constexpr int kCh = HD / 16;
     constexpr int kRowStep = 128 / kCh;
     const int c = tid % kCh, r0 = tid / kCh;
-    int entry = entry_of(0);
-    uint32_t byte = scale_of(0, entry);
-    entry = entry_of(1);
+    Bytes now = bytes_of(0, entry_of(0));
+    int entry1 = entry_of(1), entry2 = entry_of(2);
+    put_max(0, now);
+    named_barrier_sync(is_v ? 4 : 2, 128);
+    Bytes next = bytes_of(1, entry1);
     for (int t = 0; t < nkt; ++t) {
-      float* sct = sc + (t & 1) * 128;
-      sct[tid] = e8m0_to_float(byte);
-      byte = scale_of(t + 1, entry);
-      entry = entry_of(t + 2);
-      named_barrier_sync(is_v ? 4 : 2, 128);  // also: every thread is done with the scales of tile t-2's slot
+      // factors of tile t, maxima of tile t+1; bytes of t+2 go out
+      const int ref = get_max(t, 0);
+      const uint32_t mine = now.ok ? now.k : 127u;
+      factors[(t & 1) * 128 + tid] =
+          mine == 255 ? 0x7fff7fffu : pow2_f16x2(static_cast<int>(mine) - ref + kRefShift);
+      if (!is_v && tid == 0) tile_exp[t & 7] = make_int2(ref - 127 - kRefShift, get_max(t, 1) - 127 - kRefShift);
+      put_max(t + 1, next);
+      now = next;
+      next = bytes_of(t + 2, entry2);
+      entry2 = entry_of(t + 3);
+      named_barrier_sync(is_v ? 4 : 2, 128);  // also: every thread is done with tile t-2's factors and maxima
       // position in the producer's order: K_0, then K_{t+1}, V_t
       const int u = is_v ? (t + 1 < nkt ? 2 * t + 2 : 2 * t + 1) : (t == 0 ? 0 : 2 * t - 1);
       const int slot = u % 3, st = t % NS;
@@ -649,9 +729,9 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
 #pragma unroll
       for (int i = 0; i < kCh; ++i) {
         const int r = r0 + i * kRowStep;
-        const float s = sct[r];
-        const uint4 lo = dequant8_pack<T>(make_uint2(x[i].x, x[i].y), s);
-        const uint4 hi = dequant8_pack<T>(make_uint2(x[i].z, x[i].w), s);
+        const uint32_t f = factors[(t & 1) * 128 + r];
+        const uint4 lo = codes_to_f16(make_uint2(x[i].x, x[i].y), f);
+        const uint4 hi = codes_to_f16(make_uint2(x[i].z, x[i].w), f);
         // the two halves of a thread's 32 bytes swap their order in the
         // second 64-column block, so eight lanes hit eight 16-byte banks
         uint8_t* row = dst + (r >> 3) * Cfg::kGroupBytes;
@@ -666,8 +746,8 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
           uint4* at = reinterpret_cast<uint4*>(dst + (r >> 3) * Cfg::kGroupBytes + swz128(r & 7, e & 7));
           if (key >= k_end)
             *at = make_uint4(0, 0, 0, 0);
-          else if (any_nonfinite<T>(*at))
-            *at = strip_nonfinite<T>(*at, key - guard_key, bad + e * 8, any_bad);
+          else if (any_nonfinite<MT>(*at))
+            *at = strip_nonfinite<MT>(*at, key - guard_key, bad + e * 8, any_bad);
         }
       }
       fence_proxy_async_smem();
@@ -688,10 +768,21 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     const int pos = it.pos0 + r / p.GQ;
     // keys [0, vis_end) are visible; rows that do not exist see everything
     const int vis_end = !row_live ? 0x7fffffff : p.causal ? min(k_lim, max(pos + 1, 0)) : k_lim;
-    const float sc = p.scale_log2;
+    // Quantised: scores count in units of the query row's and the tile's K
+    // factor, so each tile has its own scale.  V counts in units of 2^v_exp:
+    // the exponent joins the score before the maximum, so P is relative to
+    // the largest contribution to O, and leaves the row sum again.
+    float sc = p.scale_log2;
+    float v_exp = 0.f, v_inv = 1.f;
+    const bool pos_scale = sc >= 0.f;
+    float row_scale = sc;
     float m_own = -INFINITY, l_own = 0.f;
     bool ok = true;
-    for (int j = g; j < nkt; j += 2) {
+    if (kConvertQ && nkt > 0) {
+      ok = __all_sync(0xffffffffu, tc_wait(&bars->q_ready, 0, abort));
+      row_scale = sc * reinterpret_cast<const float*>(sm + Cfg::kQScale)[r];
+    }
+    for (int j = g; j < nkt && ok; j += 2) {
       const int buf = j % NB;
       if (!__all_sync(0xffffffffu, tc_wait(&bars->s_full[buf], (j / NB) & 1, abort))) {
         ok = false;
@@ -704,8 +795,13 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       tc_fence_after();
       const uint32_t sbuf = lane_base + buf * kTcKeys;
       const int key0 = key_base + j * kTcKeys;
+      if constexpr (kQuant) {
+        const int2 e = reinterpret_cast<const int2*>(sm + Cfg::kTileExp)[j & 7];
+        sc = row_scale * pow2_f32(e.x);
+        v_exp = static_cast<float>(e.y);
+        v_inv = pow2_f32(-e.y);
+      }
       const bool all_full = __all_sync(0xffffffffu, key0 + kTcKeys <= vis_end);
-      const bool pos_scale = sc >= 0.f;
       const float ext0 = pos_scale ? -INFINITY : INFINITY;
       float ext = ext0;
       uint32_t ra[32], rb[32];
@@ -738,7 +834,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
           }
         }
       }
-      const float mx = (ext == INFINITY || ext == -INFINITY) ? -INFINITY : ext * sc;
+      const float mx = (ext == INFINITY || ext == -INFINITY) ? -INFINITY : kQuant ? fmaf(ext, sc, v_exp) : ext * sc;
       float m_in = -INFINITY;
       if (j > 0) {
         const int pj = j - 1;
@@ -775,24 +871,24 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         }
       }
       float rs = 0.f;
-      const float neg_m = -m_j;
+      const float neg_m = kQuant ? v_exp - m_j : -m_j;
       if (all_full) {
         const uint64_t sc2 = f2_pack(sc, sc), nm2 = f2_pack(neg_m, neg_m);
         uint64_t acc0 = 0, acc1 = 0;
         uint32_t pk3[16], pka[16], pkb[16];
-        exp2_chunk32<T>(rb, sc2, nm2, acc0, acc1, pk3);
+        exp2_chunk32<MT>(rb, sc2, nm2, acc0, acc1, pk3);
         tmem_wait_ld(ra);
         tmem_ld32_async(sbuf + 32, rb);
-        exp2_chunk32<T>(ra, sc2, nm2, acc0, acc1, pka);
+        exp2_chunk32<MT>(ra, sc2, nm2, acc0, acc1, pka);
         tmem_st16_async(sbuf, pka);
         tmem_wait_ld(rb);
         tmem_ld32_async(sbuf + 64, ra);
-        exp2_chunk32<T>(rb, sc2, nm2, acc0, acc1, pkb);
+        exp2_chunk32<MT>(rb, sc2, nm2, acc0, acc1, pkb);
         tmem_st16_async(sbuf + 16, pkb);
         tmem_st16_async(sbuf + 48, pk3);
         tmem_wait_ld(ra);
         tmem_wait_st();
-        exp2_chunk32<T>(ra, sc2, nm2, acc0, acc1, pka);
+        exp2_chunk32<MT>(ra, sc2, nm2, acc0, acc1, pka);
         tmem_st16_async(sbuf + 32, pka);
         tmem_wait_st();
         float a, bb;
@@ -811,12 +907,12 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
             const float p0 = v0 ? fast_exp2(fmaf(__uint_as_float(raw[i]), sc, neg_m)) : 0.f;
             const float p1 = v1 ? fast_exp2(fmaf(__uint_as_float(raw[i + 1]), sc, neg_m)) : 0.f;
             rs += p0 + p1;
-            packed[i >> 1] = Elem<T>::pack(p0, p1);
+            packed[i >> 1] = Elem<MT>::pack(p0, p1);
           }
           tmem_st8(sbuf + (c >> 1), packed);
         }
       }
-      l_own += rs;
+      l_own += kQuant ? rs * v_inv : rs;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->p_full[buf]);
