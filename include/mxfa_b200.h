@@ -420,6 +420,23 @@ int mxfa_kvcache_varlen_attention_launch(const void* q, const void* k_cache, con
                                          size_t q_token_stride, size_t q_head_stride, int causal,
                                          int bf16, float scale, void* stream);
 
+/* The same attention for a decode step: every sequence has at most max_q
+ * packed queries (one, usually; more query rows than 16 per KV head re-read
+ * the cache), on the split-KV decode kernel.  q and out contiguous.  Splits
+ * as in mxfa_kvcache_attention_counted_launch with rows = total_q * HQ; the
+ * last one runs to the end of its sequence, so num_splits * chunk_len need
+ * only cover the lengths expected.  length_order (optional) from
+ * mxfa_kvcache_length_order_launch.  Quantised caches: D = 128, page sizes
+ * that are multiples of 16, scales 16-byte aligned. */
+int mxfa_kvcache_step_attention_launch(const void* q, const void* k_cache, const void* v_cache,
+                                       const void* k_scales, const void* v_scales,
+                                       const int32_t* cu_seqlens_q, const int32_t* seqlens,
+                                       const int32_t* block_table, const int32_t* length_order, void* out,
+                                       float* lse, void* workspace, size_t workspace_bytes,
+                                       unsigned* counters, int total_q, int B, int max_q, int HQ, int HKV,
+                                       int D, int PS, int BTW, int num_pages, int num_splits,
+                                       int chunk_len, int causal, int bf16, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

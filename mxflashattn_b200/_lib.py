@@ -90,6 +90,9 @@ SIGNATURES = {
     "mxfa_kvcache_varlen_attention_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _sz, _sz, _i, _i, _f,
              _vp]),
+    "mxfa_kvcache_step_attention_launch": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i,
+             _i, _i, _i, _i, _f, _vp]),
     "mxfa_varlen_fwd_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp]),
     "mxfa_varlen_fwd_exact_launch": (

@@ -464,12 +464,31 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
         out = torch.empty((Tq, HQ, D), device=q.device, dtype=q.dtype)
     lse = torch.empty((Tq, HQ), device=q.device, dtype=torch.float32) if return_lse else None
     PS, HKV = k_cache.shape[1], k_cache.shape[2]
+    B = seq.shape[0]
     lib = _L()
     with _on(q):
         stream = _stream(q)
+        if max_seqlen_q <= 1 and Tq and B and (k_scales is None or (D == 128 and PS % 16 == 0)):
+            # a decode step: the split-KV kernel reads K/V once for the query heads of a KV head
+            # without a 128-row tile to fill
+            q = _contig(q)
+            splits, chunk = kvcache_plan(B, 1, HQ, HKV, D, max_seqlen_k)
+            ws, ws_bytes = None, 0
+            if splits > 1:
+                ws_bytes = int(lib.mxfa_split_workspace_bytes(Tq * HQ, D, splits))
+                ws = torch.empty((ws_bytes // 4,), device=q.device, dtype=torch.float32)
+            counters = split_counters(q.device, stream, int(lib.mxfa_split_counter_bytes(B, 1, HQ, HKV)))
+            name = "mxfa_kvcache_step_attention_launch"
+            rc = lib.mxfa_kvcache_step_attention_launch(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales),
+                cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), None if plan is None else _lib.ptr(plan.order),
+                out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), ws_bytes, counters.data_ptr(), Tq, B, 1, HQ, HKV, D, PS,
+                bt.shape[1], k_cache.shape[0], splits, chunk, int(causal), _bf16(q), float(softmax_scale), stream)
+            _lib.check(rc, name)
+            return (out, lse) if return_lse else out
         table = ws = counters = None
         ws_bytes = 0
-        if Tq and seq.shape[0] and PS % 8 == 0 and HQ // HKV <= _MAX_GROUP:
+        if Tq and B and PS % 8 == 0 and HQ // HKV <= _MAX_GROUP:
             table = kvcache_chunk_plan(cu, seq, Tq, HQ, HKV, causal) if plan is None else plan.table
             ws_bytes, counter_bytes = _chunk_sizes(HKV, D)
             ws = torch.empty((ws_bytes // 4,), device=q.device, dtype=torch.float32)
@@ -477,7 +496,7 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
         rc = lib.mxfa_kvcache_varlen_attention_launch(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales),
             cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), _lib.ptr(table), 0 if table is None else table.numel() * 4,
-            out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), ws_bytes, _lib.ptr(counters), Tq, seq.shape[0], HQ, HKV, D,
+            out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), ws_bytes, _lib.ptr(counters), Tq, B, HQ, HKV, D,
             PS, bt.shape[1], k_cache.shape[0], q.stride(0), q.stride(1), int(causal), _bf16(q), float(softmax_scale),
             stream)
     _lib.check(rc, "mxfa_kvcache_varlen_attention_launch")

@@ -178,12 +178,13 @@ bool encode_kv_map(CUtensorMap* map, const void* base, int D, int HKV, long long
 // step in place (cp_merge kept) or left the merge to cp_merge_kernel.
 thread_local int g_cp_merged = 0;
 
-template <typename T, int HD, int NT, bool kTma, bool kFp8 = false>
+template <typename T, int HD, int NT, bool kTma, bool kFp8 = false, bool kRowScale = false>
 int launch_decode_inst(const DecodeParams& p, dim3 grid, const CUtensorMap& tk, const CUtensorMap& tv,
                        cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  auto kern = paged_decode_kernel<T, HD, NT, kTma, kFp8>;
-  const int smem = DecodeCfg<HD, NT, kFp8>::kSmemBytes;
+  auto kern = paged_decode_kernel<T, HD, NT, kTma, kFp8, kRowScale>;
+  using Cfg = DecodeCfg<HD, NT, kFp8>;
+  const int smem = Cfg::kSmemBytes + (kRowScale ? Cfg::kSlots * Cfg::kScaleBytes : 0);
   if (int rc = ensure_smem(kern, smem, done)) return rc;
   DecodeParams pl = p;
   if (pl.cp_merge) {
@@ -230,6 +231,11 @@ int launch_decode_t(const DecodeParams& p, int nt, bool tma, dim3 grid, const CU
 template <typename T>
 int launch_decode_fp8(const DecodeParams& p, int nt, bool tma, dim3 grid, const CUtensorMap& tk,
                       const CUtensorMap& tv, cudaStream_t st) {
+  if (p.k_scales != nullptr) {
+    if (!tma) return fail(MXFA_ERR_UNSUPPORTED, "row scales need pages of a multiple of %d tokens", kTileTok);
+    return nt == 1 ? launch_decode_inst<T, 128, 1, true, true, true>(p, grid, tk, tv, st)
+                   : launch_decode_inst<T, 128, 2, true, true, true>(p, grid, tk, tv, st);
+  }
   if (nt == 1)
     return tma ? launch_decode_inst<T, 128, 1, true, true>(p, grid, tk, tv, st)
                : launch_decode_inst<T, 128, 1, false, true>(p, grid, tk, tv, st);
@@ -504,7 +510,9 @@ static int kvcache_attention_impl(const void* q, const void* k_cache, const void
                                   int PS, int BTW, int num_pages, int append_len, int num_splits, int chunk_len,
                                   int causal, int bf16, float scale, const void* k_new, const void* v_new,
                                   unsigned* counters, void* stream, bool kv_fp8 = false, float k_scale = 1.f,
-                                  float v_scale = 1.f, const int32_t* order = nullptr) {
+                                  float v_scale = 1.f, const int32_t* order = nullptr,
+                                  const uint8_t* k_scales = nullptr, const uint8_t* v_scales = nullptr,
+                                  const int32_t* cu_q = nullptr, int q_rows = 0) {
   if (D != 64 && D != 128) return fail(MXFA_ERR_UNSUPPORTED, "head dim %d not in {64, 128}", D);
   if (B < 0 || Sq < 0 || HQ <= 0 || HKV <= 0 || HQ % HKV != 0)
     return fail(MXFA_ERR_INVALID, "bad head / batch geometry (B=%d Sq=%d HQ=%d HKV=%d)", B, Sq, HQ, HKV);
@@ -514,7 +522,9 @@ static int kvcache_attention_impl(const void* q, const void* k_cache, const void
   if (!q || !k_cache || !v_cache || !seqlens || !out) return fail(MXFA_ERR_INVALID, "null tensor pointer");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || (reinterpret_cast<uintptr_t>(out) & 7))
     return fail(MXFA_ERR_INVALID, "tensors must be 16-byte aligned (out 8-byte)");
-  const long long rows = static_cast<long long>(B) * Sq * HQ;
+  // packed queries: their own row count, and splits that need only cover the expected lengths
+  const bool packed = cu_q != nullptr;
+  const long long rows = packed ? static_cast<long long>(q_rows) * HQ : static_cast<long long>(B) * Sq * HQ;
   if (rows > INT_MAX) return fail(MXFA_ERR_UNSUPPORTED, "%lld query rows (B*Sq*HQ) above 2^31-1", rows);
   DecodeParams p{};
   p.q = q;
@@ -539,6 +549,11 @@ static int kvcache_attention_impl(const void* q, const void* k_cache, const void
   p.k_new = k_new;
   p.v_new = v_new;
   p.order = order;
+  p.k_scales = k_scales;
+  p.v_scales = v_scales;
+  p.cu_q = cu_q;
+  p.q_rows = q_rows;
+  p.last_open = packed ? 1 : 0;
   int max_len = 0;
   if (int rc = cache_capacity(block_table, BTW, PS, &max_len)) return rc;
   if (num_splits <= 0 || chunk_len <= 0) {
@@ -553,7 +568,7 @@ static int kvcache_attention_impl(const void* q, const void* k_cache, const void
   const size_t need = mxfa_split_workspace_bytes(static_cast<int>(rows), D, num_splits);
   if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
     return fail(MXFA_ERR_INVALID, "split workspace too small or unaligned (%zu < %zu bytes)", workspace_bytes, need);
-  if (static_cast<long long>(num_splits) * chunk_len < max_len)
+  if (!packed && static_cast<long long>(num_splits) * chunk_len < max_len)
     return fail(MXFA_ERR_INVALID, "%d splits of %d positions do not cover the cache capacity %d", num_splits,
                 chunk_len, max_len);
   p.NP = num_splits;

@@ -380,4 +380,30 @@ int mxfa_kvcache_varlen_attention_launch(const void* q, const void* k_cache, con
   return D == 128 ? launch_varlen_rows<__half, 128>(p, quant, st) : launch_varlen_rows<__half, 64>(p, quant, st);
 }
 
+int mxfa_kvcache_step_attention_launch(const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+                                       const void* v_scales, const int32_t* cu_seqlens_q, const int32_t* seqlens,
+                                       const int32_t* block_table, const int32_t* length_order, void* out, float* lse,
+                                       void* workspace, size_t workspace_bytes, unsigned* counters, int total_q, int B,
+                                       int max_q, int HQ, int HKV, int D, int PS, int BTW, int num_pages,
+                                       int num_splits, int chunk_len, int causal, int bf16, float scale,
+                                       void* stream) {
+  if (HKV <= 0 || HQ <= 0 || HQ % HKV != 0)
+    return fail(MXFA_ERR_INVALID, "bad head geometry (HQ=%d HKV=%d)", HQ, HKV);
+  if (int rc = paged_varlen_checks(k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqlens, block_table, total_q,
+                                   B, HKV, D, PS, BTW, num_pages))
+    return rc;
+  if (total_q == 0 || B == 0 || max_q == 0) return MXFA_OK;
+  if (max_q < 0) return fail(MXFA_ERR_INVALID, "max_q must not be negative");
+  if (counters == nullptr) return fail(MXFA_ERR_INVALID, "counters is NULL");
+  const bool quant = k_scales != nullptr;
+  if (quant && (D != 128 || PS % kTileTok != 0))
+    return fail(MXFA_ERR_UNSUPPORTED, "a quantised step needs head dim 128 and pages of a multiple of %d", kTileTok);
+  if (!aligned16(k_scales) || !aligned16(v_scales)) return fail(MXFA_ERR_INVALID, "scales must be 16-byte aligned");
+  return kvcache_attention_impl(q, k_cache, v_cache, block_table, seqlens, out, lse, workspace, workspace_bytes, B,
+                                max_q, HQ, HKV, D, PS, BTW, num_pages, 0, num_splits, chunk_len, causal, bf16, scale,
+                                nullptr, nullptr, counters, stream, quant, 1.f, 1.f, length_order,
+                                static_cast<const uint8_t*>(k_scales), static_cast<const uint8_t*>(v_scales),
+                                cu_seqlens_q, total_q);
+}
+
 }  // extern "C"

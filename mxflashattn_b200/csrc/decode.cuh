@@ -80,6 +80,18 @@ struct DecodeParams {
   // written into the cache by the CTA that reads them (one query-row group only).
   const void* k_new;
   const void* v_new;
+  // e4m3 caches with a scale per token and KV head (kRowScale): e8m0 bytes
+  // [P, HKV, PS], 16-byte aligned.
+  const uint8_t* k_scales;
+  const uint8_t* v_scales;
+  // Packed queries (optional): sequence b owns rows cu_q[b] .. cu_q[b+1] of
+  // q [q_rows, HQ, D] and of the outputs, Sq at most; a sequence without rows
+  // (or with more) is left alone.
+  const int* cu_q;
+  int q_rows;
+  // The last split runs to the end of its sequence, however long: NP * c_len
+  // then only has to cover the lengths that the plan expected.
+  int last_open;
 };
 
 constexpr int kDecConsumerWarps = 4;
@@ -108,6 +120,7 @@ struct DecodeCfg {
   static constexpr int kSlotBytes = 2 * kTileBytes;      // K + V
   static constexpr int kSlots = (192 * 1024 / kCtasPerSm) / kSlotBytes / 4 * 4;  // multiple of the consumer count
   static constexpr int kRingBytes = kSlots * kSlotBytes;
+  static constexpr int kScaleBytes = 2 * kTileTok;       // K then V exponent bytes of one tile (row scales)
   static constexpr int kSmemBytes = kRingBytes + 2 * kSlots * 8 + 1024;
   static_assert(kDBlk >= 1, "rows narrower than one 128-byte swizzle block are not supported");
 };
@@ -430,7 +443,13 @@ __device__ __forceinline__ void ldsm_b8_x2_trans(uint32_t addr, uint32_t& r0, ui
                : "r"(addr));
 }
 
-template <typename T, int HD, int NT, bool kTma, bool kFp8 = false>
+// kRowScale (with kFp8 and kTma): each token of a KV head has its own
+// power-of-two scales.  The K scale multiplies the token's scores; V's
+// exponent joins the score before the maximum, so the stored state counts O
+// and d in units of 2^m with P relative to the largest p * |scale| (P never
+// leaves f16's range whatever the scales are), and is taken out of the row
+// sum again: d = sum P 2^-e.  The merge algebra is unchanged.
+template <typename T, int HD, int NT, bool kTma, bool kFp8 = false, bool kRowScale = false>
 __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPerSm)
     paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap tmk,
                         const __grid_constant__ CUtensorMap tmv) {
@@ -441,6 +460,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + Cfg::kRingBytes);
   uint64_t* empty = full + Cfg::kSlots;
+  uint8_t* slot_scales = reinterpret_cast<uint8_t*>(empty + Cfg::kSlots);  // [slot][K|V][16] (row scales)
+  static_assert(!kRowScale || (kFp8 && kTma), "row scales are for e4m3 tiles loaded by TMA");
 
   // Programmatic dependent launch: let the next kernel on the stream start
   // placing its blocks as soon as every block of this grid is running (they
@@ -453,7 +474,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   // the producer's first copies
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kSlots; ++s) {
-      mbar_init(&full[s], kTma ? 1 : 32);
+      mbar_init(&full[s], kTma ? (kRowScale ? 3 : 1) : 32);
       mbar_init(&empty[s], 1);
     }
     fence_mbar_init();
@@ -527,9 +548,16 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   // chunk z then covers [z*c_len, (z+1)*c_len) exactly as the reference's split
   const int lo = p.ows != nullptr ? z * p.c_len : 0;
   const int tile0 = (lo / kTileTok) * kTileTok;
+  int q_row0 = b * p.Sq, q_n = p.Sq;  // this sequence's query rows
+  if (p.cu_q != nullptr) {
+    q_row0 = p.cu_q[b];
+    q_n = p.cu_q[b + 1] - q_row0;
+  }
   if (!have_len) cached_len = p.seqlens[b];
+  // every CTA of the sequence agrees, so none is counted on
+  if (p.cu_q != nullptr && (q_n <= 0 || q_n > p.Sq || q_row0 < 0 || q_row0 > p.q_rows - q_n)) return;
   const int total_len = cached_len + p.append_len;
-  const int hi = p.ows != nullptr ? min(lo + p.c_len, total_len) : total_len;
+  const int hi = p.ows != nullptr && !(p.last_open && z == p.NP - 1) ? min(lo + p.c_len, total_len) : total_len;
   const int ntiles = (hi > lo) ? (hi - tile0 + kTileTok - 1) / kTileTok : 0;
 
   // The producer's first block-table reads go out now, so their latency
@@ -593,6 +621,13 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         // were resolved before the start-up barrier)
         const int slot_row = base == 0 ? first_rows : tile_slot_row(p, b, tile0, ntiles, base + lane);
         const int n = min(32, ntiles - base);
+        // row scales: where the tile's exponent bytes start, in 16-byte units (-1: no such page)
+        int scale_at = -1;
+        if constexpr (kRowScale) {
+          const int page = slot_row / p.PS;
+          if (page < p.P)
+            scale_at = (page * p.HKV + kvh) * (p.PS / kTileTok) + (slot_row - page * p.PS) / kTileTok;
+        }
         for (int j = 0; j < n; ++j) {
           const int row = __shfl_sync(0xffffffffu, slot_row, j);
           if (lane == 0 && !abort) {
@@ -627,6 +662,17 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
           }
           abort = __shfl_sync(0xffffffffu, abort, 0);
           if (abort) break;
+          if constexpr (kRowScale) {
+            // lanes 1 and 2: the tile's 16 K and 16 V exponent bytes
+            const int at = __shfl_sync(0xffffffffu, scale_at, j);
+            if (lane == 1 || lane == 2) {
+              const int slot = (base + j) % Cfg::kSlots;
+              cp_async_16_zfill(slot_scales + slot * Cfg::kScaleBytes + (lane - 1) * kTileTok,
+                                (lane == 1 ? p.k_scales : p.v_scales) + static_cast<size_t>(max(at, 0)) * kTileTok,
+                                at >= 0);
+              cp_async_mbar_arrive_noinc(&full[slot]);
+            }
+          }
         }
       }
       // every copy issued must land before the CTA exits: wait (bounded) for
@@ -634,6 +680,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
       if (lane == 0)
         for (int tt = max(issued - Cfg::kSlots, 0); tt < issued; ++tt)
           mbar_wait(&full[tt % Cfg::kSlots], (tt / Cfg::kSlots) & 1);
+      if (kRowScale) cp_async_wait_all();
     } else {
       constexpr int kRowChunks = Cfg::kRowChunks;
       constexpr int kChunks = kTileTok * kRowChunks;  // per tile per tensor (a multiple of 32)
@@ -690,12 +737,15 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   // ---------------------------------------------------------------- consumers
   const int g = lane >> 2;
   const int t4 = lane & 3;
-  const int rows_total = p.Sq * p.GQ;
+  const int rows_total = q_n * p.GQ;
   const int row_base = rg * 8 * NT;
   const T* qptr = static_cast<const T*>(p.q);
 
   // Q^T fragments (B operand): thread holds Q[row g][d = kk*16 + 2*t4 + {0,1}, +8]
   uint32_t qf[HD / 16][NT][2];
+  // row scales: factors of the score's columns (query rows 2*t4 and 2*t4 + 1
+  // of each n-tile), softmax scale included
+  float col_scale[NT][2];
   int lim[NT][2];  // last visible key position of the two rows this thread owns in each n-tile
   int lim_min = 0x7fffffff;  // the smallest of them over rows that exist
 #pragma unroll
@@ -705,7 +755,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
     if (row < rows_total) {
       const int i = row / p.GQ;
       const int h = kvh * p.GQ + row % p.GQ;
-      qr = qptr + (static_cast<size_t>(b * p.Sq + i) * p.HQ + h) * HD;
+      qr = qptr + (static_cast<size_t>(q_row0 + i) * p.HQ + h) * HD;
     }
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk) {
@@ -722,13 +772,44 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         qf[kk][nt][1] = qr ? ld_u32(qr + kk * 16 + 8 + 2 * t4) : 0u;
       }
     }
+    if constexpr (kRowScale) {
+      // bf16 rows become f16 times the power of two that brings their largest
+      // finite element to [2^14, 2^15), so any size of query keeps its bits
+      float up = 1.f;
+      if constexpr (!std::is_same_v<T, __half>) {
+        float top = 0.f;
+        uint2 raw[HD / 16];
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          raw[kk] = qr ? *reinterpret_cast<const uint2*>(qr + kk * 16 + 4 * t4) : make_uint2(0u, 0u);
+          const float2 a = Elem<T>::unpack(raw[kk].x), b2 = Elem<T>::unpack(raw[kk].y);
+          const float x[4] = {fabsf(a.x), fabsf(a.y), fabsf(b2.x), fabsf(b2.y)};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = x[i] < INFINITY ? fmaxf(top, x[i]) : top;
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = top > 0.f ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -100) : 0;
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const float2 a = Elem<T>::unpack(raw[kk].x), b2 = Elem<T>::unpack(raw[kk].y);
+          qf[kk][nt][0] = Elem<__half>::pack(a.x * down, a.y * down);
+          qf[kk][nt][1] = Elem<__half>::pack(b2.x * down, b2.y * down);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        col_scale[nt][c] = p.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * t4 + c) * 4);
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int col_row = row_base + nt * 8 + 2 * t4 + c;
       if (col_row >= rows_total)
         lim[nt][c] = -1;
       else if (p.causal)
-        lim[nt][c] = total_len - p.Sq + col_row / p.GQ;
+        lim[nt][c] = total_len - q_n + col_row / p.GQ;
       else
         lim[nt][c] = 0x7fffffff;
       if (col_row < rows_total) lim_min = min(lim_min, lim[nt][c]);
@@ -814,6 +895,31 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
       }
     }
 
+    // row scales: K's factor, V's exponent and its inverse for the two tokens
+    // (rows g and g + 8 of the product) this thread holds.  Exponents under
+    // -60 are kept there for the row sum's range and their V counts as zero.
+    float kf[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f}, iv[2] = {1.f, 1.f};
+    bool v_gone[2] = {false, false};
+    if constexpr (kRowScale) {
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(slot_scales + slot * Cfg::kScaleBytes);
+      const uint32_t kw = words[g >> 1] >> ((g & 1) * 8), vw = words[kTileTok / 4 + (g >> 1)] >> ((g & 1) * 8);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t kb = (kw >> (16 * c)) & 255u;
+        uint32_t vb = (vw >> (16 * c)) & 255u;
+        if (partial) {  // bytes of positions outside [lo, hi) may be anything
+          const int pos = pos0 + fp8_tok(g + 8 * c);
+          if (pos < lo || pos >= hi) vb = 127u;
+        }
+        kf[c] = __uint_as_float(kb << 23);
+        v_gone[c] = vb < 67u;
+        vb = max(vb, 67u);
+        ve[c] = static_cast<float>(static_cast<int>(vb) - 127);
+        iv[c] = __uint_as_float((254u - min(vb, 253u)) << 23);
+        if (vb == 255u) iv[c] = __uint_as_float(0x7fffffffu);  // a NaN scale
+      }
+    }
+
     // mask + scale into the log2 domain.  On the e4m3 path (instruction
     // bound), a tile inside [lo, hi) whose last key every existing row sees
     // needs no mask (rows past rows_total have q = 0 and are never read back).
@@ -821,7 +927,12 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] *= p.scale_log2;
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (kRowScale)
+            s[nt][e] = fmaf(s[nt][e], kf[e >> 1] * col_scale[nt][e & 1], ve[e >> 1]);
+          else
+            s[nt][e] *= p.scale_log2;
+        }
     } else {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -830,7 +941,10 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
           const int row = g + ((e >> 1) << 3);  // M row of the score product
           const int pos = pos0 + (kFp8 ? fp8_tok(row) : row);
           const bool ok = pos >= lo && pos < hi && pos <= lim[nt][e & 1];
-          s[nt][e] = ok ? s[nt][e] * p.scale_log2 : -INFINITY;
+          if constexpr (kRowScale)
+            s[nt][e] = ok ? fmaf(s[nt][e], kf[e >> 1] * col_scale[nt][e & 1], ve[e >> 1]) : -INFINITY;
+          else
+            s[nt][e] = ok ? s[nt][e] * p.scale_log2 : -INFINITY;
         }
     }
 
@@ -858,7 +972,13 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         }
         grew |= m_new != m[nt][c];
         alpha[nt][c] = a;
-        l[nt][c] = l[nt][c] * a + p0 + p1;
+        if constexpr (kRowScale) {
+          l[nt][c] = l[nt][c] * a + fmaf(p0, iv[0], p1 * iv[1]);
+          p0 = v_gone[0] ? 0.f : p0;
+          p1 = v_gone[1] ? 0.f : p1;
+        } else {
+          l[nt][c] = l[nt][c] * a + p0 + p1;
+        }
         m[nt][c] = m_new;
         s[nt][c] = p0;
         s[nt][c + 2] = p1;
@@ -1001,7 +1121,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
     }
     const int i = rr / p.GQ;
     const int h = kvh * p.GQ + rr % p.GQ;
-    const size_t R = static_cast<size_t>(b * p.Sq + i) * p.HQ + h;
+    const size_t R = static_cast<size_t>(q_row0 + i) * p.HQ + h;
     if (p.ows != nullptr) {
       *reinterpret_cast<float4*>(p.ows + (R * p.NP + z) * HD + d4) = acc;
       if (d4 == 0) {
@@ -1041,7 +1161,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         if (rr >= rows_total) break;
         const int i = rr / p.GQ;
         const int h = kvh * p.GQ + rr % p.GQ;
-        const int R = (b * p.Sq + i) * p.HQ + h;
+        const int R = (q_row0 + i) * p.HQ + h;
         if constexpr (kFp8) {
           // the e4m3 kernel runs at its register cap: the loop form, inline
           if (p.cp_bufs != nullptr)
@@ -1068,7 +1188,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
             const int rr = row_base + col;
             if (rr >= rows_total) break;
             const int h = kvh * p.GQ + rr % p.GQ;
-            const int R = (b * p.Sq + rr / p.GQ) * p.HQ + h;
+            const int R = (q_row0 + rr / p.GQ) * p.HQ + h;
             cp_merge_row_call<T, HD>(recs, rows_all, R, p.cp_world, lane, static_cast<T*>(p.out), p.lse, tag, t0);
           }
           __syncwarp();  // lanes leave their per-word waits at different times

@@ -194,7 +194,8 @@ def kvcache_gather_varlen(
 class KvChunkPlan:
     """How one step's ragged batch is divided (``kvcache_chunk_plan``); every layer of the step uses it.
 
-    ``table`` lists the items of the tiled kernel on the device.
+    On the device: ``table``, the items of the tiled kernel, and for a decode
+    step ``order``, the sequences longest first.
     """
 
     total_q: int
@@ -204,6 +205,7 @@ class KvChunkPlan:
     kv_heads: int
     causal: bool
     table: torch.Tensor | None
+    order: torch.Tensor | None = None
 
 
 def kvcache_chunk_plan(
@@ -233,7 +235,8 @@ def kvcache_chunk_plan(
     from . import backend
 
     table = backend.kvcache_chunk_plan(cu_seqlens_q, cache_seqlens, int(total_q), q_heads, kv_heads, causal)
-    return KvChunkPlan(int(total_q), batch, int(max_seqlen_q), int(q_heads), int(kv_heads), bool(causal), table)
+    return KvChunkPlan(int(total_q), batch, int(max_seqlen_q), int(q_heads), int(kv_heads), bool(causal), table,
+                       backend.kvcache_length_order(cache_seqlens) if max_seqlen_q <= 1 and batch else None)
 
 
 def flash_attn_varlen_with_kvcache(

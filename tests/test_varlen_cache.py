@@ -238,13 +238,13 @@ def _guard_args(name, **over):
                 total_q=4, B=2, HQ=8, HKV=2, D=128, PS=16, BTW=4, num_pages=8, k_token_stride=256, k_head_stride=128,
                 v_token_stride=256, v_head_stride=128, q_token_stride=1024, q_head_stride=128, causal=1, bf16=1,
                 scale=0.1, stream=None, plan=4096, plan_bytes=1 << 20, workspace=4096,
-                workspace_bytes=1 << 30, counters=4096)
+                workspace_bytes=1 << 30, counters=4096, length_order=None, max_q=1, num_splits=1, chunk_len=64)
     base.update(over)
     return [base[n] for n in NAMES[name]]
 
 
 ENTRIES = ("mxfa_kvcache_append_varlen_launch", "mxfa_kvcache_gather_varlen_launch",
-           "mxfa_kvcache_varlen_attention_launch")
+           "mxfa_kvcache_varlen_attention_launch", "mxfa_kvcache_step_attention_launch")
 
 
 @pytest.mark.parametrize("name", ENTRIES)
@@ -265,6 +265,19 @@ def test_attention_entry_refuses_bad_queries(lib):
     for over in (dict(q=None), dict(out=None), dict(q=4104), dict(q_token_stride=1025), dict(HQ=7), dict(plan=None),
                  dict(plan_bytes=64), dict(workspace=None), dict(workspace_bytes=64), dict(counters=None)):
         assert getattr(lib, name)(*_guard_args(name, **over)) == _lib.MXFA_ERR_INVALID, over
+
+
+def test_step_entry_refuses_what_the_decode_kernel_does_not_take(lib):
+    name = "mxfa_kvcache_step_attention_launch"
+    call = lambda **over: getattr(lib, name)(*_guard_args(name, **over))  # noqa: E731
+    quant = dict(k_scales=4096, v_scales=4096)
+    assert call(D=64, **quant) == _lib.MXFA_ERR_UNSUPPORTED
+    assert call(PS=24, **quant) == _lib.MXFA_ERR_UNSUPPORTED
+    assert call(k_scales=4104, v_scales=4096) == _lib.MXFA_ERR_INVALID
+    for over in (dict(counters=None), dict(max_q=-1), dict(q=None), dict(HQ=7), dict(q=4104),
+                 dict(num_splits=3, workspace=None)):
+        assert call(**over) == _lib.MXFA_ERR_INVALID, over
+    assert call(max_q=0, q=None) == _lib.MXFA_OK
 
 
 def test_plan_entry_refuses_and_sizes_are_host_only(lib):

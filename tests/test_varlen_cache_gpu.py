@@ -383,3 +383,67 @@ def test_bad_pages_and_short_tables_are_flagged_not_read(cuda_device):
     assert _lib.read_error_flags() & _lib.FLAG_TABLE_TOO_NARROW
     changed = (t["kc"].view(torch.uint8) != before).any(dim=-1).any(dim=-1).sum().item()
     assert changed <= 2
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("max_k", [None, 100])
+def test_decode_step_with_idle_sequences_padding_rows_and_an_understated_length(quant, max_k, cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    new, total = [1, 0, 1, 1, 0, 1], [3000, 50, 1, 777, 0, 16]
+    b = make_batch(930, new, total, hq=8, hkv=2, quant=quant, poison=np.nan)
+    t = b.device(cuda_device)
+    q = torch.zeros((6, b.hq, b.d), device=cuda_device, dtype=torch.bfloat16)
+    q[:4] = t["q"]
+    out = torch.full_like(q, 7.0)
+    plan = fa.kvcache_chunk_plan(t["cu"], t["lens"], 6, 1, q_heads=8, kv_heads=2, causal=True)
+    for p in (None, plan):
+        _, lse = fa.flash_attn_varlen_with_kvcache(q, t["kc"], t["vc"], t["cu"], t["lens"], t["table"], 1, max_k,
+                                                   causal=True, k_scales=t["ks"], v_scales=t["vs"], plan=p, out=out,
+                                                   return_softmax_lse=True)
+        assert (host(out)[4:] == 7.0).all()
+        assert_attention(host(out)[:4], host(lse)[:4], b, b.d ** -0.5, True, f"step max_k {max_k}")
+
+
+@pytest.mark.parametrize("new,total", [([1, 1], [700, 300]), ([40, 3], [700, 300])])
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("low,high", [(-30, 8), (-24, -20), (0, 0)])
+def test_values_whose_scales_differ_widely(new, total, dtype, d, low, high, cuda_device):
+    """V rows between 2^low and 2^high: the error stays relative to the attention over |V|, whatever the scales."""
+    from varlen_oracle import attention64
+
+    b = make_batch(940, new, total, hq=4, hkv=2, d=d, dtype=dtype, quant=True)
+    rng = np.random.default_rng(1)
+    lo = max(low, -14) if dtype == "fp16" else low
+    size = np.exp2(rng.integers(lo, max(high, lo) + 1, size=b.v.shape[:3]).astype(np.float64))
+    b.v_codes, b.v_scale = quantise64(syn.round_dtype((b.v * size[..., None]).astype(np.float32), dtype))
+    b.v = b.v_codes * b.v_scale[..., None]
+    out, lse, scale = _attend(b, cuda_device, True)
+    want, want_lse, absv, reach = attention64(b, scale, True)
+    storage = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -10}[dtype]
+    tol = 1.01 * storage * np.abs(want) + (2.0 ** -10 + 4 * d * 2.0 ** -23 * reach[..., None]) * absv
+    tol += 2.0 ** -24 if dtype == "fp16" else 0.0
+    assert (np.abs(out - want) <= tol).all(), f"worst {np.max(np.abs(out - want) / np.maximum(tol, 1e-300)):.2f} of the bound"
+    assert np.abs(lse - want_lse).max() <= 2e-5 + d * 2.0 ** -23 * reach.max()
+
+
+@pytest.mark.parametrize("new,total", [([1, 1], [700, 300]), ([40, 3], [700, 300])])
+def test_keys_and_queries_of_any_size(new, total, cuda_device):
+    """K rows between 2^-40 and 2^20 with queries scaled to match, beyond f16's range on both sides."""
+    from varlen_oracle import attention64
+
+    b = make_batch(950, new, total, hq=4, hkv=2, quant=True)
+    rng = np.random.default_rng(2)
+    size = np.exp2(rng.integers(-40, 21, size=b.k.shape[:3]).astype(np.float64))
+    b.k_codes, b.k_scale = quantise64(syn.round_dtype((b.k * size[..., None]).astype(np.float32), "bf16"))
+    b.k = b.k_codes * b.k_scale[..., None]
+    for q_size in (2.0 ** -20, 2.0 ** 20):
+        b.q = syn.round_dtype(b.q * np.float32(q_size / np.abs(b.q).max()), "bf16")
+        scale = 2.0 ** -20 / q_size
+        out, lse, _ = _attend(b, cuda_device, True, scale=scale)
+        want, want_lse, absv, reach = attention64(b, scale, True)
+        tol = np.maximum(1e-2, 2.0 ** -8 * np.abs(want)) + (2.0 ** -10 + 4 * b.d * 2.0 ** -23 * reach[..., None]) * absv
+        assert (np.abs(out - want) <= tol).all()
+        assert np.abs(lse - want_lse).max() <= 2e-5 + b.d * 2.0 ** -23 * reach.max()
