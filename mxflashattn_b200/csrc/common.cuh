@@ -265,6 +265,13 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// Maximum that keeps a NaN (fmaxf drops it).
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 __device__ __forceinline__ uint32_t ld_u32(const void* p) {
   return *reinterpret_cast<const uint32_t*>(p);
 }

@@ -212,6 +212,10 @@ __device__ __forceinline__ void load_partial(const float* src, float (&o)[HD / 3
 // pairs.  The arithmetic and its order are those of the loop form below
 // (used for NP > 64, and always when kChunked is false): the same M, L and
 // accumulation, bit for bit.
+// Whether a split's (m, d) takes part in a merge: not when it saw no key.  A
+// NaN state does, so a NaN in a visible key reaches the output.
+__device__ __forceinline__ bool split_counts(float2 v) { return v.x != -INFINITY && !(v.y <= 0.f); }
+
 template <int HD, bool kChunked = true>
 __device__ __forceinline__ void merge_split_core(const float* ows, const float* mdws, int r, int NP, int lane,
                                                  float (&acc)[HD / 32], float& M_out, float& L_out) {
@@ -230,12 +234,12 @@ __device__ __forceinline__ void merge_split_core(const float* ows, const float* 
 #pragma unroll
     for (int c = 0; c < kChunk; ++c)
       if (c < NP) load_partial<HD>(src + static_cast<size_t>(c) * HD, o[c]);
-    const bool ok0 = v0.x > -INFINITY && v0.y > 0.f;
-    const bool ok1 = v1.x > -INFINITY && v1.y > 0.f;
-    if (ok0) M = fmaxf(M, v0.x);
-    if (ok1) M = fmaxf(M, v1.x);
+    const bool ok0 = split_counts(v0);
+    const bool ok1 = split_counts(v1);
+    if (ok0) M = fmax_nan(M, v0.x);
+    if (ok1) M = fmax_nan(M, v1.x);
 #pragma unroll
-    for (int sh = 16; sh > 0; sh >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, sh));
+    for (int sh = 16; sh > 0; sh >>= 1) M = fmax_nan(M, __shfl_xor_sync(0xffffffffu, M, sh));
     float w0 = -1.f, w1 = -1.f;
     if (M != -INFINITY) {
       if (ok0) {
@@ -263,7 +267,7 @@ __device__ __forceinline__ void merge_split_core(const float* ows, const float* 
           const float wa = __shfl_sync(0xffffffffu, w0, pz & 31);
           const float wb = __shfl_sync(0xffffffffu, w1, pz & 31);
           const float w = pz < 32 ? wa : wb;
-          if (pz < NP && w >= 0.f) {
+          if (pz < NP && !(w < 0.f)) {
 #pragma unroll
             for (int j = 0; j < kPer; ++j) acc[j] = fmaf(w, o[c][j], acc[j]);
           }
@@ -273,14 +277,14 @@ __device__ __forceinline__ void merge_split_core(const float* ows, const float* 
   } else {
     for (int pz = lane; pz < NP; pz += 32) {
       const float2 v = __ldcg(md + pz);
-      if (v.x > -INFINITY && v.y > 0.f) M = fmaxf(M, v.x);
+      if (split_counts(v)) M = fmax_nan(M, v.x);
     }
 #pragma unroll
-    for (int sh = 16; sh > 0; sh >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, sh));
+    for (int sh = 16; sh > 0; sh >>= 1) M = fmax_nan(M, __shfl_xor_sync(0xffffffffu, M, sh));
     if (M != -INFINITY) {
       for (int pz = lane; pz < NP; pz += 32) {
         const float2 v = __ldcg(md + pz);
-        if (v.x > -INFINITY && v.y > 0.f) L += v.y * fast_exp2(v.x - M);
+        if (split_counts(v)) L += v.y * fast_exp2(v.x - M);
       }
     }
 #pragma unroll
@@ -294,7 +298,7 @@ __device__ __forceinline__ void merge_split_core(const float* ows, const float* 
         const float2 v = __ldcg(md + pz);
         float o[kPer];
         load_partial<HD>(src + static_cast<size_t>(pz) * HD, o);
-        const bool valid = v.x > -INFINITY && v.y > 0.f;
+        const bool valid = split_counts(v);
         const float w = fast_exp2(v.x - M);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) acc[j] = valid ? fmaf(w, o[j], acc[j]) : acc[j];
@@ -327,7 +331,7 @@ __device__ __forceinline__ void merge_split_row(const float* ows, const float* m
 #pragma unroll
     for (int j = 0; j < kPer; ++j) out_f32[static_cast<size_t>(r) * HD + lane * kPer + j] = acc[j] * inv;
   }
-  if (lse != nullptr && lane == 0) lse[r] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+  if (lse != nullptr && lane == 0) lse[r] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
 }
 
 // kFp8: e4m3 caches.  Tiles are dequantised in registers (cvt e4m3x2 ->
@@ -474,7 +478,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   // the producer's first copies
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kSlots; ++s) {
-      mbar_init(&full[s], kTma ? (kRowScale ? 3 : 1) : 32);
+      mbar_init(&full[s], kTma ? 1 : 32);
       mbar_init(&empty[s], 1);
     }
     fence_mbar_init();
@@ -621,15 +625,56 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         // were resolved before the start-up barrier)
         const int slot_row = base == 0 ? first_rows : tile_slot_row(p, b, tile0, ntiles, base + lane);
         const int n = min(32, ntiles - base);
-        // row scales: where the tile's exponent bytes start, in 16-byte units (-1: no such page)
-        int scale_at = -1;
+        // row scales: lane j holds the 16 K and 16 V exponent bytes of tile
+        // base + j, read for 32 tiles at once
+        uint4 k_exp = make_uint4(0, 0, 0, 0), v_exp = k_exp;
         if constexpr (kRowScale) {
           const int page = slot_row / p.PS;
-          if (page < p.P)
-            scale_at = (page * p.HKV + kvh) * (p.PS / kTileTok) + (slot_row - page * p.PS) / kTileTok;
+          if (lane < n && page < p.P) {
+            const size_t at = (static_cast<size_t>(page) * p.HKV + kvh) * p.PS + (slot_row - page * p.PS);
+            k_exp = *reinterpret_cast<const uint4*>(p.k_scales + at);
+            v_exp = *reinterpret_cast<const uint4*>(p.v_scales + at);
+          }
         }
-        for (int j = 0; j < n; ++j) {
+        auto put_scales = [&](int slot) {
+          uint4* at = reinterpret_cast<uint4*>(slot_scales + slot * Cfg::kScaleBytes);
+          at[0] = k_exp;
+          at[1] = v_exp;
+        };
+        int j0 = 0;
+        if constexpr (kRowScale) {
+          if (base == 0) {
+            // the first ring's tiles go out before their scales are waited
+            // for, which then enter all slots at once
+            j0 = min(n, Cfg::kSlots);
+            for (int j = 0; j < j0; ++j) {
+              const int row = __shfl_sync(0xffffffffu, slot_row, j);
+              if (lane == 0) tma_load_4d(ring + j * Cfg::kSlotBytes, &tmk, &full[j], 0, kvh, row, 0);
+            }
+            if (lane < j0) put_scales(lane);
+            __syncwarp();
+            if (lane == 0)
+              for (int j = 0; j < j0; ++j) mbar_arrive_expect_tx(&full[j], 2 * Cfg::kTileBytes);
+            issued = j0;
+          }
+        }
+        for (int j = j0; j < n; ++j) {
           const int row = __shfl_sync(0xffffffffu, slot_row, j);
+          if constexpr (kRowScale) {
+            const int tt = base + j;  // past the first ring: every slot was used
+            const int slot = tt % Cfg::kSlots;
+            if (lane == 0 && !mbar_wait(&empty[slot], (tt / Cfg::kSlots - 1) & 1)) abort = 1;
+            abort = __shfl_sync(0xffffffffu, abort, 0);
+            if (abort) break;
+            if (lane == j) put_scales(slot);
+            __syncwarp();
+            if (lane == 0) {
+              issued = tt + 1;
+              mbar_arrive_expect_tx(&full[slot], 2 * Cfg::kTileBytes);
+              tma_load_4d(ring + slot * Cfg::kSlotBytes, &tmk, &full[slot], 0, kvh, row, 0);
+            }
+            continue;
+          }
           if (lane == 0 && !abort) {
             const int tt = base + j;
             const int slot = tt % Cfg::kSlots;
@@ -662,17 +707,6 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
           }
           abort = __shfl_sync(0xffffffffu, abort, 0);
           if (abort) break;
-          if constexpr (kRowScale) {
-            // lanes 1 and 2: the tile's 16 K and 16 V exponent bytes
-            const int at = __shfl_sync(0xffffffffu, scale_at, j);
-            if (lane == 1 || lane == 2) {
-              const int slot = (base + j) % Cfg::kSlots;
-              cp_async_16_zfill(slot_scales + slot * Cfg::kScaleBytes + (lane - 1) * kTileTok,
-                                (lane == 1 ? p.k_scales : p.v_scales) + static_cast<size_t>(max(at, 0)) * kTileTok,
-                                at >= 0);
-              cp_async_mbar_arrive_noinc(&full[slot]);
-            }
-          }
         }
       }
       // every copy issued must land before the CTA exits: wait (bounded) for
@@ -680,7 +714,6 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
       if (lane == 0)
         for (int tt = max(issued - Cfg::kSlots, 0); tt < issued; ++tt)
           mbar_wait(&full[tt % Cfg::kSlots], (tt / Cfg::kSlots) & 1);
-      if (kRowScale) cp_async_wait_all();
     } else {
       constexpr int kRowChunks = Cfg::kRowChunks;
       constexpr int kChunks = kTileTok * kRowChunks;  // per tile per tensor (a multiple of 32)
@@ -896,27 +929,26 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
     }
 
     // row scales: K's factor, V's exponent and its inverse for the two tokens
-    // (rows g and g + 8 of the product) this thread holds.  Exponents under
-    // -60 are kept there for the row sum's range and their V counts as zero.
+    // (rows g and g + 8 of the product) this thread holds.  V's exponents are
+    // kept from -60 up, for the range of the row sum; a V row under that
+    // counts with 2^-60, an error below 2^-51 in an output.
     float kf[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f}, iv[2] = {1.f, 1.f};
-    bool v_gone[2] = {false, false};
     if constexpr (kRowScale) {
       const uint32_t* words = reinterpret_cast<const uint32_t*>(slot_scales + slot * Cfg::kScaleBytes);
-      const uint32_t kw = words[g >> 1] >> ((g & 1) * 8), vw = words[kTileTok / 4 + (g >> 1)] >> ((g & 1) * 8);
+      const uint32_t kw = words[g >> 1], vw = words[kTileTok / 4 + (g >> 1)];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const uint32_t kb = (kw >> (16 * c)) & 255u;
-        uint32_t vb = (vw >> (16 * c)) & 255u;
+        // the token's byte of the word, as the exponent field of a float
+        const int byte = (g & 1) + 2 * c;
+        kf[c] = __uint_as_float(__funnelshift_l(kw, kw, 23 - 8 * byte) & 0x7f800000u);
+        uint32_t vb = (vw >> (8 * byte)) & 255u;
         if (partial) {  // bytes of positions outside [lo, hi) may be anything
           const int pos = pos0 + fp8_tok(g + 8 * c);
           if (pos < lo || pos >= hi) vb = 127u;
         }
-        kf[c] = __uint_as_float(kb << 23);
-        v_gone[c] = vb < 67u;
-        vb = max(vb, 67u);
-        ve[c] = static_cast<float>(static_cast<int>(vb) - 127);
-        iv[c] = __uint_as_float((254u - min(vb, 253u)) << 23);
-        if (vb == 255u) iv[c] = __uint_as_float(0x7fffffffu);  // a NaN scale
+        const uint32_t e = max(vb, 67u);
+        ve[c] = vb == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(0x4b000000u | e) - 8388735.f;  // e - 127
+        iv[c] = __uint_as_float(0x7f000000u - (e << 23));                                                // 2^(127 - e)
       }
     }
 
@@ -955,14 +987,14 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float mx = fmaxf(s[nt][c], s[nt][c + 2]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        float mx = fmax_nan(s[nt][c], s[nt][c + 2]);
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         // the e4m3 path keeps its running max until a tile's max exceeds it
         // by more than 2^8 (P then stays below 256, exact in f16 with the
         // hi/lo split), which skips most O rescales
-        const float m_cand = fmaxf(m[nt][c], mx);
+        const float m_cand = fmax_nan(m[nt][c], mx);
         const float m_new = (kFp8 && m_cand <= m[nt][c] + 8.f) ? m[nt][c] : m_cand;
         float a = 1.f, p0 = 0.f, p1 = 0.f;
         if (m_new != -INFINITY) {
@@ -974,8 +1006,6 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         alpha[nt][c] = a;
         if constexpr (kRowScale) {
           l[nt][c] = l[nt][c] * a + fmaf(p0, iv[0], p1 * iv[1]);
-          p0 = v_gone[0] ? 0.f : p0;
-          p1 = v_gone[1] ? 0.f : p1;
         } else {
           l[nt][c] = l[nt][c] * a + p0 + p1;
         }
@@ -1104,7 +1134,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
     if (rr >= rows_total) continue;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kDecConsumerWarps; ++w) M = fmaxf(M, mm[w * Mg::kCols + col]);
+    for (int w = 0; w < kDecConsumerWarps; ++w) M = fmax_nan(M, mm[w * Mg::kCols + col]);
     float L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (M != -INFINITY) {
@@ -1135,7 +1165,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
       packed.x = Elem<T>::pack(acc.x * inv, acc.y * inv);
       packed.y = Elem<T>::pack(acc.z * inv, acc.w * inv);
       *reinterpret_cast<uint2*>(op) = packed;
-      if (d4 == 0 && p.lse != nullptr) p.lse[R] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+      if (d4 == 0 && p.lse != nullptr) p.lse[R] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
     }
   }
 

@@ -447,3 +447,19 @@ def test_keys_and_queries_of_any_size(new, total, cuda_device):
         tol = np.maximum(1e-2, 2.0 ** -8 * np.abs(want)) + (2.0 ** -10 + 4 * b.d * 2.0 ** -23 * reach[..., None]) * absv
         assert (np.abs(out - want) <= tol).all()
         assert np.abs(lse - want_lse).max() <= 2e-5 + b.d * 2.0 ** -23 * reach.max()
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("new", [1, 3])
+def test_a_nan_in_a_visible_key_reaches_the_output(quant, new, cuda_device):
+    """Whatever split of the keys holds it, and also when no other key is visible."""
+    total = [new, 20000, 3000, 40]
+    b = make_batch(960, [new] * 4, total, hq=8, hkv=2, quant=quant)
+    for s, at in ((0, 0), (1, 13000), (2, 2990)):
+        slot = int(b.slots(s, at, at + 1)[0])
+        for x in (b.k.reshape(-1, b.hkv, b.d),) + ((b.k_codes.reshape(-1, b.hkv, b.d),) if quant else ()):
+            x[slot, :, 7] = np.nan
+    out, lse, scale = _attend(b, cuda_device, True)
+    dirty = 3 * new
+    assert np.isnan(out[:dirty]).all() and np.isnan(lse[:dirty]).all()
+    assert np.isfinite(out[dirty:]).all() and np.isfinite(lse[dirty:]).all()
