@@ -16,6 +16,7 @@ int paged_varlen_checks(const void* k_cache, const void* v_cache, const void* k_
   if ((k_scales == nullptr) != (v_scales == nullptr))
     return fail(MXFA_ERR_INVALID, "k_scales and v_scales must both be given");
   if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(MXFA_ERR_INVALID, "caches must be 16-byte aligned");
+  if (!aligned4(k_scales) || !aligned4(v_scales)) return fail(MXFA_ERR_INVALID, "scales must be 4-byte aligned");
   int cap = 0;
   return cache_capacity(block_table, BTW, PS, &cap);
 }

@@ -240,15 +240,14 @@ struct ChunkCfg {
   static constexpr int kRaw = kV + kStages * kTile;
   static constexpr int kMl = kQ;                          // epilogue exchange over Q once every product is done
   static constexpr int kMPub = kRaw + kRawSlots * kRawTile;  // [2][128] running maxima
-  // quantised: [K|V][2][128] row factors (f16 pairs), [K|V][2][4] warp maxima,
-  // [8] (K, V) exponents of a tile, [128] factors of the query rows
+  // quantised: [4 tiles][K|V][128] row factors (f16 pairs), [8] (K, V)
+  // exponents of a tile, [128] factors of the query rows
   static constexpr int kScale = kMPub + 2 * kTcRows * 4;
-  static constexpr int kTileMax = kScale + (kQuant ? 2 * 2 * 128 * 4 : 0);
-  static constexpr int kTileExp = kTileMax + (kQuant ? 2 * 16 * 4 : 0);
+  static constexpr int kTileExp = kScale + (kQuant ? 4 * 2 * 128 * 4 : 0);
   static constexpr int kQScale = kTileExp + (kQuant ? 8 * 8 : 0);
   static constexpr int kBad = kQScale + (kQuant ? 128 * 4 : 0);  // [HD] first keys with a non-finite V
   static constexpr int kBar = kBad + HD * 4;
-  static constexpr int kNumBars = 40;
+  static constexpr int kNumBars = 46;
   static constexpr int kSmemBytes = kBar + kNumBars * 8 + 32 + 1024;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kTmemO = 3 * kTcKeys;
@@ -259,10 +258,11 @@ struct ChunkBars {
   uint64_t q_full, q_ready, k_full[3], v_full[3], raw_full[3], raw_empty[3];
   uint64_t s_full[3], p_full[3], pv_done[3];
   uint64_t m_ready[2][4];
+  uint64_t scale_ready[4], scale_free[4];  // quantised: the factors of tile t, slot t % 4
   uint64_t v_ok[2];  // 16-bit caches: the guarded V tiles (the last two at most) are clean
   uint64_t all_done;
 };
-static_assert(sizeof(ChunkBars) <= 40 * 8, "barrier block");
+static_assert(sizeof(ChunkBars) <= 46 * 8, "barrier block");
 
 // Pairs of 16-bit values with an exponent of all ones.
 template <typename T>
@@ -387,6 +387,10 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
     mbar_init(&bars->q_ready, 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bars->scale_ready[i], 1);
+      mbar_init(&bars->scale_free[i], 8);
+    }
     for (int i = 0; i < 3; ++i) {
       mbar_init(&bars->k_full[i], kQuant ? 4 : 1);
       mbar_init(&bars->v_full[i], kQuant ? 4 : 1);
@@ -541,6 +545,74 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       }
     }
     __syncwarp();
+   } else if (kQuant && nkt > 0 && warp == 3) {
+    // --------------------------------------------------------------- scales
+    // The exponent bytes of a tile become f16 factors relative to the tile's
+    // largest byte.  Lane i has keys 4i .. 4i+3 (one page: pages hold a
+    // multiple of 8), read two tiles ahead; what it reads is not looked at
+    // before its tile (addresses stay in range instead).
+    uint32_t* factors = reinterpret_cast<uint32_t*>(sm + Cfg::kScale);
+    int2* tile_exp = reinterpret_cast<int2*>(sm + Cfg::kTileExp);
+    const int lane_pos = key_base + 4 * lane;
+    auto entry_of = [&](int t) {
+      return p.bt[static_cast<size_t>(it.b) * p.BTW + min((lane_pos + t * kTcKeys) / p.PS, p.BTW - 1)];
+    };
+    auto page_ok = [&](int t, int phys) {
+      return t < nkt && lane_pos + t * kTcKeys < k_lim && phys >= 0 && phys < p.P;
+    };
+    auto word_at = [&](const uint8_t* scales, int t, int phys) -> uint32_t {
+      const size_t at = (static_cast<size_t>(page_ok(t, phys) ? phys : 0) * p.HKV + hk) * p.PS +
+                        (lane_pos + t * kTcKeys) % p.PS;
+      return *reinterpret_cast<const uint32_t*>(scales + at);
+    };
+    // bytes of keys outside the sequence (or its pages) become 0, which takes no part in the maximum
+    auto cut = [&](uint32_t w, int t, int phys) -> uint32_t {
+      const int left = k_lim - (lane_pos + t * kTcKeys);  // keys of this word that exist
+      if (!page_ok(t, phys)) return 0u;
+      return left >= 4 ? w : w & ((1u << (8 * max(left, 0))) - 1u);
+    };
+    auto largest = [&](uint32_t w) -> int {  // over the tile's 128 bytes; NaN scales (255) do not count
+      const uint32_t nan = __vcmpeq4(w, 0xffffffffu);
+      uint32_t m = w & ~nan;
+      m = __vmaxu4(m, m >> 16);
+      m = __vmaxu4(m, m >> 8) & 255u;
+      return max(static_cast<int>(__reduce_max_sync(0xffffffffu, m)), kRefMin);
+    };
+    auto factor4 = [&](uint32_t w, int ref) -> uint4 {
+      uint32_t f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int byte = (w >> (8 * i)) & 255;
+        f[i] = byte == 255 ? 0x7fff7fffu : pow2_f16x2(byte - ref + kRefShift);
+      }
+      return make_uint4(f[0], f[1], f[2], f[3]);
+    };
+    int e0 = entry_of(0), e1 = entry_of(1), e2 = entry_of(2);
+    uint32_t k0 = word_at(p.k_scales, 0, e0), v0 = word_at(p.v_scales, 0, e0);
+    uint32_t k1 = word_at(p.k_scales, 1, e1), v1 = word_at(p.v_scales, 1, e1);
+    for (int t = 0; t < nkt; ++t) {
+      const int e3 = entry_of(t + 3);
+      const uint32_t k2 = word_at(p.k_scales, t + 2, e2), v2 = word_at(p.v_scales, t + 2, e2);
+      const uint32_t kw = cut(k0, t, e0), vw = cut(v0, t, e0);
+      const int rk = largest(kw), rv = largest(vw);
+      // slot t % 4 is free once tile t-4's K and V are converted
+      const bool ok = t < 4 || tc_wait(&bars->scale_free[t & 3], (t / 4 - 1) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      uint4* f = reinterpret_cast<uint4*>(factors + (t & 3) * 256);
+      f[lane] = factor4(kw, rk);
+      f[32 + lane] = factor4(vw, rv);
+      if (lane == 0) tile_exp[t & 7] = make_int2(rk - 127 - kRefShift, rv - 127 - kRefShift);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->scale_ready[t & 3]);
+      k0 = k1;
+      v0 = v1;
+      k1 = k2;
+      v1 = v2;
+      e0 = e1;
+      e1 = e2;
+      e2 = e3;
+    }
+    __syncwarp();
    } else if (nkt > 0 && (warp == 1 || warp == 2)) {
     // ------------------------------------------------------------ MMA issue
     if (lane == 0) {
@@ -609,21 +681,16 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     // ----------------------------------------------------------- converters
     // Warps 12-15 turn the e4m3 K tiles into 16-bit tiles, warps 16-19 the V
     // tiles: a thread takes the 16-byte chunk tid % (HD/16) of rows apart by
-    // 128 / (HD/16).  The raw slot is free again once it is in registers, so
-    // all three slots are loads in flight nearly all the time.  Scales of the
-    // next tile are read (through the table) while this one converts.
+    // 128 / (HD/16).
     const bool is_v = warp >= 16;
     const int tid = (threadIdx.x - 384) & 127;
-    const int kvi = is_v ? 1 : 0;
-    uint32_t* factors = reinterpret_cast<uint32_t*>(sm + Cfg::kScale) + kvi * 256;  // [2][128]
-    int* wmax = reinterpret_cast<int*>(sm + Cfg::kTileMax) + kvi * 16;              // K warps: [2][K|V][4]; V: [2][4]
-    int2* tile_exp = reinterpret_cast<int2*>(sm + Cfg::kTileExp);
+    const uint32_t* factors = reinterpret_cast<const uint32_t*>(sm + Cfg::kScale) + (is_v ? 128 : 0);
     if (kConvertQ && is_v) {
       // Query row tid to f16, times the power of two that brings its largest
       // finite element to [2^14, 2^15): exact for elements down to 2^-28 of it.
       if (__all_sync(0xffffffffu, tc_wait(&bars->q_full, 0, abort))) {
         float top = 0.f;
-#pragma unroll 4
+#pragma unroll 1
         for (int ch = 0; ch < HD / 8; ++ch) {
           const uint4 v = *reinterpret_cast<const uint4*>(sm + Cfg::kQ + (ch >> 3) * Cfg::kQBlk + swz128(tid, ch & 7));
           const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -636,7 +703,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         }
         const int e = top > 0.f ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -100) : 0;
         const float down = pow2_f32(-e);
-#pragma unroll 4
+#pragma unroll 1
         for (int ch = 0; ch < HD / 8; ++ch) {
           uint4* at = reinterpret_cast<uint4*>(sm + Cfg::kQ + (ch >> 3) * Cfg::kQBlk + swz128(tid, ch & 7));
           const uint4 v = *at;
@@ -651,93 +718,49 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         if (lane == 0) mbar_arrive(&bars->q_ready);
       }
     }
-    // This thread's key row: table entry and exponent bytes, read ahead and
-    // not looked at before their tile (addresses stay in range instead).
-    const int row_pos = key_base + tid;
-    auto has_row = [&](int t) { return t < nkt && row_pos + t * kTcKeys < k_lim; };
-    auto entry_of = [&](int t) {
-      return p.bt[static_cast<size_t>(it.b) * p.BTW + min((row_pos + t * kTcKeys) / p.PS, p.BTW - 1)];
-    };
-    auto page_ok = [&](int t, int phys) { return has_row(t) && phys >= 0 && phys < p.P; };
-    auto byte_at = [&](int t, int phys) {
-      return (static_cast<size_t>(page_ok(t, phys) ? phys : 0) * p.HKV + hk) * p.PS + (row_pos + t * kTcKeys) % p.PS;
-    };
-    const uint8_t* own = is_v ? p.v_scales : p.k_scales;
-    // The K warps also follow V's exponents: the softmax of a tile needs its
-    // V exponent long before the tile's V is converted.
-    struct Bytes {
-      uint32_t k, v;
-      bool ok;
-    };
-    auto bytes_of = [&](int t, int phys) -> Bytes {
-      const size_t at = byte_at(t, phys);
-      return {own[at], is_v ? 0u : p.v_scales[at], page_ok(t, phys)};
-    };
-    auto known = [](uint32_t byte, bool ok) { return ok && byte < 255 ? static_cast<int>(byte) : 0; };
-    auto put_max = [&](int t, const Bytes& x) {
-      const int mk = __reduce_max_sync(0xffffffffu, known(x.k, x.ok));
-      const int mv = __reduce_max_sync(0xffffffffu, known(x.v, x.ok));
-      if (lane == 0) {
-        wmax[(t & 1) * 8 + (warp & 3)] = mk;
-        if (!is_v) wmax[(t & 1) * 8 + 4 + (warp & 3)] = mv;
-      }
-    };
-    auto get_max = [&](int t, int which) {
-      const int* w = wmax + (t & 1) * 8 + which * 4;
-      return max(max(max(w[0], w[1]), max(w[2], w[3])), kRefMin);
-    };
     constexpr int kCh = HD / 16;
     constexpr int kRowStep = 128 / kCh;
     const int c = tid % kCh, r0 = tid / kCh;
-    Bytes now = bytes_of(0, entry_of(0));
-    int entry1 = entry_of(1), entry2 = entry_of(2);
-    put_max(0, now);
-    named_barrier_sync(is_v ? 4 : 2, 128);
-    Bytes next = bytes_of(1, entry1);
     for (int t = 0; t < nkt; ++t) {
-      // factors of tile t, maxima of tile t+1; bytes of t+2 go out
-      const int ref = get_max(t, 0);
-      const uint32_t mine = now.ok ? now.k : 127u;
-      factors[(t & 1) * 128 + tid] =
-          mine == 255 ? 0x7fff7fffu : pow2_f16x2(static_cast<int>(mine) - ref + kRefShift);
-      if (!is_v && tid == 0) tile_exp[t & 7] = make_int2(ref - 127 - kRefShift, get_max(t, 1) - 127 - kRefShift);
-      put_max(t + 1, next);
-      now = next;
-      next = bytes_of(t + 2, entry2);
-      entry2 = entry_of(t + 3);
-      named_barrier_sync(is_v ? 4 : 2, 128);  // also: every thread is done with tile t-2's factors and maxima
       // position in the producer's order: K_0, then K_{t+1}, V_t
       const int u = is_v ? (t + 1 < nkt ? 2 * t + 2 : 2 * t + 1) : (t == 0 ? 0 : 2 * t - 1);
       const int slot = u % 3, st = t % NS;
       const int key0 = key_base + t * kTcKeys;
-      bool ready = !*abort && tc_wait(&bars->raw_full[slot], (u / 3) & 1, abort);
-      uint4 x[kCh];
-      {
-        const uint8_t* raw = sm + Cfg::kRaw + slot * Cfg::kRawTile + r0 * HD + c * 16;
-#pragma unroll
-        for (int i = 0; i < kCh; ++i) x[i] = *reinterpret_cast<const uint4*>(raw + i * kRowStep * HD);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->raw_empty[slot]);
+      bool ready = tc_wait(&bars->scale_ready[t & 3], (t >> 2) & 1, abort) &&
+                   tc_wait(&bars->raw_full[slot], (u / 3) & 1, abort);
+      const uint8_t* raw = sm + Cfg::kRaw + slot * Cfg::kRawTile + r0 * HD + c * 16;
       // the 16-bit stage is free once the product that read it is done
       if (t >= NS)
         ready = tc_wait(is_v ? &bars->pv_done[(t - NS) % NB] : &bars->s_full[(t - NS) % NB], ((t - NS) / NB) & 1, abort) &&
                 ready;
-      if (!__all_sync(0xffffffffu, ready)) continue;  // aborted: only the barrier above still counts
+      if (!__all_sync(0xffffffffu, ready)) break;
       uint8_t* dst = sm + (is_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile + (c >> 2) * 1024;
       const int ch = (c & 3) * 2, odd = c >> 2;
+      // two chunks at a time: the whole tile unrolled pushed the kernel's loops
+      // out of the instruction cache (504 us for the case that takes 415)
+#pragma unroll 1
+      for (int i0 = 0; i0 < kCh; i0 += 2) {
+        uint4 x[2];
+        uint32_t f[2];
 #pragma unroll
-      for (int i = 0; i < kCh; ++i) {
-        const int r = r0 + i * kRowStep;
-        const uint32_t f = factors[(t & 1) * 128 + r];
-        const uint4 lo = codes_to_f16(make_uint2(x[i].x, x[i].y), f);
-        const uint4 hi = codes_to_f16(make_uint2(x[i].z, x[i].w), f);
-        // the two halves of a thread's 32 bytes swap their order in the
-        // second 64-column block, so eight lanes hit eight 16-byte banks
-        uint8_t* row = dst + (r >> 3) * Cfg::kGroupBytes;
-        *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + odd)) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + 1 - odd)) = odd ? lo : hi;
+        for (int i = 0; i < 2; ++i) {
+          x[i] = *reinterpret_cast<const uint4*>(raw + (i0 + i) * kRowStep * HD);
+          f[i] = factors[(t & 3) * 256 + r0 + (i0 + i) * kRowStep];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = r0 + (i0 + i) * kRowStep;
+          const uint4 lo = codes_to_f16(make_uint2(x[i].x, x[i].y), f[i]);
+          const uint4 hi = codes_to_f16(make_uint2(x[i].z, x[i].w), f[i]);
+          // the two halves of a thread's 32 bytes swap their order in the
+          // second 64-column block, so eight lanes hit eight 16-byte banks
+          uint8_t* row = dst + (r >> 3) * Cfg::kGroupBytes;
+          *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + odd)) = odd ? hi : lo;
+          *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + 1 - odd)) = odd ? lo : hi;
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->raw_empty[slot]);
       if (is_v && t >= guard0) {  // V guard, each thread over its own chunks
 #pragma unroll 1
         for (int i = 0; i < 2 * kCh; ++i) {
@@ -752,7 +775,10 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(is_v ? &bars->v_full[st] : &bars->k_full[st]);
+      if (lane == 0) {
+        mbar_arrive(is_v ? &bars->v_full[st] : &bars->k_full[st]);
+        mbar_arrive(&bars->scale_free[t & 3]);
+      }
     }
    }
   } else {
@@ -805,21 +831,22 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       const float ext0 = pos_scale ? -INFINITY : INFINITY;
       float ext = ext0;
       uint32_t ra[32], rb[32];
+      // Two chunks of 32 columns a turn, the second's load in flight while the
+      // first is worked on.  Loops, not straight code: all warps' loops
+      // together have to stay in the instruction cache (unrolled over the
+      // tile the kernel took 5% longer, the quantised one 20%).  Tiles with
+      // masked columns take short loops of their own, for the same reason.
       if (all_full) {
         float e[4] = {ext0, ext0, ext0, ext0};
-        tmem_ld32_async(sbuf, ra);
-        tmem_wait_ld(ra);
-        tmem_ld32_async(sbuf + 32, rb);
-        ext_chunk32(ra, pos_scale, e);
-        tmem_wait_ld(rb);
-        tmem_ld32_async(sbuf + 64, ra);
-        ext_chunk32(rb, pos_scale, e);
-        tmem_wait_ld(ra);
-        tmem_ld32_async(sbuf + 96, rb);
-        ext_chunk32(ra, pos_scale, e);
-        tmem_wait_ld(rb);
-        tmem_ld32_async(sbuf, ra);
-        ext_chunk32(rb, pos_scale, e);
+#pragma unroll 1
+        for (int c = 0; c < kTcKeys; c += 64) {
+          tmem_ld32_async(sbuf + c, ra);
+          tmem_wait_ld(ra);
+          tmem_ld32_async(sbuf + c + 32, rb);
+          ext_chunk32(ra, pos_scale, e);
+          tmem_wait_ld(rb);
+          ext_chunk32(rb, pos_scale, e);
+        }
         ext = pos_scale ? fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) : fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
       } else {
 #pragma unroll 1
@@ -860,8 +887,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         }
         tc_fence_after();
         const float alpha = grow ? fast_exp2(m_in - m_j) : 1.f;
-        if (all_full) tmem_wait_ld(ra);  // the first chunk's load must not stay open across the ones below
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           uint32_t o[32];
           tmem_ld32(o_base + c, o);
@@ -875,22 +901,19 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       if (all_full) {
         const uint64_t sc2 = f2_pack(sc, sc), nm2 = f2_pack(neg_m, neg_m);
         uint64_t acc0 = 0, acc1 = 0;
-        uint32_t pk3[16], pka[16], pkb[16];
-        exp2_chunk32<MT>(rb, sc2, nm2, acc0, acc1, pk3);
-        tmem_wait_ld(ra);
-        tmem_ld32_async(sbuf + 32, rb);
-        exp2_chunk32<MT>(ra, sc2, nm2, acc0, acc1, pka);
-        tmem_st16_async(sbuf, pka);
-        tmem_wait_ld(rb);
-        tmem_ld32_async(sbuf + 64, ra);
-        exp2_chunk32<MT>(rb, sc2, nm2, acc0, acc1, pkb);
-        tmem_st16_async(sbuf + 16, pkb);
-        tmem_st16_async(sbuf + 48, pk3);
-        tmem_wait_ld(ra);
-        tmem_wait_st();
-        exp2_chunk32<MT>(ra, sc2, nm2, acc0, acc1, pka);
-        tmem_st16_async(sbuf + 32, pka);
-        tmem_wait_st();
+        uint32_t pka[16], pkb[16];
+#pragma unroll 1
+        for (int c = 0; c < kTcKeys; c += 64) {
+          tmem_ld32_async(sbuf + c, ra);
+          tmem_wait_ld(ra);
+          tmem_ld32_async(sbuf + c + 32, rb);
+          exp2_chunk32<MT>(ra, sc2, nm2, acc0, acc1, pka);
+          tmem_st16_async(sbuf + (c >> 1), pka);
+          tmem_wait_ld(rb);
+          exp2_chunk32<MT>(rb, sc2, nm2, acc0, acc1, pkb);
+          tmem_st16_async(sbuf + (c >> 1) + 16, pkb);
+          tmem_wait_st();
+        }
         float a, bb;
         f2_unpack(f2_add(acc0, acc1), a, bb);
         rs = a + bb;
