@@ -174,8 +174,8 @@ int run_chunk(const VarlenAttnParams& a, int D, const void* plan, size_t plan_by
   p.PS = a.PS;
   p.BTW = a.BTW;
   p.P = a.P;
-  p.box = kTcKeys;
-  while (a.PS % p.box != 0) p.box >>= 1;  // the largest power of two up to a tile that divides the page
+  p.box = quant ? ChunkCfg<128, true>::kRawKeys : kTcKeys;
+  while (a.PS % p.box != 0) p.box >>= 1;  // the largest power of two, up to a (half) tile, that divides the page
   p.causal = a.causal;
   p.scale_log2 = a.scale_log2;
   int dev = 0;

@@ -226,28 +226,31 @@ struct ChunkParams {
 
 template <int HD, bool kQuant>
 struct ChunkCfg {
-  static constexpr int kThreads = kQuant ? 640 : 384;
+  static constexpr int kThreads = kQuant ? 768 : 384;
   static constexpr int kDBlk = HD / 64;
   static constexpr int kStages = kQuant ? 2 : 3;
   static constexpr int kGroupBytes = kDBlk * 1024;        // 8 rows of a K or V tile
   static constexpr int kQBlk = 128 * 128;                 // one 64-column block of the Q tile
   static constexpr int kTile = 128 * HD * 2;
-  static constexpr int kRawSlots = kQuant ? 3 : 0;
-  static constexpr int kRawTile = 128 * HD;
+  // quantised: three e4m3 half tiles (64 keys) of K and three of V in flight
+  static constexpr int kRawSlots = 3, kRawKeys = 64;
+  static constexpr int kRawTile = kRawKeys * HD;
+  static constexpr int kRawBytes = kQuant ? 2 * kRawSlots * kRawTile : 0;
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + kTile;
   static constexpr int kV = kK + kStages * kTile;
   static constexpr int kRaw = kV + kStages * kTile;
   static constexpr int kMl = kQ;                          // epilogue exchange over Q once every product is done
-  static constexpr int kMPub = kRaw + kRawSlots * kRawTile;  // [2][128] running maxima
+  static constexpr int kMPub = kRaw + kRawBytes;  // [2][128] running maxima
   // quantised: [4 tiles][K|V][128] row factors (f16 pairs), [8] (K, V)
   // exponents of a tile, [128] factors of the query rows
   static constexpr int kScale = kMPub + 2 * kTcRows * 4;
   static constexpr int kTileExp = kScale + (kQuant ? 4 * 2 * 128 * 4 : 0);
-  static constexpr int kQScale = kTileExp + (kQuant ? 8 * 8 : 0);
+  static constexpr int kExpBytes = kTileExp + (kQuant ? 8 * 8 : 0);  // [8 tiles][K|V][128] exponent bytes
+  static constexpr int kQScale = kExpBytes + (kQuant ? 8 * 256 : 0);
   static constexpr int kBad = kQScale + (kQuant ? 128 * 4 : 0);  // [HD] first keys with a non-finite V
   static constexpr int kBar = kBad + HD * 4;
-  static constexpr int kNumBars = 46;
+  static constexpr int kNumBars = 52;
   static constexpr int kSmemBytes = kBar + kNumBars * 8 + 32 + 1024;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kTmemO = 3 * kTcKeys;
@@ -255,14 +258,14 @@ struct ChunkCfg {
 };
 
 struct ChunkBars {
-  uint64_t q_full, q_ready, k_full[3], v_full[3], raw_full[3], raw_empty[3];
+  uint64_t q_full, q_ready, k_full[3], v_full[3], raw_full[2][3], raw_empty[2][3];
   uint64_t s_full[3], p_full[3], pv_done[3];
   uint64_t m_ready[2][4];
   uint64_t scale_ready[4], scale_free[4];  // quantised: the factors of tile t, slot t % 4
   uint64_t v_ok[2];  // 16-bit caches: the guarded V tiles (the last two at most) are clean
   uint64_t all_done;
 };
-static_assert(sizeof(ChunkBars) <= 46 * 8, "barrier block");
+static_assert(sizeof(ChunkBars) <= 52 * 8, "barrier block");
 
 // Pairs of 16-bit values with an exponent of all ones.
 template <typename T>
@@ -334,8 +337,9 @@ __device__ __forceinline__ uint4 codes_to_f16(uint2 codes, uint32_t factor) {
   return make_uint4(mul_f16x2(h.x, factor), mul_f16x2(h.y, factor), mul_f16x2(h.z, factor), mul_f16x2(h.w, factor));
 }
 
-// Register shares of the quantised kernel's five warpgroups (launched with
-// 96 each): producers, issuers and converters give theirs to the softmax.
+// Register shares of the quantised kernel's six warpgroups (launched with 80
+// each): producers, issuers, converters and the scale warp give theirs to
+// the softmax.
 template <int N>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -344,8 +348,8 @@ template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
-constexpr int kRegsIssue = 48, kRegsSoftmax = 152, kRegsConvert = 64;
-static_assert(kRegsIssue + 2 * kRegsSoftmax + 2 * kRegsConvert <= 5 * 96, "the launch's registers");
+constexpr int kRegsIssue = 56, kRegsSoftmax = 128, kRegsConvert = 64, kRegsScale = 40;
+static_assert(kRegsIssue + 2 * kRegsSoftmax + 2 * kRegsConvert + kRegsScale <= 6 * 80, "the launch's registers");
 
 __device__ __forceinline__ void named_barrier_arrive(int id, int threads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -394,8 +398,10 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     for (int i = 0; i < 3; ++i) {
       mbar_init(&bars->k_full[i], kQuant ? 4 : 1);
       mbar_init(&bars->v_full[i], kQuant ? 4 : 1);
-      mbar_init(&bars->raw_full[i], 1);
-      mbar_init(&bars->raw_empty[i], 4);
+      for (int kv = 0; kv < 2; ++kv) {
+        mbar_init(&bars->raw_full[kv][i], 1);
+        mbar_init(&bars->raw_empty[kv][i], 4);
+      }
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], kTcGroupWarps);
       mbar_init(&bars->pv_done[i], 1);
@@ -419,21 +425,22 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Physical page of position pos as the table has it (-1 past the keys).
-  // The value is not looked at before it is used, a tile later: a compare
-  // beside the load would wait out its latency.
-  auto page_entry = [&](int pos, bool want) -> int {
-    return want && pos < k_lim ? p.bt[static_cast<size_t>(it.b) * p.BTW + pos / p.PS] : -1;
+  // Boxes of this item, numbered from key_base on: the table entry of box g
+  // (of the last page past the table), and from it the cache row in units of
+  // `unit` rows -- the first row past the cache, where TMA fills zeros and
+  // reads nothing, for an entry that names no page.  Entries are read 32
+  // boxes ahead, a box per lane, and not looked at before.
+  auto box_entry = [&](int g) -> int {
+    return p.bt[static_cast<size_t>(it.b) * p.BTW + min((key_base + g * p.box) / p.PS, p.BTW - 1)];
   };
-  // Cache row (in units of `unit` rows) of position pos on page phys; the
-  // first row past the cache, where TMA fills zeros and reads nothing, for
-  // an entry that names no page.
-  auto box_row = [&](int pos, int phys, int unit) -> int {
+  auto box_row = [&](int g, int phys, int unit) -> int {
+    const int pos = key_base + g * p.box;
+    if (pos >= k_lim) return 0;
     if (phys < 0 || phys >= p.P) {
       raise_flag(MXFA_FLAG_PAGE_OUT_OF_RANGE);
       return static_cast<int>(static_cast<long long>(p.P) * p.PS / unit);
     }
-    return static_cast<int>((static_cast<long long>(phys) * p.PS + pos % p.PS) / unit);
+    return (phys * p.PS + pos % p.PS) / unit;  // slots fit 31 bits
   };
   // first tile (of this item) that some row does not see in full
   const int guard0 = max(0, vis_first / kTcKeys - it.kt0);
@@ -441,34 +448,33 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
 
   if (warp < 4) {
    if constexpr (kQuant) regs_dec<kRegsIssue>();
-   if (nkt > 0 && (warp == 0 || (warp == 3 && !kQuant))) {
+   if (nkt > 0 && (warp == 0 || warp == 3)) {
     // ------------------------------------------------------------ producers
-    // 16-bit: warp 0 loads Q and K, warp 3 loads V.  Quantised: warp 0 loads
-    // Q and the e4m3 tiles in the converter's order.  Lane i owns box i of a
-    // tile; the block-table entries of the next tile are read ahead.
+    // Warp 0 loads Q and K, warp 3 loads V; lane i issues box i of a tile.
     const int nbox = kTcKeys / p.box;
     const bool for_v = warp == 3;
+    const CUtensorMap* map = for_v ? &tmv : &tmk;
     if (lane == 0 && !for_v) {
-      prefetch_tensormap(&tmq);
       mbar_arrive_expect_tx(&bars->q_full, Cfg::kDBlk * (kTcRows / p.GQ) * p.GQ * 128);
 #pragma unroll
       for (int db = 0; db < Cfg::kDBlk; ++db)
         tma_load_3d(sm + Cfg::kQ + db * Cfg::kQBlk, &tmq, &bars->q_full, db * 64, hk * p.GQ, it.row0);
     }
-    const int lane_pos = key_base + lane * p.box;  // this lane's box of tile 0
-    auto entry_of = [&](int t) { return page_entry(lane_pos + t * kTcKeys, t < nkt && lane < nbox); };
-    auto has_box = [&](int t) { return lane < nbox && lane_pos + t * kTcKeys < k_lim; };
     bool ok = true;
-    int filled = 0;
-    if constexpr (!kQuant) {
-      int entry = entry_of(0);
-      for (int t = 0; t < nkt; ++t) {
-        const int next = entry_of(t + 1);
+    int filled = 0;  // tiles, or half tiles, whose copies were started
+    int entry = box_entry(lane), rows = 0;
+    for (int t = 0; t < nkt && ok; ++t) {
+      const int g0 = t * nbox;
+      if ((g0 & 31) == 0) {
+        rows = box_row(g0 + lane, entry, kQuant ? 1 : 8);
+        entry = box_entry(g0 + 32 + lane);
+      }
+      const int row = __shfl_sync(0xffffffffu, rows, (g0 + (lane & (nbox - 1))) & 31);
+      const bool has = lane < nbox && key_base + (g0 + lane) * p.box < k_lim;
+      if constexpr (!kQuant) {
         const int st = t % NS, use = t / NS;
         uint64_t* full = for_v ? &bars->v_full[st] : &bars->k_full[st];
-        const bool has = has_box(t);
         const int n = __popc(__ballot_sync(0xffffffffu, has));
-        const int row = has ? box_row(lane_pos + t * kTcKeys, entry, 8) : 0;
         if (lane == 0) {
           // K stage: free once S_{t-3} is done; V stage: once P.V_{t-3} is
           if (use > 0) ok = tc_wait(for_v ? &bars->pv_done[st] : &bars->s_full[st], (use - 1) & 1, abort);
@@ -477,10 +483,34 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         filled = t + 1;
-        uint8_t* dst = sm + (for_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile + lane * (p.box / 8) * Cfg::kGroupBytes;
-        if (has) tma_load_5d(dst, for_v ? &tmv : &tmk, full, 0, hk, 0, 0, row);
-        entry = next;
+        if (has)
+          tma_load_5d(sm + (for_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile + lane * (p.box / 8) * Cfg::kGroupBytes, map,
+                      full, 0, hk, 0, 0, row);
+      } else {
+        const int half = Cfg::kRawKeys / p.box;  // boxes of a half tile
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int slot = filled % Cfg::kRawSlots, use = filled / Cfg::kRawSlots;
+          const bool mine = has && lane / half == h;
+          const int n = __popc(__ballot_sync(0xffffffffu, mine));
+          if (lane == 0) {
+            if (use > 0) ok = tc_wait(&bars->raw_empty[for_v][slot], (use - 1) & 1, abort);
+            if (ok) mbar_arrive_expect_tx(&bars->raw_full[for_v][slot], n * p.box * HD);
+          }
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) break;
+          ++filled;
+          if (mine)
+            tma_load_3d(sm + Cfg::kRaw + ((for_v ? Cfg::kRawSlots : 0) + slot) * Cfg::kRawTile + lane % half * p.box * HD,
+                        map, &bars->raw_full[for_v][slot], 0, hk, row);
+        }
       }
+    }
+    if constexpr (kQuant) {
+      if (*abort && lane == 0)  // leave no copy in flight
+        for (int w = max(0, filled - Cfg::kRawSlots); w < filled; ++w)
+          mbar_wait(&bars->raw_full[for_v][w % Cfg::kRawSlots], (w / Cfg::kRawSlots) & 1);
+    } else {
       if (for_v) {
         // V guard: keys [vis_first, end of tile) of the last tiles
         for (int t = guard0; t < nkt && ok; ++t) {
@@ -504,113 +534,9 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
           if (lane == 0) mbar_arrive(&bars->v_ok[t - guard0]);
         }
       }
-      if (*abort) {  // leave no copy in flight
-        if (lane == 0)
-          for (int t = max(0, filled - NS); t < filled; ++t)
-            mbar_wait(for_v ? &bars->v_full[t % NS] : &bars->k_full[t % NS], (t / NS) & 1);
-      }
-    } else {
-      // order: K_0, then per tile K_{t+1} and V_t
-      int u = 0;
-      auto emit = [&](int t, int row, const CUtensorMap* map) {
-        const int slot = u % 3;
-        const bool has = has_box(t);
-        const int n = __popc(__ballot_sync(0xffffffffu, has));
-        if (lane == 0) {
-          if (u >= 3) ok = tc_wait(&bars->raw_empty[slot], (u / 3 - 1) & 1, abort);
-          if (ok) mbar_arrive_expect_tx(&bars->raw_full[slot], n * p.box * HD);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) return;
-        if (has)
-          tma_load_3d(sm + Cfg::kRaw + slot * Cfg::kRawTile + lane * p.box * HD, map, &bars->raw_full[slot], 0, hk, row);
-        filled = ++u;
-      };
-      auto row_of = [&](int t, int entry) { return has_box(t) ? box_row(lane_pos + t * kTcKeys, entry, 1) : 0; };
-      const int e0 = entry_of(0);
-      int e1 = entry_of(1);
-      int r0 = row_of(0, e0);
-      emit(0, r0, &tmk);
-      for (int t = 0; t < nkt && ok; ++t) {
-        const int e2 = entry_of(t + 2);
-        const int r1 = t + 1 < nkt ? row_of(t + 1, e1) : 0;
-        if (t + 1 < nkt) emit(t + 1, r1, &tmk);
-        if (ok) emit(t, r0, &tmv);
-        r0 = r1;
-        e1 = e2;
-      }
-      if (*abort) {
-        if (lane == 0)
-          for (int u = max(0, filled - 3); u < filled; ++u) mbar_wait(&bars->raw_full[u % 3], (u / 3) & 1);
-      }
-    }
-    __syncwarp();
-   } else if (kQuant && nkt > 0 && warp == 3) {
-    // --------------------------------------------------------------- scales
-    // The exponent bytes of a tile become f16 factors relative to the tile's
-    // largest byte.  Lane i has keys 4i .. 4i+3 (one page: pages hold a
-    // multiple of 8), read two tiles ahead; what it reads is not looked at
-    // before its tile (addresses stay in range instead).
-    uint32_t* factors = reinterpret_cast<uint32_t*>(sm + Cfg::kScale);
-    int2* tile_exp = reinterpret_cast<int2*>(sm + Cfg::kTileExp);
-    const int lane_pos = key_base + 4 * lane;
-    auto entry_of = [&](int t) {
-      return p.bt[static_cast<size_t>(it.b) * p.BTW + min((lane_pos + t * kTcKeys) / p.PS, p.BTW - 1)];
-    };
-    auto page_ok = [&](int t, int phys) {
-      return t < nkt && lane_pos + t * kTcKeys < k_lim && phys >= 0 && phys < p.P;
-    };
-    auto word_at = [&](const uint8_t* scales, int t, int phys) -> uint32_t {
-      const size_t at = (static_cast<size_t>(page_ok(t, phys) ? phys : 0) * p.HKV + hk) * p.PS +
-                        (lane_pos + t * kTcKeys) % p.PS;
-      return *reinterpret_cast<const uint32_t*>(scales + at);
-    };
-    // bytes of keys outside the sequence (or its pages) become 0, which takes no part in the maximum
-    auto cut = [&](uint32_t w, int t, int phys) -> uint32_t {
-      const int left = k_lim - (lane_pos + t * kTcKeys);  // keys of this word that exist
-      if (!page_ok(t, phys)) return 0u;
-      return left >= 4 ? w : w & ((1u << (8 * max(left, 0))) - 1u);
-    };
-    auto largest = [&](uint32_t w) -> int {  // over the tile's 128 bytes; NaN scales (255) do not count
-      const uint32_t nan = __vcmpeq4(w, 0xffffffffu);
-      uint32_t m = w & ~nan;
-      m = __vmaxu4(m, m >> 16);
-      m = __vmaxu4(m, m >> 8) & 255u;
-      return max(static_cast<int>(__reduce_max_sync(0xffffffffu, m)), kRefMin);
-    };
-    auto factor4 = [&](uint32_t w, int ref) -> uint4 {
-      uint32_t f[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int byte = (w >> (8 * i)) & 255;
-        f[i] = byte == 255 ? 0x7fff7fffu : pow2_f16x2(byte - ref + kRefShift);
-      }
-      return make_uint4(f[0], f[1], f[2], f[3]);
-    };
-    int e0 = entry_of(0), e1 = entry_of(1), e2 = entry_of(2);
-    uint32_t k0 = word_at(p.k_scales, 0, e0), v0 = word_at(p.v_scales, 0, e0);
-    uint32_t k1 = word_at(p.k_scales, 1, e1), v1 = word_at(p.v_scales, 1, e1);
-    for (int t = 0; t < nkt; ++t) {
-      const int e3 = entry_of(t + 3);
-      const uint32_t k2 = word_at(p.k_scales, t + 2, e2), v2 = word_at(p.v_scales, t + 2, e2);
-      const uint32_t kw = cut(k0, t, e0), vw = cut(v0, t, e0);
-      const int rk = largest(kw), rv = largest(vw);
-      // slot t % 4 is free once tile t-4's K and V are converted
-      const bool ok = t < 4 || tc_wait(&bars->scale_free[t & 3], (t / 4 - 1) & 1, abort);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      uint4* f = reinterpret_cast<uint4*>(factors + (t & 3) * 256);
-      f[lane] = factor4(kw, rk);
-      f[32 + lane] = factor4(vw, rv);
-      if (lane == 0) tile_exp[t & 7] = make_int2(rk - 127 - kRefShift, rv - 127 - kRefShift);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->scale_ready[t & 3]);
-      k0 = k1;
-      v0 = v1;
-      k1 = k2;
-      v1 = v2;
-      e0 = e1;
-      e1 = e2;
-      e2 = e3;
+      if (*abort && lane == 0)
+        for (int t = max(0, filled - NS); t < filled; ++t)
+          mbar_wait(for_v ? &bars->v_full[t % NS] : &bars->k_full[t % NS], (t / NS) & 1);
     }
     __syncwarp();
    } else if (nkt > 0 && (warp == 1 || warp == 2)) {
@@ -675,6 +601,78 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
      tc_fence_after();
      tmem_dealloc(tmem, Cfg::kTmemCols);
    }
+  } else if (kQuant && warp >= 20) {
+   if constexpr (kQuant) regs_dec<kRegsScale>();
+   if (nkt > 0 && warp == 20) {
+    // --------------------------------------------------------------- scales
+    // The exponent bytes of a tile become f16 factors relative to the tile's
+    // largest byte.  Lane i has keys 4i .. 4i+3 (one page: pages hold a
+    // multiple of 8), copied to its own words of a ring four tiles ahead.
+    uint32_t* factors = reinterpret_cast<uint32_t*>(sm + Cfg::kScale);
+    int2* tile_exp = reinterpret_cast<int2*>(sm + Cfg::kTileExp);
+    uint32_t* ring = reinterpret_cast<uint32_t*>(sm + Cfg::kExpBytes);  // [8][K|V][32]
+    const int nbox = kTcKeys / p.box;
+    // box g's first byte in units of 8, ~0u without a page
+    auto box_bytes = [&](int g, int phys) -> unsigned {
+      const int pos = key_base + g * p.box;
+      if (pos >= k_lim || phys < 0 || phys >= p.P) return ~0u;
+      return static_cast<unsigned>(((static_cast<size_t>(phys) * p.HKV + hk) * p.PS + pos % p.PS) >> 3);
+    };
+    int entry = box_entry(lane);
+    unsigned base = 0;
+    auto fetch = [&](int t) {
+      const int g0 = t * nbox;
+      if ((g0 & 31) == 0) {
+        base = box_bytes(g0 + lane, entry);
+        entry = box_entry(g0 + 32 + lane);
+      }
+      const unsigned at8 = __shfl_sync(0xffffffffu, base, (g0 + 4 * lane / p.box) & 31);
+      const bool has = at8 != ~0u;
+      const size_t at = (has ? static_cast<size_t>(at8) << 3 : 0) + (4 * lane) % p.box;
+      uint32_t* dst = ring + (t & 7) * 64 + lane;
+      cp_async_4_zfill(dst, p.k_scales + at, has);
+      cp_async_4_zfill(dst + 32, p.v_scales + at, has);
+    };
+    // the word's bytes of keys past the sequence become 0, which takes no part in the maximum
+    auto cut = [&](uint32_t w, int t) -> uint32_t {
+      const int left = k_lim - (key_base + t * kTcKeys + 4 * lane);  // keys of this word that exist
+      return left >= 4 ? w : w & ((1u << (8 * max(left, 0))) - 1u);
+    };
+    auto largest = [&](uint32_t w) -> int {  // over the tile's 128 bytes; NaN scales (255) do not count
+      uint32_t m = w & ~__vcmpeq4(w, 0xffffffffu);
+      m = __vmaxu4(m, m >> 16);
+      m = __vmaxu4(m, m >> 8) & 255u;
+      return max(static_cast<int>(__reduce_max_sync(0xffffffffu, m)), kRefMin);
+    };
+    auto factor4 = [&](uint32_t w, int ref) -> uint4 {
+      uint32_t f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int byte = (w >> (8 * i)) & 255;
+        f[i] = byte == 255 ? 0x7fff7fffu : pow2_f16x2(byte - ref + kRefShift);
+      }
+      return make_uint4(f[0], f[1], f[2], f[3]);
+    };
+#pragma unroll 1
+    for (int t = -4; t < nkt; ++t) {
+      if (t + 4 < nkt) fetch(t + 4);
+      cp_async_commit();
+      if (t < 0) continue;
+      cp_async_wait<4>();  // tile t's group
+      const uint32_t kw = cut(ring[(t & 7) * 64 + lane], t), vw = cut(ring[(t & 7) * 64 + 32 + lane], t);
+      const int rk = largest(kw), rv = largest(vw);
+      // slot t % 4 is free once tile t-4's K and V are converted
+      const bool ok = t < 4 || tc_wait(&bars->scale_free[t & 3], (t / 4 - 1) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      uint4* f = reinterpret_cast<uint4*>(factors + (t & 3) * 256);
+      f[lane] = factor4(kw, rk);
+      f[32 + lane] = factor4(vw, rv);
+      if (lane == 0) tile_exp[t & 7] = make_int2(rk - 127 - kRefShift, rv - 127 - kRefShift);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->scale_ready[t & 3]);
+    }
+    cp_async_wait_all();
+   }
   } else if (kQuant && warp >= 12) {
    if constexpr (kQuant) regs_dec<kRegsConvert>();
    if (nkt > 0) {
@@ -722,45 +720,48 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     constexpr int kRowStep = 128 / kCh;
     const int c = tid % kCh, r0 = tid / kCh;
     for (int t = 0; t < nkt; ++t) {
-      // position in the producer's order: K_0, then K_{t+1}, V_t
-      const int u = is_v ? (t + 1 < nkt ? 2 * t + 2 : 2 * t + 1) : (t == 0 ? 0 : 2 * t - 1);
-      const int slot = u % 3, st = t % NS;
-      const int key0 = key_base + t * kTcKeys;
-      bool ready = tc_wait(&bars->scale_ready[t & 3], (t >> 2) & 1, abort) &&
-                   tc_wait(&bars->raw_full[slot], (u / 3) & 1, abort);
-      const uint8_t* raw = sm + Cfg::kRaw + slot * Cfg::kRawTile + r0 * HD + c * 16;
+      const int st = t % NS, key0 = key_base + t * kTcKeys;
+      bool ready = tc_wait(&bars->scale_ready[t & 3], (t >> 2) & 1, abort);
       // the 16-bit stage is free once the product that read it is done
       if (t >= NS)
         ready = tc_wait(is_v ? &bars->pv_done[(t - NS) % NB] : &bars->s_full[(t - NS) % NB], ((t - NS) / NB) & 1, abort) &&
                 ready;
-      if (!__all_sync(0xffffffffu, ready)) break;
       uint8_t* dst = sm + (is_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile + (c >> 2) * 1024;
       const int ch = (c & 3) * 2, odd = c >> 2;
-      // two chunks at a time: the whole tile unrolled pushed the kernel's loops
-      // out of the instruction cache (504 us for the case that takes 415)
 #pragma unroll 1
-      for (int i0 = 0; i0 < kCh; i0 += 2) {
-        uint4 x[2];
-        uint32_t f[2];
+      for (int h = 0; h < 2; ++h) {
+        const int w = 2 * t + h, slot = w % Cfg::kRawSlots;
+        ready = tc_wait(&bars->raw_full[is_v][slot], (w / Cfg::kRawSlots) & 1, abort) && ready;
+        if (!__all_sync(0xffffffffu, ready)) break;
+        const uint8_t* raw = sm + Cfg::kRaw + ((is_v ? Cfg::kRawSlots : 0) + slot) * Cfg::kRawTile + c * 16;
+        // two chunks at a time: the whole tile unrolled pushed the kernel's
+        // loops out of the instruction cache
+#pragma unroll 1
+        for (int r = r0; r < Cfg::kRawKeys; r += 2 * kRowStep) {
+          const int key = h * Cfg::kRawKeys + r;  // row of the tile
+          uint4 x[2];
+          uint32_t f[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          x[i] = *reinterpret_cast<const uint4*>(raw + (i0 + i) * kRowStep * HD);
-          f[i] = factors[(t & 3) * 256 + r0 + (i0 + i) * kRowStep];
-        }
+          for (int i = 0; i < 2; ++i) {
+            x[i] = *reinterpret_cast<const uint4*>(raw + (r + i * kRowStep) * HD);
+            f[i] = factors[(t & 3) * 256 + key + i * kRowStep];
+          }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = r0 + (i0 + i) * kRowStep;
-          const uint4 lo = codes_to_f16(make_uint2(x[i].x, x[i].y), f[i]);
-          const uint4 hi = codes_to_f16(make_uint2(x[i].z, x[i].w), f[i]);
-          // the two halves of a thread's 32 bytes swap their order in the
-          // second 64-column block, so eight lanes hit eight 16-byte banks
-          uint8_t* row = dst + (r >> 3) * Cfg::kGroupBytes;
-          *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + odd)) = odd ? hi : lo;
-          *reinterpret_cast<uint4*>(row + swz128(r & 7, ch + 1 - odd)) = odd ? lo : hi;
+          for (int i = 0; i < 2; ++i) {
+            const int k = key + i * kRowStep;
+            const uint4 lo = codes_to_f16(make_uint2(x[i].x, x[i].y), f[i]);
+            const uint4 hi = codes_to_f16(make_uint2(x[i].z, x[i].w), f[i]);
+            // the two halves of a thread's 32 bytes swap their order in the
+            // second 64-column block, so eight lanes hit eight 16-byte banks
+            uint8_t* at = dst + (k >> 3) * Cfg::kGroupBytes;
+            *reinterpret_cast<uint4*>(at + swz128(k & 7, ch + odd)) = odd ? hi : lo;
+            *reinterpret_cast<uint4*>(at + swz128(k & 7, ch + 1 - odd)) = odd ? lo : hi;
+          }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->raw_empty[is_v][slot]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->raw_empty[slot]);
+      if (!__all_sync(0xffffffffu, ready)) break;
       if (is_v && t >= guard0) {  // V guard, each thread over its own chunks
 #pragma unroll 1
         for (int i = 0; i < 2 * kCh; ++i) {

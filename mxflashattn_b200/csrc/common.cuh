@@ -147,6 +147,12 @@ __device__ __forceinline__ void cp_async_16_zfill(void* dst, const void* src, bo
                : "memory");
 }
 
+// Copies 4 bytes when `valid`, else writes 4 zero bytes (src not read).
+__device__ __forceinline__ void cp_async_4_zfill(void* dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 4 : 0)
+               : "memory");
+}
+
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 template <int N>
