@@ -226,7 +226,7 @@ struct ChunkParams {
 
 template <int HD, bool kQuant>
 struct ChunkCfg {
-  static constexpr int kThreads = kQuant ? 768 : 384;
+  static constexpr int kThreads = kQuant ? 1024 : 384;
   static constexpr int kDBlk = HD / 64;
   static constexpr int kStages = kQuant ? 2 : 3;
   static constexpr int kGroupBytes = kDBlk * 1024;        // 8 rows of a K or V tile
@@ -337,7 +337,7 @@ __device__ __forceinline__ uint4 codes_to_f16(uint2 codes, uint32_t factor) {
   return make_uint4(mul_f16x2(h.x, factor), mul_f16x2(h.y, factor), mul_f16x2(h.z, factor), mul_f16x2(h.w, factor));
 }
 
-// Register shares of the quantised kernel's six warpgroups (launched with 80
+// Register shares of the quantised kernel's eight warpgroups (launched with 64
 // each): producers, issuers, converters and the scale warp give theirs to
 // the softmax.
 template <int N>
@@ -348,8 +348,8 @@ template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
-constexpr int kRegsIssue = 56, kRegsSoftmax = 128, kRegsConvert = 64, kRegsScale = 40;
-static_assert(kRegsIssue + 2 * kRegsSoftmax + 2 * kRegsConvert + kRegsScale <= 6 * 80, "the launch's registers");
+constexpr int kRegsIssue = 56, kRegsSoftmax = 128, kRegsConvert = 40, kRegsScale = 40;
+static_assert(kRegsIssue + 2 * kRegsSoftmax + 4 * kRegsConvert + kRegsScale <= 8 * 64, "the launch's registers");
 
 __device__ __forceinline__ void named_barrier_arrive(int id, int threads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -368,7 +368,6 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   ChunkBars* bars = reinterpret_cast<ChunkBars*>(sm + Cfg::kBar);
   float* ml = reinterpret_cast<float*>(sm + Cfg::kMl);
-  float* mpub = reinterpret_cast<float*>(sm + Cfg::kMPub);
   unsigned* bad = reinterpret_cast<unsigned*>(sm + Cfg::kBad);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Cfg::kBar + Cfg::kNumBars * 8);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -393,11 +392,11 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     mbar_init(&bars->q_ready, 4);
     for (int i = 0; i < 4; ++i) {
       mbar_init(&bars->scale_ready[i], 1);
-      mbar_init(&bars->scale_free[i], 8);
+      mbar_init(&bars->scale_free[i], 16);
     }
     for (int i = 0; i < 3; ++i) {
-      mbar_init(&bars->k_full[i], kQuant ? 4 : 1);
-      mbar_init(&bars->v_full[i], kQuant ? 4 : 1);
+      mbar_init(&bars->k_full[i], kQuant ? 8 : 1);
+      mbar_init(&bars->v_full[i], kQuant ? 8 : 1);
       for (int kv = 0; kv < 2; ++kv) {
         mbar_init(&bars->raw_full[kv][i], 1);
         mbar_init(&bars->raw_empty[kv][i], 4);
@@ -601,9 +600,9 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
      tc_fence_after();
      tmem_dealloc(tmem, Cfg::kTmemCols);
    }
-  } else if (kQuant && warp >= 20) {
+  } else if (kQuant && warp >= 28) {
    if constexpr (kQuant) regs_dec<kRegsScale>();
-   if (nkt > 0 && warp == 20) {
+   if (nkt > 0 && warp == 28) {
     // --------------------------------------------------------------- scales
     // The exponent bytes of a tile become f16 factors relative to the tile's
     // largest byte.  Lane i has keys 4i .. 4i+3 (one page: pages hold a
@@ -677,13 +676,14 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
    if constexpr (kQuant) regs_dec<kRegsConvert>();
    if (nkt > 0) {
     // ----------------------------------------------------------- converters
-    // Warps 12-15 turn the e4m3 K tiles into 16-bit tiles, warps 16-19 the V
-    // tiles: a thread takes the 16-byte chunk tid % (HD/16) of rows apart by
-    // 128 / (HD/16).
-    const bool is_v = warp >= 16;
+    // Warps 12-19 turn the e4m3 K tiles into f16 tiles, warps 20-27 the V
+    // tiles; each warpgroup takes one half (64 keys) of every tile.  A thread
+    // has the eight codes c of rows kRowStep apart, one 16-byte store each:
+    // eight lanes fill a row of one 64-column block, all banks once.
+    const bool is_v = warp >= 20;
+    const int h = (warp >> 2) & 1 ? 0 : 1;  // warps 12-15 and 20-23: the first half
     const int tid = (threadIdx.x - 384) & 127;
-    const uint32_t* factors = reinterpret_cast<const uint32_t*>(sm + Cfg::kScale) + (is_v ? 128 : 0);
-    if (kConvertQ && is_v) {
+    if (kConvertQ && is_v && h == 0) {
       // Query row tid to f16, times the power of two that brings its largest
       // finite element to [2^14, 2^15): exact for elements down to 2^-28 of it.
       if (__all_sync(0xffffffffu, tc_wait(&bars->q_full, 0, abort))) {
@@ -716,62 +716,51 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         if (lane == 0) mbar_arrive(&bars->q_ready);
       }
     }
-    constexpr int kCh = HD / 16;
-    constexpr int kRowStep = 128 / kCh;
+    constexpr int kCh = HD / 8;            // eight-code chunks of a row
+    constexpr int kRowStep = 128 / kCh;    // 8 or 16: a thread's rows share their place in an 8-row group
+    constexpr int kSteps = Cfg::kRawKeys / kRowStep;
     const int c = tid % kCh, r0 = tid / kCh;
+    // shared-space addresses of this thread's first chunk in a raw slot, in a
+    // 16-bit stage and of its first row's factor; the others follow at
+    // constant distances (generic addresses took twice the instructions)
+    const uint32_t raw_0 = smem_u32(sm + Cfg::kRaw) + (is_v ? Cfg::kRawSlots : 0) * Cfg::kRawTile + r0 * HD + c * 8;
+    const uint32_t dst_off = ((h * Cfg::kRawKeys + r0) >> 3) * Cfg::kGroupBytes + (c >> 3) * 1024 + swz128(r0 & 7, c & 7);
+    const uint32_t dst_0 = smem_u32(sm + (is_v ? Cfg::kV : Cfg::kK)) + dst_off;
+    const uint32_t factor_0 = smem_u32(sm + Cfg::kScale) + ((is_v ? 128 : 0) + h * Cfg::kRawKeys + r0) * 4;
     for (int t = 0; t < nkt; ++t) {
       const int st = t % NS, key0 = key_base + t * kTcKeys;
-      bool ready = tc_wait(&bars->scale_ready[t & 3], (t >> 2) & 1, abort);
+      // the codes go to registers as soon as they are there, and their slot
+      // back to the producer: a slot held through the waits below bounded the
+      // kernel by its round trip
+      const int w = 2 * t + h, slot = w % Cfg::kRawSlots;
+      bool ready = tc_wait(&bars->raw_full[is_v][slot], (w / Cfg::kRawSlots) & 1, abort);
+      uint2 x[kSteps];
+      const uint32_t src = raw_0 + slot * Cfg::kRawTile;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) x[i] = lds_v2(src + i * kRowStep * HD);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->raw_empty[is_v][slot]);
+      ready = tc_wait(&bars->scale_ready[t & 3], (t >> 2) & 1, abort) && ready;
       // the 16-bit stage is free once the product that read it is done
       if (t >= NS)
         ready = tc_wait(is_v ? &bars->pv_done[(t - NS) % NB] : &bars->s_full[(t - NS) % NB], ((t - NS) / NB) & 1, abort) &&
                 ready;
-      uint8_t* dst = sm + (is_v ? Cfg::kV : Cfg::kK) + st * Cfg::kTile + (c >> 2) * 1024;
-      const int ch = (c & 3) * 2, odd = c >> 2;
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        const int w = 2 * t + h, slot = w % Cfg::kRawSlots;
-        ready = tc_wait(&bars->raw_full[is_v][slot], (w / Cfg::kRawSlots) & 1, abort) && ready;
-        if (!__all_sync(0xffffffffu, ready)) break;
-        const uint8_t* raw = sm + Cfg::kRaw + ((is_v ? Cfg::kRawSlots : 0) + slot) * Cfg::kRawTile + c * 16;
-        // two chunks at a time: the whole tile unrolled pushed the kernel's
-        // loops out of the instruction cache
-#pragma unroll 1
-        for (int r = r0; r < Cfg::kRawKeys; r += 2 * kRowStep) {
-          const int key = h * Cfg::kRawKeys + r;  // row of the tile
-          uint4 x[2];
-          uint32_t f[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            x[i] = *reinterpret_cast<const uint4*>(raw + (r + i * kRowStep) * HD);
-            f[i] = factors[(t & 3) * 256 + key + i * kRowStep];
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int k = key + i * kRowStep;
-            const uint4 lo = codes_to_f16(make_uint2(x[i].x, x[i].y), f[i]);
-            const uint4 hi = codes_to_f16(make_uint2(x[i].z, x[i].w), f[i]);
-            // the two halves of a thread's 32 bytes swap their order in the
-            // second 64-column block, so eight lanes hit eight 16-byte banks
-            uint8_t* at = dst + (k >> 3) * Cfg::kGroupBytes;
-            *reinterpret_cast<uint4*>(at + swz128(k & 7, ch + odd)) = odd ? hi : lo;
-            *reinterpret_cast<uint4*>(at + swz128(k & 7, ch + 1 - odd)) = odd ? lo : hi;
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->raw_empty[is_v][slot]);
-      }
       if (!__all_sync(0xffffffffu, ready)) break;
+      const uint32_t dst = dst_0 + st * Cfg::kTile, fac = factor_0 + (t & 3) * 1024;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+        sts_v4(dst + i * (kRowStep / 8) * Cfg::kGroupBytes, codes_to_f16(x[i], lds_u32(fac + i * kRowStep * 4)));
       if (is_v && t >= guard0) {  // V guard, each thread over its own chunks
 #pragma unroll 1
-        for (int i = 0; i < 2 * kCh; ++i) {
-          const int r = r0 + (i >> 1) * kRowStep, e = c * 2 + (i & 1), key = key0 + r;
+        for (int r = h * Cfg::kRawKeys + r0; r < (h + 1) * Cfg::kRawKeys; r += kRowStep) {
+          const int key = key0 + r;
           if (key < vis_first) continue;
-          uint4* at = reinterpret_cast<uint4*>(dst + (r >> 3) * Cfg::kGroupBytes + swz128(r & 7, e & 7));
+          uint4* at = reinterpret_cast<uint4*>(sm + Cfg::kV + st * Cfg::kTile + (r >> 3) * Cfg::kGroupBytes +
+                                               (c >> 3) * 1024 + swz128(r & 7, c & 7));
           if (key >= k_end)
             *at = make_uint4(0, 0, 0, 0);
           else if (any_nonfinite<MT>(*at))
-            *at = strip_nonfinite<MT>(*at, key - guard_key, bad + e * 8, any_bad);
+            *at = strip_nonfinite<MT>(*at, key - guard_key, bad + c * 8, any_bad);
         }
       }
       fence_proxy_async_smem();
@@ -804,6 +793,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     const bool pos_scale = sc >= 0.f;
     float row_scale = sc;
     float m_own = -INFINITY, l_own = 0.f;
+    const uint32_t mpub_r = smem_u32(sm + Cfg::kMPub) + r * 4;  // [tile parity][row] running maxima
     bool ok = true;
     if (kConvertQ && nkt > 0) {
       ok = __all_sync(0xffffffffu, tc_wait(&bars->q_ready, 0, abort));
@@ -823,10 +813,10 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       const uint32_t sbuf = lane_base + buf * kTcKeys;
       const int key0 = key_base + j * kTcKeys;
       if constexpr (kQuant) {
-        const int2 e = reinterpret_cast<const int2*>(sm + Cfg::kTileExp)[j & 7];
-        sc = row_scale * pow2_f32(e.x);
-        v_exp = static_cast<float>(e.y);
-        v_inv = pow2_f32(-e.y);
+        const uint2 e = lds_v2(smem_u32(sm + Cfg::kTileExp) + (j & 7) * 8);
+        sc = row_scale * pow2_f32(static_cast<int>(e.x));
+        v_exp = static_cast<float>(static_cast<int>(e.y));
+        v_inv = pow2_f32(-static_cast<int>(e.y));
       }
       const bool all_full = __all_sync(0xffffffffu, key0 + kTcKeys <= vis_end);
       const float ext0 = pos_scale ? -INFINITY : INFINITY;
@@ -870,10 +860,10 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
           ok = false;
           break;
         }
-        m_in = mpub[(pj & 1) * kTcRows + r];
+        m_in = lds_f32(mpub_r + (pj & 1) * kTcRows * 4);
       }
       const float m_j = mx > m_in + kRescaleThreshold ? mx : m_in;
-      mpub[(j & 1) * kTcRows + r] = m_j;
+      sts_f32(mpub_r + (j & 1) * kTcRows * 4, m_j);
       mbar_arrive(&bars->m_ready[j & 1][quad]);
       if (m_j != m_own) {
         l_own *= fast_exp2(m_own - m_j);
