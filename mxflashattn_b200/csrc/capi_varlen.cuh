@@ -168,6 +168,8 @@ int run_chunk(const VarlenAttnParams& a, int D, const void* plan, size_t plan_by
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<size_t>(a.HKV) * p.parts_cap * kTcRows * D;
   p.counters = counters;
+  p.T = a.T;
+  p.B = a.B;
   p.HQ = a.HQ;
   p.HKV = a.HKV;
   p.GQ = a.GQ;
@@ -323,6 +325,8 @@ int mxfa_kvcache_chunk_plan_launch(const int32_t* cu_seqlens_q, const int32_t* s
   p.tok = kTcRows / (HQ / HKV);
   p.items_cap = chunk_items_cap(total_q, B, HQ, HKV);
   p.parts_cap = chunk_parts_cap(HKV);
+  p.slots = sm_count();
+  p.HKV = HKV;
   p.share = chunk_share(HKV);
   p.min_part = 4;
   p.causal = causal ? 1 : 0;

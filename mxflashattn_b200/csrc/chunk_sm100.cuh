@@ -48,6 +48,7 @@ struct ChunkItem {
 constexpr int kPlanHeader = 16;  // ints before the items: [0] items
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBuckets = 256;
+constexpr int kChunkMaxParts = 160;  // parts of one tile (their weights share memory with the K and V stages)
 
 struct ChunkPlanParams {
   const int* cu;
@@ -55,7 +56,8 @@ struct ChunkPlanParams {
   int* plan;     // header, items, then B + 1 tile offsets
   int T, B, tok; // tok: tokens per tile
   int items_cap, parts_cap;
-  int share;     // CTA slots per KV head that the step's work is divided by
+  int slots, HKV;  // CTAs the GPU holds at once, KV heads
+  int share;     // slots / HKV: what the step's work per KV head is divided by
   int min_part;  // key tiles a part holds at least
   int causal;
 };
@@ -91,24 +93,37 @@ __device__ __forceinline__ int chunk_tile(const ChunkPlanParams& p, const int* o
   return max(1, (k_end + kTcKeys - 1) / kTcKeys);
 }
 
-// One block.  The work is counted in key tiles; parts hold at most
-// max(work / share, min_part) of them, which bounds the items by tiles +
-// share and the parts of split tiles by 2 * share.  Buckets of equal length
-// order the items; which item of a bucket comes first is left to the
-// atomics, since the order only schedules.
+// Sum over the block (every thread gets it); s: one int of shared memory.
+__device__ __forceinline__ int block_sum(int x, int* s) {
+  x = __reduce_add_sync(0xffffffffu, x);
+  __syncthreads();
+  if (threadIdx.x == 0) *s = 0;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) atomicAdd(s, x);
+  __syncthreads();
+  return *s;
+}
+
+// One block; the work is counted in key tiles.  Let fair = work / share, the
+// tiles a CTA slot would get of an even division.
+//  - Fewer tiles than slots: every tile is split into parts of at most L,
+//    L the smallest for which the parts still go out in one wave.
+//  - More: tiles longer than fair are split to it, so one long sequence does
+//    not outlast the rest; without such, what remains after whole waves (the
+//    shortest tiles) is split over the slots of the last one.  512 equal
+//    items on 148 SMs: 3 waves and a split one instead of 4.
+// Parts of split tiles never exceed 2 * share.  Buckets of equal length
+// order the items, longest first; which item of a bucket comes first is left
+// to the atomics, since the order only schedules.
 __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const ChunkPlanParams p) {
   __shared__ int s_scan[kPlanThreads / 32];
-  __shared__ unsigned long long s_work;
-  __shared__ int s_max, s_parts, s_groups, s_hist[kPlanBuckets];
+  __shared__ int s_sum, s_max, s_parts, s_groups, s_tail, s_hist[kPlanBuckets];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   ChunkItem* items = reinterpret_cast<ChunkItem*>(p.plan + kPlanHeader);
   int* off = p.plan + kPlanHeader + p.items_cap * static_cast<int>(sizeof(ChunkItem) / 4);
-  if (tid == 0) {
-    s_work = 0;
-    s_max = s_parts = s_groups = 0;
-  }
+  if (tid == 0) s_max = s_parts = s_groups = s_tail = 0;
   for (int i = tid; i < kPlanBuckets; i += kPlanThreads) s_hist[i] = 0;
   // tile offsets: block-wide exclusive scan over the sequences
   int base = 0;
@@ -145,64 +160,111 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const ChunkPla
   if (tid == 0) off[p.B] = tiles;
   __syncthreads();  // off (global, this block's own writes) and the counters are visible
 
-  unsigned long long work = 0;
-  int longest = 0;
-  for (int i = tid; i < tiles; i += kPlanThreads) {
+  // f(tile, its key tiles) over this thread's tiles; the first four lengths
+  // stay in registers
+  constexpr int kKeep = 4;
+  int len[kKeep];
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k) {
     ChunkItem it;
-    const int n = chunk_tile(p, off, i, it);
+    const int i = tid + k * kPlanThreads;
+    len[k] = i < tiles ? chunk_tile(p, off, i, it) : 0;
+  }
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      if (tid + k * kPlanThreads < tiles) f(tid + k * kPlanThreads, len[k]);
+    for (int i = tid + kKeep * kPlanThreads; i < tiles; i += kPlanThreads) {
+      ChunkItem it;
+      f(i, chunk_tile(p, off, i, it));
+    }
+  };
+  long long work = 0;  // 64-bit sum in two halves
+  int longest = 0;
+  each([&](int, int n) {
     work += n;
     longest = max(longest, n);
-  }
-  atomicAdd(&s_work, work);
+  });
   atomicMax(&s_max, longest);
-  __syncthreads();
-  const long long fair = (static_cast<long long>(s_work) + p.share - 1) / p.share;
-  const int limit = static_cast<int>(min(max(fair, static_cast<long long>(p.min_part)), 1ll << 30));
-  const int top = min(s_max, limit);
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int i = tid; i < tiles; i += kPlanThreads) {
-      ChunkItem it;
-      const int n = chunk_tile(p, off, i, it);
-      const int parts = (n + limit - 1) / limit;
-      const int per = (n + parts - 1) / parts;
-      const int bucket =
-          kPlanBuckets - 1 - static_cast<int>(static_cast<long long>(per) * (kPlanBuckets - 1) / max(top, 1));
-      if (pass == 0) {
-        atomicAdd(&s_hist[bucket], parts);
-        continue;
-      }
-      const int at = atomicAdd(&s_hist[bucket], parts);
-      it.nsplit = parts;
-      it.part0 = it.group = -1;
-      if (parts > 1) {
-        it.part0 = atomicAdd(&s_parts, parts);
-        it.group = atomicAdd(&s_groups, 1);
-      }
-      for (int s = 0; s < parts; ++s) {
-        it.split = s;
-        it.kt0 = min(s * per, n);
-        it.kt1 = min((s + 1) * per, n);
-        if (at + s < p.items_cap) items[at + s] = it;
-      }
+  const int lo16 = block_sum(static_cast<int>(work & 0xffff), &s_sum);
+  const int hi16 = block_sum(static_cast<int>(work >> 16), &s_sum);
+  const long long total = static_cast<long long>(hi16) * 65536 + lo16;
+  longest = s_max;
+  const int fair = static_cast<int>(min((total + p.share - 1) / p.share, 1ll << 30));
+  int limit = max(max(fair, p.min_part), (longest + kChunkMaxParts - 1) / kChunkMaxParts);
+  if (tiles > 0 && tiles < p.share) {
+    int lo = limit, hi = max(longest, limit);
+    while (lo < hi) {  // the smallest limit whose parts fit one wave
+      const int mid = (lo + hi) >> 1;
+      int n = 0;
+      each([&](int, int m) { n += (m + mid - 1) / mid; });
+      if (block_sum(n, &s_sum) <= p.share)
+        hi = mid;
+      else
+        lo = mid + 1;
     }
-    __syncthreads();
-    if (pass == 0 && warp == 0) {  // exclusive scan of the buckets, longest first
-      int run = 0;
-      for (int b0 = 0; b0 < kPlanBuckets; b0 += 32) {
-        const int n = s_hist[b0 + lane];
-        int x = n;
-#pragma unroll
-        for (int sh = 1; sh < 32; sh <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, x, sh);
-          if (lane >= sh) x += y;
-        }
-        s_hist[b0 + lane] = run + x - n;
-        run += __shfl_sync(0xffffffffu, x, 31);
-      }
-      if (lane == 0) p.plan[0] = min(run, p.items_cap);
-    }
-    __syncthreads();
+    limit = lo;
   }
+  // tiles that whole waves take unsplit, and the parts of each one behind them
+  int whole = tiles, tail_parts = 1;
+  if (tiles >= p.share && longest <= limit) {
+    const int waves = static_cast<int>(static_cast<long long>(tiles) * p.HKV / p.slots);
+    const int rest = tiles - static_cast<int>(static_cast<long long>(waves) * p.slots / p.HKV);
+    if (rest > 0 && rest < tiles && p.slots / (rest * p.HKV) > 1) {
+      whole = tiles - rest;
+      tail_parts = p.slots / (rest * p.HKV);
+    }
+  }
+  const int top = min(longest, limit);
+  auto bucket_of = [&](int per) {
+    return kPlanBuckets - 1 - static_cast<int>(static_cast<long long>(per) * (kPlanBuckets - 1) / max(top, 1));
+  };
+  each([&](int, int n) {
+    const int parts = (n + limit - 1) / limit;
+    atomicAdd(&s_hist[bucket_of((n + parts - 1) / parts)], parts);
+  });
+  __syncthreads();
+  if (warp == 0) {  // exclusive scan of the buckets, longest first
+    int run = 0;
+    for (int b0 = 0; b0 < kPlanBuckets; b0 += 32) {
+      const int n = s_hist[b0 + lane];
+      int x = n;
+#pragma unroll
+      for (int sh = 1; sh < 32; sh <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, sh);
+        if (lane >= sh) x += y;
+      }
+      s_hist[b0 + lane] = run + x - n;
+      run += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) s_sum = run;
+  }
+  __syncthreads();
+  each([&](int i, int n) {
+    int parts = (n + limit - 1) / limit;
+    int at = atomicAdd(&s_hist[bucket_of((n + parts - 1) / parts)], parts);
+    if (tail_parts > 1 && at >= whole) {  // (parts is 1 wherever whole waves precede split tiles)
+      parts = max(1, min(tail_parts, n / p.min_part));
+      at = whole + atomicAdd(&s_tail, parts);
+    }
+    const int per = (n + parts - 1) / parts;
+    ChunkItem it;
+    chunk_tile(p, off, i, it);
+    it.nsplit = parts;
+    it.part0 = it.group = -1;
+    if (parts > 1) {
+      it.part0 = atomicAdd(&s_parts, parts);
+      it.group = atomicAdd(&s_groups, 1);
+    }
+    for (int s = 0; s < parts; ++s) {
+      it.split = s;
+      it.kt0 = min(s * per, n);
+      it.kt1 = min((s + 1) * per, n);
+      if (at + s < p.items_cap) items[at + s] = it;
+    }
+  });
+  __syncthreads();
+  if (tid == 0) p.plan[0] = min(tail_parts > 1 ? whole + s_tail : s_sum, p.items_cap);
 }
 
 // --------------------------------------------------------------- attention
@@ -218,7 +280,7 @@ struct ChunkParams {
   float* part_ml;   // [HKV][parts_cap][128][2]
   unsigned* counters;  // [HKV][parts_cap / 2 + 1], zero on entry and on exit
   int parts_cap;
-  int HQ, HKV, GQ, PS, BTW, P;
+  int T, B, HQ, HKV, GQ, PS, BTW, P;
   int box;       // rows of one TMA box: divides PS and 128, a multiple of 8
   int causal;
   float scale_log2;
@@ -226,7 +288,11 @@ struct ChunkParams {
 
 template <int HD, bool kQuant>
 struct ChunkCfg {
-  static constexpr int kThreads = kQuant ? 1024 : 384;
+  // softmax groups of four warps; group g takes tiles j % kGroups == g.  At D = 64 the products
+  // of a tile are short and a third group pays (46.2 -> 43.4 us on ragged pieces); at D = 128 it
+  // costs (477 -> 494 us on a long one).
+  static constexpr int kGroups = !kQuant && HD == 64 ? 3 : 2;
+  static constexpr int kThreads = kQuant ? 1024 : 128 + 128 * kGroups;
   static constexpr int kDBlk = HD / 64;
   static constexpr int kStages = kQuant ? 2 : 3;
   static constexpr int kGroupBytes = kDBlk * 1024;        // 8 rows of a K or V tile
@@ -362,6 +428,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   using Cfg = ChunkCfg<HD, kQuant>;
   constexpr int NS = Cfg::kStages;
   constexpr int NB = 3;
+  constexpr int NG = Cfg::kGroups, kSoft = 128 * NG;  // softmax groups and threads
   using MT = std::conditional_t<kQuant, __half, T>;              // tensor-core operand type
   constexpr bool kConvertQ = kQuant && !std::is_same_v<T, __half>;  // bf16 queries become f16 in shared memory
   extern __shared__ uint8_t smem_raw[];
@@ -378,6 +445,13 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   const int hk = blockIdx.x;
   if (static_cast<int>(blockIdx.y) >= p.plan[0]) return;
   const ChunkItem it = reinterpret_cast<const ChunkItem*>(p.plan + kPlanHeader)[blockIdx.y];
+  // a plan made for another batch reaches nothing outside this one's tensors
+  if (it.b < 0 || it.b >= p.B || it.row0 < 0 || it.ntok < 1 || it.ntok * p.GQ > kTcRows || it.row0 > p.T - it.ntok ||
+      it.kt0 < 0 || it.nsplit < 1 || it.nsplit > kChunkMaxParts || it.split < 0 || it.split >= it.nsplit ||
+      (it.nsplit > 1 && (it.part0 < 0 || it.part0 > p.parts_cap - it.nsplit || it.group < 0 || it.group > p.parts_cap / 2))) {
+    if (threadIdx.x == 0) raise_flag(MXFA_FLAG_BAD_ORDER);
+    return;
+  }
   // keys the block table can hold; a longer sequence is flagged and cut
   const int k_lim = min(it.total, p.BTW * p.PS);
   if (threadIdx.x == 0 && it.total > k_lim) raise_flag(MXFA_FLAG_TABLE_TOO_NARROW);
@@ -596,7 +670,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     __syncwarp();
    }
    if (warp == 1) {  // tensor memory goes back once the softmax warps have read it
-     named_barrier_sync(3, 256 + 32);
+     named_barrier_sync(3, kSoft + 32);
      tc_fence_after();
      tmem_dealloc(tmem, Cfg::kTmemCols);
    }
@@ -799,7 +873,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       ok = __all_sync(0xffffffffu, tc_wait(&bars->q_ready, 0, abort));
       row_scale = sc * reinterpret_cast<const float*>(sm + Cfg::kQScale)[r];
     }
-    for (int j = g; j < nkt && ok; j += 2) {
+    for (int j = g; j < nkt && ok; j += NG) {
       const int buf = j % NB;
       if (!__all_sync(0xffffffffu, tc_wait(&bars->s_full[buf], (j / NB) & 1, abort))) {
         ok = false;
@@ -939,13 +1013,16 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     fence_proxy_async_smem();
     ml[(g * 2) * kTcRows + r] = m_own;
     ml[(g * 2 + 1) * kTcRows + r] = l_own;
-    named_barrier_sync(1, 256);
+    named_barrier_sync(1, kSoft);
     tc_fence_after();
-    const float m0 = ml[r], m1 = ml[2 * kTcRows + r];
-    const float M = fmaxf(m0, m1);
-    // a sum at maximum -inf is 0, or NaN when every score it saw was
-    float L = ml[kTcRows + r] * (m0 == -INFINITY ? 1.f : fast_exp2(m0 - M));
-    L += ml[3 * kTcRows + r] * (m1 == -INFINITY ? 1.f : fast_exp2(m1 - M));
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int gg = 0; gg < NG; ++gg) M = fmaxf(M, ml[(gg * 2) * kTcRows + r]);
+#pragma unroll
+    for (int gg = 0; gg < NG; ++gg) {
+      const float mg = ml[(gg * 2) * kTcRows + r], lg = ml[(gg * 2 + 1) * kTcRows + r];
+      L += lg * (mg == -INFINITY ? 1.f : fast_exp2(mg - M));  // at maximum -inf a sum is 0, or NaN when every score was
+    }
     const bool split = it.nsplit > 1;
     const float inv = split ? 1.f : (L != 0.f ? 1.f / L : 0.f);
     const int head = hk * p.GQ + r % p.GQ;
@@ -954,7 +1031,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     T* orow = static_cast<T*>(p.out) + R * HD;
     if (warp_live && done_ok) {
       const bool patch = *any_bad != 0;
-      for (int c = g * 32; c < HD; c += 64) {
+      for (int c = g * 32; c < HD; c += 32 * NG) {
         uint32_t o[32];
         if (nkt > 0)
           tmem_ld32(o_base + c, o);
@@ -1001,45 +1078,77 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         p.lse[R] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
     }
     tc_fence_before();
-    named_barrier_arrive(3, 256 + 32);  // tensor memory is read
+    named_barrier_arrive(3, kSoft + 32);  // tensor memory is read
     if (split) {
       // publish this part; the last one of the tile merges them all, in split order
       __threadfence();
-      named_barrier_sync(1, 256);
+      named_barrier_sync(1, kSoft);
       unsigned* counter = p.counters + static_cast<size_t>(hk) * (p.parts_cap / 2 + 1) + it.group;
       const int tid = threadIdx.x - 128;
       if (tid == 0) *s_last = atomicAdd(counter, 1u) == static_cast<unsigned>(it.nsplit) - 1u;
-      named_barrier_sync(1, 256);
+      named_barrier_sync(1, kSoft);
       if (*s_last) {
         __threadfence();
+        // Weights first, one thread per row, over the K and V stages (every
+        // product is done): w = 2^(m_z - M) / L.  Then O = sum w_z O_z, four
+        // loads in flight per thread.
         const size_t first = (static_cast<size_t>(hk) * p.parts_cap + it.part0) * kTcRows;
-        constexpr int kQuads = HD / 4;
-        for (int idx = tid; idx < nrows * kQuads; idx += 256) {
-          const int rr = idx / kQuads, d4 = (idx % kQuads) * 4;
-          const float* po = p.part_o + (first + rr) * HD + d4;
-          const float* pm = p.part_ml + (first + rr) * 2;
-          float Mx = -INFINITY;
-          for (int z = 0; z < it.nsplit; ++z) Mx = fmaxf(Mx, __ldcg(pm + static_cast<size_t>(z) * kTcRows * 2));
-          float Ls = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float* wz = reinterpret_cast<float*>(sm + Cfg::kK);  // [part][row]
+        static_assert(2 * Cfg::kStages * Cfg::kTile + Cfg::kRawBytes >= kChunkMaxParts * kTcRows * 4, "room for weights");
+        if (tid < nrows) {
+          const float2* pm = reinterpret_cast<const float2*>(p.part_ml) + first + tid;
+          float Mx = -INFINITY, Ls = 0.f;
+#pragma unroll 8
+          for (int z = 0; z < it.nsplit; ++z) Mx = fmaxf(Mx, __ldcg(pm + static_cast<size_t>(z) * kTcRows).x);
+#pragma unroll 8
           for (int z = 0; z < it.nsplit; ++z) {
-            const float2 s = __ldcg(reinterpret_cast<const float2*>(pm + static_cast<size_t>(z) * kTcRows * 2));
-            if (s.x == -INFINITY && s.y == 0.f) continue;  // a part that saw no key
-            const float w = s.x == -INFINITY ? 1.f : fast_exp2(s.x - Mx);
-            const float4 o4 = __ldcg(reinterpret_cast<const float4*>(po + static_cast<size_t>(z) * kTcRows * HD));
+            const float2 s = __ldcg(pm + static_cast<size_t>(z) * kTcRows);
+            // a part at -inf saw no key (sum 0), or only NaN scores
+            const float w = s.x != -INFINITY ? fast_exp2(s.x - Mx) : s.y == 0.f ? 0.f : 1.f;
             Ls = fmaf(s.y, w, Ls);
-            acc.x = fmaf(o4.x, w, acc.x);
-            acc.y = fmaf(o4.y, w, acc.y);
-            acc.z = fmaf(o4.z, w, acc.z);
-            acc.w = fmaf(o4.w, w, acc.w);
+            wz[z * kTcRows + tid] = w;
           }
           const float iv = Ls != 0.f ? 1.f / Ls : 0.f;
-          const size_t RR = static_cast<size_t>(it.row0 + rr / p.GQ) * p.HQ + hk * p.GQ + rr % p.GQ;
-          uint2 v;
-          v.x = Elem<T>::pack(acc.x * iv, acc.y * iv);
-          v.y = Elem<T>::pack(acc.z * iv, acc.w * iv);
-          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + RR * HD + d4) = v;
-          if (d4 == 0 && p.lse != nullptr) p.lse[RR] = Ls != 0.f ? (Mx + log2f(Ls)) * kLn2 : -INFINITY;
+          for (int z = 0; z < it.nsplit; ++z) wz[z * kTcRows + tid] *= iv;
+          const size_t RR = static_cast<size_t>(it.row0 + tid / p.GQ) * p.HQ + hk * p.GQ + tid % p.GQ;
+          if (p.lse != nullptr) p.lse[RR] = Ls != 0.f ? (Mx + log2f(Ls)) * kLn2 : -INFINITY;
+        }
+        named_barrier_sync(1, kSoft);
+        constexpr int kQuads = HD / 4, kBatch = 4;
+        for (int idx0 = tid; idx0 < nrows * kQuads; idx0 += kSoft * kBatch) {
+          float4 acc[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int z = 0; z < it.nsplit; ++z) {
+            const float* po = p.part_o + (first + static_cast<size_t>(z) * kTcRows) * HD;
+            float4 o4[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+              const int idx = idx0 + u * kSoft;
+              o4[u] = idx < nrows * kQuads ? __ldcg(reinterpret_cast<const float4*>(po) + idx) : acc[0];
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+              const int row = min(idx0 + u * kSoft, nrows * kQuads - 1) / kQuads;
+              const float w = wz[z * kTcRows + row];
+              if (w == 0.f) continue;  // its O may be anything
+              acc[u].x = fmaf(o4[u].x, w, acc[u].x);
+              acc[u].y = fmaf(o4[u].y, w, acc[u].y);
+              acc[u].z = fmaf(o4[u].z, w, acc[u].z);
+              acc[u].w = fmaf(o4[u].w, w, acc[u].w);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int idx = idx0 + u * kSoft;
+            if (idx >= nrows * kQuads) break;
+            const int row = idx / kQuads, d4 = (idx % kQuads) * 4;
+            const size_t RR = static_cast<size_t>(it.row0 + row / p.GQ) * p.HQ + hk * p.GQ + row % p.GQ;
+            uint2 v;
+            v.x = Elem<T>::pack(acc[u].x, acc[u].y);
+            v.y = Elem<T>::pack(acc[u].z, acc[u].w);
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + RR * HD + d4) = v;
+          }
         }
         if (tid == 0) *counter = 0u;
       }
