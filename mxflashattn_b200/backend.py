@@ -25,6 +25,13 @@ from . import _lib
 SUPPORTED_DTYPES = (torch.float16, torch.bfloat16)
 
 
+# torch's own unwrapped queries of the current device and stream: a tenth of the time of the public
+# functions, which build a context check or a Stream object around them
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = torch.cuda.is_current_stream_capturing
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 _AVAILABLE: dict[int, bool] = {}
 
 
@@ -37,7 +44,7 @@ def is_available() -> bool:
         if not torch.cuda.is_available():
             return False
         _CUDA_OK.append(True)
-    dev = torch.cuda.current_device()
+    dev = _current_device()
     cached = _AVAILABLE.get(dev)
     if cached is not None:
         return cached
@@ -71,7 +78,7 @@ _NULL_CTX = contextlib.nullcontext()
 def _on(t: torch.Tensor):
     """Device context for a launch: a no-op when ``t`` already lives on the current device."""
     idx = t.device.index
-    return _NULL_CTX if idx == torch.cuda.current_device() else torch.cuda.device(idx)
+    return _NULL_CTX if idx == _current_device() else torch.cuda.device(idx)
 
 
 _LIB: list = []
@@ -85,7 +92,7 @@ def _L():
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.device.index)
 
 
 # ------------------------------------------------------------------ prefill
@@ -138,7 +145,7 @@ def kvcache_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, head_dim: 
     """(num_splits, chunk_len) the library picks for this shape on the current device (cached)."""
     import ctypes
 
-    key = (torch.cuda.current_device() if (_CUDA_OK or torch.cuda.is_available()) else -1, batch, q_len, q_heads,
+    key = (_current_device() if (_CUDA_OK or torch.cuda.is_available()) else -1, batch, q_len, q_heads,
            kv_heads, head_dim, max_len)
     plan = _PLANS.get(key)
     if plan is None:
@@ -150,6 +157,7 @@ def kvcache_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, head_dim: 
 
 
 _COUNTERS: dict[tuple, "torch.Tensor"] = {}
+_OUTGROWN: list["torch.Tensor"] = []
 
 
 def split_counters(device, stream_handle: int, nbytes: int):
@@ -162,6 +170,8 @@ def split_counters(device, stream_handle: int, nbytes: int):
     buf = _COUNTERS.get(key)
     n = max(nbytes // 4, 1)
     if buf is None or buf.numel() < n:
+        if buf is not None:
+            _OUTGROWN.append(buf)  # a captured graph may still replay with it
         buf = _COUNTERS[key] = torch.zeros((max(n, 4096),), device=device, dtype=torch.int32)
     return buf
 
@@ -420,12 +430,32 @@ def kvcache_gather_varlen(k_cache, v_cache, cu_seqlens, cache_seqlens, block_tab
     _lib.check(rc, "mxfa_kvcache_gather_varlen_launch")
 
 
+_SCRATCH: dict[tuple, "torch.Tensor"] = {}
+_SCRATCH_KEEP = 64 << 20
+
+
+def _scratch(q, stream_handle: int, nbytes: int):
+    """Workspace for launches ordered on one (device, stream): kept and grown up to 64 MB, larger ones per call.
+
+    Nothing in it outlives the launch that writes it, so launches ordered on
+    the stream share it, as they share the split counters.
+    """
+    # a captured launch replays with the pointer it was given: its workspace belongs to the graph
+    if nbytes > _SCRATCH_KEEP or (q.is_cuda and _capturing()):
+        return q.new_empty((nbytes,), dtype=torch.uint8)
+    key = (q.device, stream_handle)
+    buf = _SCRATCH.get(key)
+    if buf is None or buf.shape[0] < nbytes:
+        buf = _SCRATCH[key] = q.new_empty((nbytes,), dtype=torch.uint8)
+    return buf
+
+
 _CHUNK_SIZES: dict[tuple, tuple[int, int]] = {}
 
 
 def _chunk_sizes(kv_heads: int, head_dim: int) -> tuple[int, int]:
     """(workspace bytes, counter bytes) of the tiled attention on the current device (cached)."""
-    key = (torch.cuda.current_device() if (_CUDA_OK or torch.cuda.is_available()) else -1, kv_heads, head_dim)
+    key = (_current_device() if (_CUDA_OK or torch.cuda.is_available()) else -1, kv_heads, head_dim)
     sizes = _CHUNK_SIZES.get(key)
     if sizes is None:
         lib = _L()
@@ -461,9 +491,9 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
     cu, seq, bt = _i32(cu_seqlens_q), _i32(cache_seqlens), _i32(block_table)
     Tq, HQ, D = q.shape
     if out is None:
-        out = torch.empty((Tq, HQ, D), device=q.device, dtype=q.dtype)
-    lse = torch.empty((Tq, HQ), device=q.device, dtype=torch.float32) if return_lse else None
-    PS, HKV = k_cache.shape[1], k_cache.shape[2]
+        out = q.new_empty((Tq, HQ, D))
+    lse = q.new_empty((Tq, HQ), dtype=torch.float32) if return_lse else None
+    pages, PS, HKV, _ = k_cache.shape
     B = seq.shape[0]
     lib = _L()
     with _on(q):
@@ -476,14 +506,14 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
             ws, ws_bytes = None, 0
             if splits > 1:
                 ws_bytes = int(lib.mxfa_split_workspace_bytes(Tq * HQ, D, splits))
-                ws = torch.empty((ws_bytes // 4,), device=q.device, dtype=torch.float32)
+                ws = _scratch(q, stream, ws_bytes)
             counters = split_counters(q.device, stream, int(lib.mxfa_split_counter_bytes(B, 1, HQ, HKV)))
             name = "mxfa_kvcache_step_attention_launch"
             rc = lib.mxfa_kvcache_step_attention_launch(
                 q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales),
                 cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), None if plan is None else _lib.ptr(plan.order),
                 out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), ws_bytes, counters.data_ptr(), Tq, B, 1, HQ, HKV, D, PS,
-                bt.shape[1], k_cache.shape[0], splits, chunk, int(causal), _bf16(q), float(softmax_scale), stream)
+                bt.shape[1], pages, splits, chunk, int(causal), _bf16(q), float(softmax_scale), stream)
             _lib.check(rc, name)
             return (out, lse) if return_lse else out
         table = ws = counters = None
@@ -491,14 +521,13 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
         if Tq and B and PS % 8 == 0 and HQ // HKV <= _MAX_GROUP:
             table = kvcache_chunk_plan(cu, seq, Tq, HQ, HKV, causal) if plan is None else plan.table
             ws_bytes, counter_bytes = _chunk_sizes(HKV, D)
-            ws = torch.empty((ws_bytes // 4,), device=q.device, dtype=torch.float32)
+            ws = _scratch(q, stream, ws_bytes)
             counters = split_counters(q.device, stream, counter_bytes)
         rc = lib.mxfa_kvcache_varlen_attention_launch(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales),
             cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), _lib.ptr(table), 0 if table is None else table.numel() * 4,
             out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), ws_bytes, _lib.ptr(counters), Tq, B, HQ, HKV, D,
-            PS, bt.shape[1], k_cache.shape[0], q.stride(0), q.stride(1), int(causal), _bf16(q), float(softmax_scale),
-            stream)
+            PS, bt.shape[1], pages, q.stride(0), q.stride(1), int(causal), _bf16(q), float(softmax_scale), stream)
     _lib.check(rc, "mxfa_kvcache_varlen_attention_launch")
     return (out, lse) if return_lse else out
 

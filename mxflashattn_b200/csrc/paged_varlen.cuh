@@ -68,15 +68,38 @@ struct PagedVarlenParams {
 constexpr int kPvThreads = 256;
 constexpr int kPvMaxTok = 32;  // tokens of one CTA
 
-// The cache rows of this CTA's tokens, one warp per token: -1 not mapped.
+// The cache rows of this CTA's tokens (-1: not mapped), a token per lane of
+// the first warp: one search for the first token, then each lane walks on to
+// its own (consecutive tokens share sequences), so a CTA waits for three
+// dependent loads however many tokens it has.
 __device__ __forceinline__ void cta_token_rows(const PagedVarlenParams& p, int t0, int n, long long* rows) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = warp; i < n; i += kPvThreads / 32) {
-    const int t = t0 + i;
-    const int b = token_sequence(p.cu, p.B, t, lane);
-    if (lane == 0)
-      rows[i] = b < p.B ? paged_row(p.bt, b, p.seqlens[b] - p.cu[b + 1] + t, p.PS, p.BTW, p.P) : -1;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, t = t0 + lane;
+    int b = token_sequence(p.cu, p.B, t0, lane);
+    if (lane < n) {
+      while (b < p.B && p.cu[b + 1] <= t) ++b;
+      rows[lane] = b < p.B ? paged_row(p.bt, b, p.seqlens[b] - p.cu[b + 1] + t, p.PS, p.BTW, p.P) : -1;
+    }
   }
+  __syncthreads();
+}
+
+// A CTA's share of its rows (token, K heads then V heads): groups of D/8
+// lanes take a row each; with fewer rows per token than groups, several
+// tokens go side by side.  A thread keeps its head and walks tokens, kPvBatch
+// rows at a time with their loads in flight together.
+constexpr int kPvBatch = 4;
+struct RowWalk {
+  int pair, tok, step;  // first (K|V, head) pair, first token, tokens apart
+  bool live;
+};
+template <int kGroup>
+__device__ __forceinline__ RowWalk row_walk(int per_tok) {
+  constexpr int kGroups = kPvThreads / kGroup;
+  const int g = threadIdx.x / kGroup;
+  if (per_tok >= kGroups) return {g, 0, 1, true};
+  const int side = kGroups / per_tok;
+  return {g % per_tok, g / per_tok, side, g / per_tok < side};
 }
 
 // Exponent k of the row scale 2^k for the largest finite magnitude amax:
@@ -99,67 +122,74 @@ __global__ void __launch_bounds__(kPvThreads) append_varlen_kernel(const PagedVa
   const int t0 = blockIdx.x * p.tok_per_cta;
   const int n = min(p.tok_per_cta, p.T - t0);
   cta_token_rows(p, t0, n, s_rows);
-  __syncthreads();
   const int sub = threadIdx.x % kGroup;
-  const int per_tok = 2 * p.HKV;  // K heads, then V heads
-  const int total = n * per_tok;
-  // every lane of a warp runs the same number of rounds: the shuffles below
-  // need all of them
-  for (int base = 0; base < total; base += kPvThreads / kGroup) {
-    const int idx = base + threadIdx.x / kGroup;
-    const int i = idx / per_tok;
-    const int kv = (idx - i * per_tok) / p.HKV;
-    const int h = idx - i * per_tok - kv * p.HKV;
-    const long long row = idx < total ? s_rows[i] : -1;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (row >= 0) {
-      const T* src = kv ? static_cast<const T*>(p.v) + static_cast<size_t>(t0 + i) * p.v_tok + h * p.v_head
-                        : static_cast<const T*>(p.k) + static_cast<size_t>(t0 + i) * p.k_tok + h * p.k_head;
-      src += sub * 8;
-      if constexpr (kVec) {
-        raw = *reinterpret_cast<const uint4*>(src);
-      } else {
-        const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
-        raw.x = s16[0] | (static_cast<uint32_t>(s16[1]) << 16);
-        raw.y = s16[2] | (static_cast<uint32_t>(s16[3]) << 16);
-        raw.z = s16[4] | (static_cast<uint32_t>(s16[5]) << 16);
-        raw.w = s16[6] | (static_cast<uint32_t>(s16[7]) << 16);
-      }
-    }
+  const RowWalk walk = row_walk<kGroup>(2 * p.HKV);
+  // loop bounds are the same for every lane: the shuffles need all of them
+  for (int pair0 = 0; pair0 < 2 * p.HKV; pair0 += kPvThreads / kGroup) {
+    const int pair = pair0 + walk.pair;
+    const bool live = walk.live && pair < 2 * p.HKV;
+    const int kv = pair >= p.HKV, h = live ? pair - kv * p.HKV : 0;
+    const T* src = kv ? static_cast<const T*>(p.v) + h * p.v_head : static_cast<const T*>(p.k) + h * p.k_head;
+    const size_t stride = kv ? p.v_tok : p.k_tok;
     uint8_t* cache = kv ? p.v_cache : p.k_cache;
-    if constexpr (!kQuant) {
-      if (row >= 0) *reinterpret_cast<uint4*>(cache + ((row * p.HKV + h) * HD + sub * 8) * 2) = raw;
-    } else {
-      const float2 a = Elem<T>::unpack(raw.x), b = Elem<T>::unpack(raw.y);
-      const float2 c = Elem<T>::unpack(raw.z), d = Elem<T>::unpack(raw.w);
-      const float x[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-      // the maximum is over finite values: an infinity saturates to 448 s and
-      // a NaN stays a NaN, and neither costs the rest of its row
-      float amax = 0.f;
+    for (int i0 = 0; i0 < n; i0 += walk.step * kPvBatch) {
+      long long row[kPvBatch];
+      uint4 raw[kPvBatch];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float m = fabsf(x[j]);
-        amax = m < INFINITY ? fmaxf(amax, m) : amax;
+      for (int u = 0; u < kPvBatch; ++u) {
+        const int i = i0 + walk.tok + u * walk.step;
+        row[u] = live && i < n ? s_rows[i] : -1;
+        raw[u] = make_uint4(0, 0, 0, 0);
+        if (row[u] >= 0) {
+          const T* at = src + static_cast<size_t>(t0 + i) * stride + sub * 8;
+          if constexpr (kVec) {
+            raw[u] = *reinterpret_cast<const uint4*>(at);
+          } else {
+            const uint16_t* s16 = reinterpret_cast<const uint16_t*>(at);
+            raw[u].x = s16[0] | (static_cast<uint32_t>(s16[1]) << 16);
+            raw[u].y = s16[2] | (static_cast<uint32_t>(s16[3]) << 16);
+            raw[u].z = s16[4] | (static_cast<uint32_t>(s16[5]) << 16);
+            raw[u].w = s16[6] | (static_cast<uint32_t>(s16[7]) << 16);
+          }
+        }
       }
 #pragma unroll
-      for (int sh = kGroup / 2; sh > 0; sh >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
-      const int k = scale_exponent(amax);
-      const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-      uint32_t q[2];
+      for (int u = 0; u < kPvBatch; ++u) {
+        if constexpr (!kQuant) {
+          if (row[u] >= 0) *reinterpret_cast<uint4*>(cache + ((row[u] * p.HKV + h) * HD + sub * 8) * 2) = raw[u];
+        } else {
+          const float2 a = Elem<T>::unpack(raw[u].x), b = Elem<T>::unpack(raw[u].y);
+          const float2 c = Elem<T>::unpack(raw[u].z), d = Elem<T>::unpack(raw[u].w);
+          const float x[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+          // the maximum is over finite values: an infinity saturates to 448 s
+          // and a NaN stays a NaN, and neither costs the rest of its row
+          float amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * j] * inv, x[4 * j + 1] * inv), __NV_SATFINITE,
-                                                     __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * j + 2] * inv, x[4 * j + 3] * inv),
-                                                     __NV_SATFINITE, __NV_E4M3);
-        q[j] = lo | (hi << 16);
-      }
-      if (row >= 0) {
-        *reinterpret_cast<uint2*>(cache + (row * p.HKV + h) * HD + sub * 8) = make_uint2(q[0], q[1]);
-        if (sub == 0) {
-          const long long page = row / p.PS;
-          (kv ? p.v_scales : p.k_scales)[(page * p.HKV + h) * p.PS + (row - page * p.PS)] =
-              static_cast<uint8_t>(k + 127);
+          for (int j = 0; j < 8; ++j) {
+            const float m = fabsf(x[j]);
+            amax = m < INFINITY ? fmaxf(amax, m) : amax;
+          }
+#pragma unroll
+          for (int sh = kGroup / 2; sh > 0; sh >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
+          const int k = scale_exponent(amax);
+          const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+          uint32_t q[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * j] * inv, x[4 * j + 1] * inv),
+                                                         __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * j + 2] * inv, x[4 * j + 3] * inv),
+                                                         __NV_SATFINITE, __NV_E4M3);
+            q[j] = lo | (hi << 16);
+          }
+          if (row[u] >= 0) {
+            *reinterpret_cast<uint2*>(cache + (row[u] * p.HKV + h) * HD + sub * 8) = make_uint2(q[0], q[1]);
+            if (sub == 0) {
+              const long long page = row[u] / p.PS;
+              (kv ? p.v_scales : p.k_scales)[(page * p.HKV + h) * p.PS + (row[u] - page * p.PS)] =
+                  static_cast<uint8_t>(k + 127);
+            }
+          }
         }
       }
     }
@@ -194,34 +224,47 @@ __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVa
   const int t0 = blockIdx.x * p.tok_per_cta;
   const int n = min(p.tok_per_cta, p.T - t0);
   cta_token_rows(p, t0, n, s_rows);
-  __syncthreads();
   const int sub = threadIdx.x % kGroup;
-  const int per_tok = 2 * p.HKV;
-  const int total = n * per_tok;
-  for (int idx = threadIdx.x / kGroup; idx < total; idx += kPvThreads / kGroup) {
-    const int i = idx / per_tok;
-    const int kv = (idx - i * per_tok) / p.HKV;
-    const int h = idx - i * per_tok - kv * p.HKV;
-    const long long row = s_rows[i];
+  const RowWalk walk = row_walk<kGroup>(2 * p.HKV);
+  if (!walk.live) return;
+  for (int pair = walk.pair; pair < 2 * p.HKV; pair += kPvThreads / kGroup) {
+    const int kv = pair >= p.HKV, h = pair - kv * p.HKV;
     const uint8_t* cache = kv ? p.v_cache : p.k_cache;
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (row >= 0) {
-      if constexpr (!kQuant) {
-        out = *reinterpret_cast<const uint4*>(cache + ((row * p.HKV + h) * HD + sub * 8) * 2);
-      } else {
-        const uint2 codes = *reinterpret_cast<const uint2*>(cache + (row * p.HKV + h) * HD + sub * 8);
-        const long long page = row / p.PS;
-        const float s =
-            e8m0_to_float((kv ? p.v_scales : p.k_scales)[(page * p.HKV + h) * p.PS + (row - page * p.PS)]);
-        float x[8];
-        dequant8(codes, s, x);
-        out = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
-                         Elem<T>::pack(x[6], x[7]));
+    const uint8_t* scales = kv ? p.v_scales : p.k_scales;
+    T* dst = static_cast<T*>(const_cast<void*>(kv ? p.v : p.k)) + static_cast<size_t>(t0) * p.HKV * HD + h * HD + sub * 8;
+    for (int i0 = walk.tok; i0 < n; i0 += walk.step * kPvBatch) {
+      uint4 out[kPvBatch];
+      uint2 codes[kPvBatch];
+      uint32_t byte[kPvBatch];
+#pragma unroll
+      for (int u = 0; u < kPvBatch; ++u) {
+        const int i = i0 + u * walk.step;
+        const long long row = i < n ? s_rows[i] : -1;
+        out[u] = make_uint4(0, 0, 0, 0);
+        codes[u] = make_uint2(0, 0);
+        byte[u] = 127;
+        if (row >= 0) {
+          if constexpr (!kQuant) {
+            out[u] = *reinterpret_cast<const uint4*>(cache + ((row * p.HKV + h) * HD + sub * 8) * 2);
+          } else {
+            const long long page = row / p.PS;
+            codes[u] = *reinterpret_cast<const uint2*>(cache + (row * p.HKV + h) * HD + sub * 8);
+            byte[u] = scales[(page * p.HKV + h) * p.PS + (row - page * p.PS)];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kPvBatch; ++u) {
+        const int i = i0 + u * walk.step;
+        if constexpr (kQuant) {
+          float x[8];
+          dequant8(codes[u], e8m0_to_float(byte[u]), x);
+          out[u] = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
+                              Elem<T>::pack(x[6], x[7]));
+        }
+        if (i < n) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(i) * p.HKV * HD) = out[u];
       }
     }
-    T* dst = static_cast<T*>(const_cast<void*>(kv ? p.v : p.k)) +
-             (static_cast<size_t>(t0 + i) * p.HKV + h) * HD + sub * 8;
-    *reinterpret_cast<uint4*>(dst) = out;
   }
 }
 

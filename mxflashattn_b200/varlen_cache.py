@@ -35,11 +35,44 @@ from .validation import validate_softmax_scale
 _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
 _HALF = (torch.float16, torch.bfloat16)
+_INDEX = (torch.int32, torch.int64)
 
 
 def _require(ok: bool, message: str, error=ValueError) -> None:
     if not ok:
         raise error(message)
+
+
+def _quick(check) -> bool:
+    """Whether ``check()`` holds; arguments that are not tensors make it False.
+
+    The checks below name what is wrong, one at a time, which costs a call
+    more than its kernel's launch.  So each entry point asks one combined
+    question first and goes through them only when its answer is no.
+    """
+    try:
+        return check()
+    except (AttributeError, TypeError, IndexError):
+        return False
+
+
+def _plain_caches(kc, vc, ks, vs) -> bool:
+    s, d, dt = kc.shape, kc.device, kc.dtype
+    if not (len(s) == 4 and vc.shape == s and vc.dtype == dt and vc.device == d and (s[3] == 128 or s[3] == 64)
+            and s[0] > 0 and s[1] > 0 and s[2] > 0 and kc.is_contiguous() and vc.is_contiguous()):
+        return False
+    if dt != _E4M3:
+        return dt in _HALF and ks is None and vs is None
+    want = (s[0], s[2], s[1])
+    return (ks.dtype == _E8M0 and vs.dtype == _E8M0 and ks.shape == want and vs.shape == want and ks.device == d
+            and vs.device == d and ks.is_contiguous() and vs.is_contiguous())
+
+
+def _plain_batch(cu, seq, bt, d) -> bool:
+    b, w = bt.shape
+    return (bt.dtype in _INDEX and cu.dtype in _INDEX and seq.dtype in _INDEX and seq.ndim == 1 and cu.ndim == 1
+            and seq.shape[0] == b and cu.shape[0] == b + 1 and (w > 0 or b == 0) and cu.device == d
+            and seq.device == d and bt.device == d)
 
 
 def _validate_caches(k_cache, v_cache, k_scales, v_scales) -> bool:
@@ -110,6 +143,21 @@ def _strict() -> bool:
     return os.getenv("MXFLASHATTN_STRICT_VALIDATION", "0") == "1"
 
 
+def _validate_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, k_scales, v_scales) -> None:
+    quant = _validate_caches(k_cache, v_cache, k_scales, v_scales)
+    for name, t in (("k", k), ("v", v)):
+        _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor", TypeError)
+        _require(t.ndim == 3 and t.shape[1:] == k_cache.shape[2:],
+                 f"{name} must have rank 3 with layout [total_tokens, kv_heads, dim] matching the cache")
+        _require(t.device == k_cache.device, f"{name} must be on the cache's device")
+        _require(t.dtype in _HALF, f"{name} must be float16 or bfloat16", TypeError)
+    _require(k.shape == v.shape, "k and v must have identical shapes")
+    _require(k.dtype == v.dtype, "k and v must have the same dtype")
+    _require(quant or k.dtype == k_cache.dtype, "k and v must have the cache's dtype")
+    _validate_batch(cu_seqlens, cache_seqlens, block_table, k_cache.device)
+    _require(block_table is not None, "block_table is required")
+
+
 def kvcache_append_varlen(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -132,18 +180,12 @@ def kvcache_append_varlen(
     ``k`` and ``v`` may be strided views (slices of a fused projection); rows
     past ``cu_seqlens[-1]`` are padding and are not written.
     """
-    quant = _validate_caches(k_cache, v_cache, k_scales, v_scales)
-    for name, t in (("k", k), ("v", v)):
-        _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor", TypeError)
-        _require(t.ndim == 3 and t.shape[1:] == k_cache.shape[2:],
-                 f"{name} must have rank 3 with layout [total_tokens, kv_heads, dim] matching the cache")
-        _require(t.device == k_cache.device, f"{name} must be on the cache's device")
-        _require(t.dtype in _HALF, f"{name} must be float16 or bfloat16", TypeError)
-    _require(k.shape == v.shape, "k and v must have identical shapes")
-    _require(k.dtype == v.dtype, "k and v must have the same dtype")
-    _require(quant or k.dtype == k_cache.dtype, "k and v must have the cache's dtype")
-    _validate_batch(cu_seqlens, cache_seqlens, block_table, k_cache.device)
-    _require(block_table is not None, "block_table is required")
+    if not _quick(lambda: _plain_caches(k_cache, v_cache, k_scales, v_scales)
+                  and _plain_batch(cu_seqlens, cache_seqlens, block_table, k_cache.device)
+                  and k.ndim == 3 and k.shape == v.shape and k.shape[1:] == k_cache.shape[2:] and k.dtype == v.dtype
+                  and k.dtype in _HALF and (k_scales is not None or k.dtype == k_cache.dtype)
+                  and k.device == k_cache.device and v.device == k_cache.device):
+        _validate_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, k_scales, v_scales)
     if _strict():
         _strict_batch_checks(cu_seqlens, cache_seqlens, block_table, k.shape[0], k_cache.shape[1], k_cache.shape[0],
                              True)
@@ -170,21 +212,26 @@ def kvcache_gather_varlen(
     bfloat16, the default).  A 16-bit cache is copied bit for bit.  Rows that
     no sequence owns, or whose page the table does not have, are zero.
     """
-    quant = _validate_caches(k_cache, v_cache, k_scales, v_scales)
+    quant = k_scales is not None
+    if not _quick(lambda: _plain_caches(k_cache, v_cache, k_scales, v_scales)
+                  and _plain_batch(cu_seqlens, cache_seqlens, block_table, k_cache.device)):
+        quant = _validate_caches(k_cache, v_cache, k_scales, v_scales)
+        _validate_batch(cu_seqlens, cache_seqlens, block_table, k_cache.device)
+        _require(block_table is not None, "block_table is required")
     if dtype is None:
         dtype = torch.bfloat16 if quant else k_cache.dtype
-    _require(dtype in _HALF, "dtype must be float16 or bfloat16", TypeError)
-    _require(quant or dtype == k_cache.dtype, "a 16-bit cache is read back in its own dtype")
-    _validate_batch(cu_seqlens, cache_seqlens, block_table, k_cache.device)
-    _require(block_table is not None, "block_table is required")
+    if not (dtype in _HALF and (quant or dtype == k_cache.dtype)):
+        _require(dtype in _HALF, "dtype must be float16 or bfloat16", TypeError)
+        _require(quant or dtype == k_cache.dtype, "a 16-bit cache is read back in its own dtype")
     total_tokens = int(total_tokens)
-    _require(total_tokens >= 0, "total_tokens must be non-negative")
+    if total_tokens < 0:
+        raise ValueError("total_tokens must be non-negative")
     if _strict():
         _strict_batch_checks(cu_seqlens, cache_seqlens, block_table, total_tokens, k_cache.shape[1],
                              k_cache.shape[0], True)
     shape = (total_tokens, *k_cache.shape[2:])
-    k = torch.empty(shape, device=k_cache.device, dtype=dtype)
-    v = torch.empty(shape, device=k_cache.device, dtype=dtype)
+    k = k_cache.new_empty(shape, dtype=dtype)
+    v = k_cache.new_empty(shape, dtype=dtype)
     dispatch("kvcache_gather_varlen", k,
              (k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, k_scales, v_scales, k, v))
     return k, v
@@ -206,6 +253,7 @@ class KvChunkPlan:
     causal: bool
     table: torch.Tensor | None
     order: torch.Tensor | None = None
+    device: torch.device | None = None
 
 
 def kvcache_chunk_plan(
@@ -236,7 +284,40 @@ def kvcache_chunk_plan(
 
     table = backend.kvcache_chunk_plan(cu_seqlens_q, cache_seqlens, int(total_q), q_heads, kv_heads, causal)
     return KvChunkPlan(int(total_q), batch, int(max_seqlen_q), int(q_heads), int(kv_heads), bool(causal), table,
-                       backend.kvcache_length_order(cache_seqlens) if max_seqlen_q <= 1 and batch else None)
+                       backend.kvcache_length_order(cache_seqlens) if max_seqlen_q <= 1 and batch else None,
+                       cu_seqlens_q.device)
+
+
+def _plan_fits(plan, q, k_cache, cache_seqlens, max_seqlen_q, causal) -> bool:
+    """Whether ``plan`` was made for a batch of these counts."""
+    return (plan.total_q == q.shape[0] and plan.batch == cache_seqlens.shape[0] and plan.max_seqlen_q == max_seqlen_q
+            and plan.q_heads == q.shape[1] and plan.kv_heads == k_cache.shape[2] and plan.causal == bool(causal)
+            and plan.device == q.device)
+
+
+def _validate_attention(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q, max_seqlen_k,
+                        softmax_scale, causal, k_scales, v_scales, plan, out) -> None:
+    validate_softmax_scale(softmax_scale)
+    quant = _validate_caches(k_cache, v_cache, k_scales, v_scales)
+    _require(isinstance(q, torch.Tensor), "q must be a torch.Tensor", TypeError)
+    _require(q.ndim == 3, "q must have rank 3 with layout [total_tokens, heads, dim]")
+    _require(q.device == k_cache.device, "q must be on the cache's device")
+    _require(q.shape[2] == k_cache.shape[3], "q and the cache must have the same head dimension")
+    _require(q.shape[1] > 0 and q.shape[1] % k_cache.shape[2] == 0, "q heads must be a positive multiple of kv heads")
+    _require(q.dtype in _HALF, "q must be float16 or bfloat16", TypeError)
+    _require(quant or q.dtype == k_cache.dtype, "q must have the cache's dtype")
+    _validate_batch(cu_seqlens_q, cache_seqlens, block_table, k_cache.device, "cu_seqlens_q")
+    _require(block_table is not None, "block_table is required")
+    _require(max_seqlen_q >= 0, "max_seqlen_q must be non-negative")
+    _require(max_seqlen_k is None or max_seqlen_k >= 0, "max_seqlen_k must be non-negative")
+    if plan is not None:
+        _require(isinstance(plan, KvChunkPlan), "plan must come from kvcache_chunk_plan", TypeError)
+        _require(_plan_fits(plan, q, k_cache, cache_seqlens, max_seqlen_q, causal),
+                 "plan was made for another batch")
+    if out is not None:
+        _require(isinstance(out, torch.Tensor) and out.shape == q.shape and out.dtype == q.dtype
+                 and out.device == q.device and out.is_contiguous(),
+                 "out must be a contiguous tensor with q's shape, dtype and device")
 
 
 def flash_attn_varlen_with_kvcache(
@@ -273,35 +354,27 @@ def flash_attn_varlen_with_kvcache(
     the result.  With ``return_softmax_lse`` the natural-log LSE [Tq, HQ]
     (float32) is returned too.
     """
-    validate_softmax_scale(softmax_scale)
-    quant = _validate_caches(k_cache, v_cache, k_scales, v_scales)
-    _require(isinstance(q, torch.Tensor), "q must be a torch.Tensor", TypeError)
-    _require(q.ndim == 3, "q must have rank 3 with layout [total_tokens, heads, dim]")
-    _require(q.device == k_cache.device, "q must be on the cache's device")
-    _require(q.shape[2] == k_cache.shape[3], "q and the cache must have the same head dimension")
-    _require(q.shape[1] > 0 and q.shape[1] % k_cache.shape[2] == 0, "q heads must be a positive multiple of kv heads")
-    _require(q.dtype in _HALF, "q must be float16 or bfloat16", TypeError)
-    _require(quant or q.dtype == k_cache.dtype, "q must have the cache's dtype")
-    batch = _validate_batch(cu_seqlens_q, cache_seqlens, block_table, k_cache.device, "cu_seqlens_q")
-    _require(block_table is not None, "block_table is required")
     max_seqlen_q = int(max_seqlen_q)
-    _require(max_seqlen_q >= 0, "max_seqlen_q must be non-negative")
+    max_seqlen_k = None if max_seqlen_k is None else int(max_seqlen_k)
+    if softmax_scale is not None or not _quick(
+            lambda: _plain_caches(k_cache, v_cache, k_scales, v_scales)
+            and _plain_batch(cu_seqlens_q, cache_seqlens, block_table, k_cache.device)
+            and q.ndim == 3 and q.shape[2] == k_cache.shape[3] and q.shape[1] > 0
+            and q.shape[1] % k_cache.shape[2] == 0 and q.device == k_cache.device
+            and q.dtype in _HALF and (k_scales is not None or q.dtype == k_cache.dtype)
+            and max_seqlen_q >= 0 and (max_seqlen_k is None or max_seqlen_k >= 0)
+            and (plan is None or _plan_fits(plan, q, k_cache, cache_seqlens, max_seqlen_q, causal))
+            and (out is None or (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device
+                                 and out.is_contiguous()))):
+        _validate_attention(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q, max_seqlen_k,
+                            softmax_scale, causal, k_scales, v_scales, plan, out)
     capacity = block_table.shape[1] * k_cache.shape[1]
-    max_seqlen_k = capacity if max_seqlen_k is None else int(max_seqlen_k)
-    _require(max_seqlen_k >= 0, "max_seqlen_k must be non-negative")
-    if plan is not None:
-        _require(isinstance(plan, KvChunkPlan), "plan must come from kvcache_chunk_plan", TypeError)
-        _require((plan.total_q, plan.batch, plan.max_seqlen_q, plan.q_heads, plan.kv_heads, plan.causal)
-                 == (q.shape[0], batch, max_seqlen_q, q.shape[1], k_cache.shape[2], bool(causal)),
-                 "plan was made for another batch")
-    if out is not None:
-        _require(isinstance(out, torch.Tensor) and out.shape == q.shape and out.dtype == q.dtype
-                 and out.device == q.device and out.is_contiguous(),
-                 "out must be a contiguous tensor with q's shape, dtype and device")
+    if max_seqlen_k is None or max_seqlen_k > capacity:
+        max_seqlen_k = capacity
     if _strict():
         _strict_batch_checks(cu_seqlens_q, cache_seqlens, block_table, q.shape[0], k_cache.shape[1],
                              k_cache.shape[0], False)
     return dispatch("flash_attn_varlen_with_kvcache", q,
                     (q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q,
-                     min(max_seqlen_k, capacity), _resolved_scale(q.shape[-1], softmax_scale), bool(causal), k_scales,
+                     max_seqlen_k, _resolved_scale(q.shape[-1], softmax_scale), bool(causal), k_scales,
                      v_scales, plan, out, bool(return_softmax_lse)))

@@ -115,6 +115,17 @@ def test_append_refusals():
         _append(a)
 
 
+def test_rows_that_are_already_codes_are_refused():
+    a = _args(quant=True)
+    a["k"] = a["v"] = a["k"].to(E4M3)
+    with pytest.raises(TypeError, match="float16 or bfloat16"):
+        _append(a)
+    b = _args(quant=True)
+    b["q"] = b["q"].to(E4M3)
+    with pytest.raises(TypeError, match="float16 or bfloat16"):
+        _attend(b)
+
+
 def test_gather_refusals():
     with pytest.raises(ValueError, match="non-negative"):
         _gather(_args(), total=-1)
