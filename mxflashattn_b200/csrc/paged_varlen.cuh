@@ -34,20 +34,27 @@ __device__ __forceinline__ int token_sequence(const int* __restrict__ cu, int B,
   return n;
 }
 
-// Cache row (page * PS + offset) of position pos of sequence b, or -1 with
-// the flag raised when the table or the cache does not have it.
-__device__ __forceinline__ long long paged_row(const int* __restrict__ bt, int b, int pos, int PS, int BTW, int P) {
+// Physical page and slot of position pos of sequence b; page -1, and the flag
+// raised, when the table or the cache does not have it.
+__device__ __forceinline__ int2 paged_slot(const int* __restrict__ bt, int b, int pos, int PS, int BTW, int P) {
   const int page = pos / PS;
   if (pos < 0 || page >= BTW) {
     raise_flag(MXFA_FLAG_TABLE_TOO_NARROW);
-    return -1;
+    return make_int2(-1, 0);
   }
   const int phys = bt[static_cast<size_t>(b) * BTW + page];
   if (phys < 0 || phys >= P) {
     raise_flag(MXFA_FLAG_PAGE_OUT_OF_RANGE);
-    return -1;
+    return make_int2(-1, 0);
   }
-  return static_cast<long long>(phys) * PS + (pos - page * PS);
+  return make_int2(phys, pos - page * PS);
+}
+// Element offset of a head's row in the cache, and of its scale.
+__device__ __forceinline__ size_t row_offset(int2 slot, int h, int PS, int HKV, int D) {
+  return ((static_cast<size_t>(slot.x) * PS + slot.y) * HKV + h) * D;
+}
+__device__ __forceinline__ size_t scale_offset(int2 slot, int h, int PS, int HKV) {
+  return (static_cast<size_t>(slot.x) * HKV + h) * PS + slot.y;
 }
 
 struct PagedVarlenParams {
@@ -66,19 +73,19 @@ struct PagedVarlenParams {
 };
 
 constexpr int kPvThreads = 256;
-constexpr int kPvMaxTok = 32;  // tokens of one CTA
+constexpr int kPvMaxTok = 16;  // tokens of one CTA (8 to 32 differ by 7%)
 
-// The cache rows of this CTA's tokens (-1: not mapped), a token per lane of
+// The cache slots of this CTA's tokens (page -1: not mapped), a token per lane of
 // the first warp: one search for the first token, then each lane walks on to
 // its own (consecutive tokens share sequences), so a CTA waits for three
 // dependent loads however many tokens it has.
-__device__ __forceinline__ void cta_token_rows(const PagedVarlenParams& p, int t0, int n, long long* rows) {
+__device__ __forceinline__ void cta_token_rows(const PagedVarlenParams& p, int t0, int n, int2* slots) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x, t = t0 + lane;
     int b = token_sequence(p.cu, p.B, t0, lane);
     if (lane < n) {
       while (b < p.B && p.cu[b + 1] <= t) ++b;
-      rows[lane] = b < p.B ? paged_row(p.bt, b, p.seqlens[b] - p.cu[b + 1] + t, p.PS, p.BTW, p.P) : -1;
+      slots[lane] = b < p.B ? paged_slot(p.bt, b, p.seqlens[b] - p.cu[b + 1] + t, p.PS, p.BTW, p.P) : make_int2(-1, 0);
     }
   }
   __syncthreads();
@@ -111,6 +118,15 @@ __device__ __forceinline__ int scale_exponent(float amax) {
   return max(k, -126);
 }
 
+// The value of a 16-bit pattern without sign.
+template <typename T>
+__device__ __forceinline__ float magnitude_to_float(uint32_t bits) {
+  if constexpr (std::is_same_v<T, __half>)
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+  else
+    return __uint_as_float(bits << 16);
+}
+
 // Append: a group of D/8 lanes moves one (token, KV head) row of K or V,
 // eight values a lane.  HBM-bound: each value is read once and its code (or
 // itself) written once; a group reduces its row's maximum by shuffles, so
@@ -118,10 +134,10 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 template <typename T, int HD, bool kQuant, bool kVec>
 __global__ void __launch_bounds__(kPvThreads) append_varlen_kernel(const PagedVarlenParams p) {
   constexpr int kGroup = HD / 8;
-  __shared__ long long s_rows[kPvMaxTok];
+  __shared__ int2 s_slots[kPvMaxTok];
   const int t0 = blockIdx.x * p.tok_per_cta;
   const int n = min(p.tok_per_cta, p.T - t0);
-  cta_token_rows(p, t0, n, s_rows);
+  cta_token_rows(p, t0, n, s_slots);
   const int sub = threadIdx.x % kGroup;
   const RowWalk walk = row_walk<kGroup>(2 * p.HKV);
   // loop bounds are the same for every lane: the shuffles need all of them
@@ -133,14 +149,14 @@ __global__ void __launch_bounds__(kPvThreads) append_varlen_kernel(const PagedVa
     const size_t stride = kv ? p.v_tok : p.k_tok;
     uint8_t* cache = kv ? p.v_cache : p.k_cache;
     for (int i0 = 0; i0 < n; i0 += walk.step * kPvBatch) {
-      long long row[kPvBatch];
+      int2 slot[kPvBatch];
       uint4 raw[kPvBatch];
 #pragma unroll
       for (int u = 0; u < kPvBatch; ++u) {
         const int i = i0 + walk.tok + u * walk.step;
-        row[u] = live && i < n ? s_rows[i] : -1;
+        slot[u] = live && i < n ? s_slots[i] : make_int2(-1, 0);
         raw[u] = make_uint4(0, 0, 0, 0);
-        if (row[u] >= 0) {
+        if (slot[u].x >= 0) {
           const T* at = src + static_cast<size_t>(t0 + i) * stride + sub * 8;
           if constexpr (kVec) {
             raw[u] = *reinterpret_cast<const uint4*>(at);
@@ -156,21 +172,32 @@ __global__ void __launch_bounds__(kPvThreads) append_varlen_kernel(const PagedVa
 #pragma unroll
       for (int u = 0; u < kPvBatch; ++u) {
         if constexpr (!kQuant) {
-          if (row[u] >= 0) *reinterpret_cast<uint4*>(cache + ((row[u] * p.HKV + h) * HD + sub * 8) * 2) = raw[u];
+          if (slot[u].x >= 0)
+            *reinterpret_cast<uint4*>(cache + (row_offset(slot[u], h, p.PS, p.HKV, HD) + sub * 8) * 2) = raw[u];
         } else {
+          // magnitudes compare as integers, two at a time
+          uint32_t top = __vmaxu2(__vmaxu2(raw[u].x & 0x7fff7fffu, raw[u].y & 0x7fff7fffu),
+                                  __vmaxu2(raw[u].z & 0x7fff7fffu, raw[u].w & 0x7fff7fffu));
+#pragma unroll
+          for (int sh = kGroup / 2; sh > 0; sh >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, sh));
+          top = max(top & 0xffffu, top >> 16);
+          constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+          float amax = magnitude_to_float<T>(top);
           const float2 a = Elem<T>::unpack(raw[u].x), b = Elem<T>::unpack(raw[u].y);
           const float2 c = Elem<T>::unpack(raw[u].z), d = Elem<T>::unpack(raw[u].w);
           const float x[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-          // the maximum is over finite values: an infinity saturates to 448 s
-          // and a NaN stays a NaN, and neither costs the rest of its row
-          float amax = 0.f;
+          if (__any_sync(0xffffffffu, top >= kInf)) {
+            // the maximum is over finite values: an infinity saturates to 448 s
+            // and a NaN stays a NaN, and neither costs the rest of its row
+            amax = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float m = fabsf(x[j]);
-            amax = m < INFINITY ? fmaxf(amax, m) : amax;
+            for (int j = 0; j < 8; ++j) {
+              const float m = fabsf(x[j]);
+              amax = m < INFINITY ? fmaxf(amax, m) : amax;
+            }
+#pragma unroll
+            for (int sh = kGroup / 2; sh > 0; sh >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
           }
-#pragma unroll
-          for (int sh = kGroup / 2; sh > 0; sh >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
           const int k = scale_exponent(amax);
           const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
           uint32_t q[2];
@@ -182,13 +209,10 @@ __global__ void __launch_bounds__(kPvThreads) append_varlen_kernel(const PagedVa
                                                          __NV_SATFINITE, __NV_E4M3);
             q[j] = lo | (hi << 16);
           }
-          if (row[u] >= 0) {
-            *reinterpret_cast<uint2*>(cache + (row[u] * p.HKV + h) * HD + sub * 8) = make_uint2(q[0], q[1]);
-            if (sub == 0) {
-              const long long page = row[u] / p.PS;
-              (kv ? p.v_scales : p.k_scales)[(page * p.HKV + h) * p.PS + (row[u] - page * p.PS)] =
-                  static_cast<uint8_t>(k + 127);
-            }
+          if (slot[u].x >= 0) {
+            *reinterpret_cast<uint2*>(cache + row_offset(slot[u], h, p.PS, p.HKV, HD) + sub * 8) = make_uint2(q[0], q[1]);
+            if (sub == 0)
+              (kv ? p.v_scales : p.k_scales)[scale_offset(slot[u], h, p.PS, p.HKV)] = static_cast<uint8_t>(k + 127);
           }
         }
       }
@@ -220,10 +244,10 @@ __device__ __forceinline__ void dequant8(uint2 codes, float s, float (&x)[8]) {
 template <typename T, int HD, bool kQuant>
 __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVarlenParams p) {
   constexpr int kGroup = HD / 8;
-  __shared__ long long s_rows[kPvMaxTok];
+  __shared__ int2 s_slots[kPvMaxTok];
   const int t0 = blockIdx.x * p.tok_per_cta;
   const int n = min(p.tok_per_cta, p.T - t0);
-  cta_token_rows(p, t0, n, s_rows);
+  cta_token_rows(p, t0, n, s_slots);
   const int sub = threadIdx.x % kGroup;
   const RowWalk walk = row_walk<kGroup>(2 * p.HKV);
   if (!walk.live) return;
@@ -239,17 +263,17 @@ __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVa
 #pragma unroll
       for (int u = 0; u < kPvBatch; ++u) {
         const int i = i0 + u * walk.step;
-        const long long row = i < n ? s_rows[i] : -1;
+        const int2 slot = i < n ? s_slots[i] : make_int2(-1, 0);
         out[u] = make_uint4(0, 0, 0, 0);
         codes[u] = make_uint2(0, 0);
         byte[u] = 127;
-        if (row >= 0) {
+        if (slot.x >= 0) {
+          const size_t at = row_offset(slot, h, p.PS, p.HKV, HD) + sub * 8;
           if constexpr (!kQuant) {
-            out[u] = *reinterpret_cast<const uint4*>(cache + ((row * p.HKV + h) * HD + sub * 8) * 2);
+            out[u] = *reinterpret_cast<const uint4*>(cache + at * 2);
           } else {
-            const long long page = row / p.PS;
-            codes[u] = *reinterpret_cast<const uint2*>(cache + (row * p.HKV + h) * HD + sub * 8);
-            byte[u] = scales[(page * p.HKV + h) * p.PS + (row - page * p.PS)];
+            codes[u] = *reinterpret_cast<const uint2*>(cache + at);
+            byte[u] = scales[scale_offset(slot, h, p.PS, p.HKV)];
           }
         }
       }
@@ -314,14 +338,14 @@ __global__ void __launch_bounds__(128) varlen_rows_kernel(const VarlenAttnParams
 #pragma unroll
   for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
   for (int k0 = 0; k0 < end; k0 += 32) {
-    long long row = -1;
+    int2 slot = make_int2(-1, 0);
     float vs = 1.f, s = -INFINITY;
-    if (k0 + lane < end) row = paged_row(p.bt, b, k0 + lane, p.PS, p.BTW, p.P);
+    if (k0 + lane < end) slot = paged_slot(p.bt, b, k0 + lane, p.PS, p.BTW, p.P);
+    const long long row = slot.x < 0 ? -1 : static_cast<long long>(slot.x) * p.PS + slot.y;
     if (row >= 0) {
       s = 0.f;
       if constexpr (kQuant) {
-        const long long page = row / p.PS;
-        const long long at = (page * p.HKV + hk) * p.PS + (row - page * p.PS);
+        const size_t at = scale_offset(slot, hk, p.PS, p.HKV);
         vs = e8m0_to_float(p.v_scales[at]);
         const float ks = e8m0_to_float(p.k_scales[at]);
         const uint8_t* kr = p.k + (row * p.HKV + hk) * HD;
