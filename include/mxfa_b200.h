@@ -389,6 +389,15 @@ int mxfa_kvcache_gather_varlen_launch(const void* k_cache, const void* v_cache, 
                                       void* v_out, int total, int B, int HKV, int D, int PS, int BTW,
                                       int num_pages, int bf16, void* stream);
 
+/* Quantised caches to 16-bit ones for one attention call: sequence b's tokens
+ * 0 .. seqlens[b] to rows b * rows .. of k_out, v_out [B, rows, HKV, D], and
+ * table_out [B] = 0 .. B-1, the block table that reads them as B pages of
+ * `rows` tokens.  fp16 saturates at 65504. */
+int mxfa_kvcache_unpack_launch(const void* k_cache, const void* v_cache, const void* k_scales,
+                               const void* v_scales, const int32_t* seqlens, const int32_t* block_table,
+                               void* k_out, void* v_out, int32_t* table_out, int B, int rows, int HKV,
+                               int D, int PS, int BTW, int num_pages, int bf16, void* stream);
+
 /* The division of a step's attention into items, written to `plan` (device,
  * mxfa_chunk_plan_bytes, 16-byte aligned) from the lengths, once per step
  * for every layer.  A plan belongs to the lengths, head counts and causal

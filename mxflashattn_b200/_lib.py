@@ -83,6 +83,8 @@ SIGNATURES = {
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _sz, _sz, _sz, _sz, _i, _vp]),
     "mxfa_kvcache_gather_varlen_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "mxfa_kvcache_unpack_launch": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "mxfa_chunk_plan_bytes": (_sz, [_i, _i, _i, _i]),
     "mxfa_chunk_workspace_bytes": (_sz, [_i, _i]),
     "mxfa_chunk_counter_bytes": (_sz, [_i]),

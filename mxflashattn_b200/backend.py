@@ -464,6 +464,16 @@ def _chunk_sizes(kv_heads: int, head_dim: int) -> tuple[int, int]:
     return sizes
 
 
+UNPACK_TILES = 4
+UNPACK_BYTES = 1 << 30
+
+
+def unpack_pays(total_q: int, batch: int, group: int, kv_heads: int, head_dim: int, max_len: int) -> bool:
+    """Whether a quantised call first unpacks its sequences to 16 bits."""
+    return (total_q * group >= UNPACK_TILES * 128 * batch
+            and 4 * batch * max_len * kv_heads * head_dim <= UNPACK_BYTES)
+
+
 _MAX_GROUP = 128  # query heads of one KV head that the tiled kernel takes
 
 
@@ -523,6 +533,16 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
             ws_bytes, counter_bytes = _chunk_sizes(HKV, D)
             ws = _scratch(q, stream, ws_bytes)
             counters = split_counters(q.device, stream, counter_bytes)
+            if k_scales is not None and unpack_pays(Tq, B, HQ // HKV, HKV, D, max_seqlen_k):
+                rows = -(-max_seqlen_k // 128) * 128
+                kv = q.new_empty((2, B, rows, HKV, D))
+                pages_of = q.new_empty((B, 1), dtype=torch.int32)
+                rc = lib.mxfa_kvcache_unpack_launch(
+                    k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), seq.data_ptr(),
+                    bt.data_ptr(), kv.data_ptr(), kv[1].data_ptr(), pages_of.data_ptr(), B, rows, HKV, D, PS,
+                    bt.shape[1], pages, _bf16(q), stream)
+                _lib.check(rc, "mxfa_kvcache_unpack_launch")
+                k_cache, v_cache, k_scales, v_scales, bt, pages, PS = kv[0], kv[1], None, None, pages_of, B, rows
         rc = lib.mxfa_kvcache_varlen_attention_launch(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales),
             cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), _lib.ptr(table), 0 if table is None else table.numel() * 4,

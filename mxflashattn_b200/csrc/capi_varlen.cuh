@@ -411,4 +411,45 @@ int mxfa_kvcache_step_attention_launch(const void* q, const void* k_cache, const
                                 cu_seqlens_q, total_q);
 }
 
+int mxfa_kvcache_unpack_launch(const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
+                               const int32_t* seqlens, const int32_t* block_table, void* k_out, void* v_out,
+                               int32_t* table_out, int B, int rows, int HKV, int D, int PS, int BTW, int num_pages,
+                               int bf16, void* stream) {
+  // (the lengths stand in for the offsets, which this call has none of)
+  if (int rc = paged_varlen_checks(k_cache, v_cache, k_scales, v_scales, seqlens, seqlens, block_table, rows, B, HKV,
+                                   D, PS, BTW, num_pages))
+    return rc;
+  if (rows == 0 || B == 0) return MXFA_OK;
+  if (k_scales == nullptr) return fail(MXFA_ERR_INVALID, "unpacking is for quantised caches");
+  if (!k_out || !v_out || !table_out) return fail(MXFA_ERR_INVALID, "null tensor pointer");
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(MXFA_ERR_INVALID, "outputs must be 16-byte aligned");
+  if (B > 65535) return fail(MXFA_ERR_UNSUPPORTED, "%d sequences exceed the grid", B);
+  PagedVarlenParams p{};
+  p.k = k_out;
+  p.v = v_out;
+  p.k_cache = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  p.v_cache = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  p.k_scales = static_cast<uint8_t*>(const_cast<void*>(k_scales));
+  p.v_scales = static_cast<uint8_t*>(const_cast<void*>(v_scales));
+  p.seqlens = seqlens;
+  p.bt = block_table;
+  p.T = rows;
+  p.B = B;
+  p.HKV = HKV;
+  p.PS = PS;
+  p.BTW = BTW;
+  p.P = num_pages;
+  p.tok_per_cta = kPvMaxTok;
+  p.table = table_out;
+  const dim3 grid((rows + kPvMaxTok - 1) / kPvMaxTok, B);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (bf16)
+    D == 128 ? gather_varlen_kernel<__nv_bfloat16, 128, true, true><<<grid, kPvThreads, 0, st>>>(p)
+             : gather_varlen_kernel<__nv_bfloat16, 64, true, true><<<grid, kPvThreads, 0, st>>>(p);
+  else
+    D == 128 ? gather_varlen_kernel<__half, 128, true, true><<<grid, kPvThreads, 0, st>>>(p)
+             : gather_varlen_kernel<__half, 64, true, true><<<grid, kPvThreads, 0, st>>>(p);
+  return check_launch("gather_varlen_kernel(dense)");
+}
+
 }  // extern "C"

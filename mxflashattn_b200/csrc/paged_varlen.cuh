@@ -70,6 +70,7 @@ struct PagedVarlenParams {
   const int* bt;       // [B, BTW]
   int T, B, HKV, PS, BTW, P;
   int tok_per_cta;
+  int* table;  // dense read-back: [B], written
 };
 
 constexpr int kPvThreads = 256;
@@ -238,16 +239,43 @@ __device__ __forceinline__ void dequant8(uint2 codes, float s, float (&x)[8]) {
   }
 }
 
+// Two floats to T, fp16 saturating at its largest value (NaN stays NaN).
+template <typename T>
+__device__ __forceinline__ uint32_t pack_sat(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  } else {
+    return Elem<T>::pack(lo, hi);
+  }
+}
+
 // Read-back: the append's mirror; packed rows of tokens that are not mapped
 // (or that no sequence holds) are zero.  HBM-bound, each code read once and
 // each value written once.
-template <typename T, int HD, bool kQuant>
+// kDense: every sequence's tokens from position 0 on, sequence b (blockIdx.y)
+// to rows b * T .. of the output, T rows a sequence, with the table
+// (sequence b: page b) that reads the output as a cache of pages of T tokens.
+// Rows past a sequence's length are left alone.
+template <typename T, int HD, bool kQuant, bool kDense = false>
 __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVarlenParams p) {
   constexpr int kGroup = HD / 8;
   __shared__ int2 s_slots[kPvMaxTok];
   const int t0 = blockIdx.x * p.tok_per_cta;
-  const int n = min(p.tok_per_cta, p.T - t0);
-  cta_token_rows(p, t0, n, s_slots);
+  int n = min(p.tok_per_cta, p.T - t0);
+  size_t row0 = t0;
+  if constexpr (kDense) {
+    const int b = blockIdx.y;
+    n = min(n, p.seqlens[b] - t0);
+    row0 += static_cast<size_t>(b) * p.T;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.table[b] = b;
+    if (n <= 0) return;
+    if (threadIdx.x < n) s_slots[threadIdx.x] = paged_slot(p.bt, b, t0 + threadIdx.x, p.PS, p.BTW, p.P);
+    __syncthreads();
+  } else {
+    cta_token_rows(p, t0, n, s_slots);
+  }
   const int sub = threadIdx.x % kGroup;
   const RowWalk walk = row_walk<kGroup>(2 * p.HKV);
   if (!walk.live) return;
@@ -255,7 +283,7 @@ __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVa
     const int kv = pair >= p.HKV, h = pair - kv * p.HKV;
     const uint8_t* cache = kv ? p.v_cache : p.k_cache;
     const uint8_t* scales = kv ? p.v_scales : p.k_scales;
-    T* dst = static_cast<T*>(const_cast<void*>(kv ? p.v : p.k)) + static_cast<size_t>(t0) * p.HKV * HD + h * HD + sub * 8;
+    T* dst = static_cast<T*>(const_cast<void*>(kv ? p.v : p.k)) + row0 * p.HKV * HD + h * HD + sub * 8;
     for (int i0 = walk.tok; i0 < n; i0 += walk.step * kPvBatch) {
       uint4 out[kPvBatch];
       uint2 codes[kPvBatch];
@@ -283,8 +311,9 @@ __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVa
         if constexpr (kQuant) {
           float x[8];
           dequant8(codes[u], e8m0_to_float(byte[u]), x);
-          out[u] = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
-                              Elem<T>::pack(x[6], x[7]));
+          // read back, a value past fp16's largest is its infinity; as an operand it saturates
+          auto pack = [](float lo, float hi) { return kDense ? pack_sat<T>(lo, hi) : Elem<T>::pack(lo, hi); };
+          out[u] = make_uint4(pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7]));
         }
         if (i < n) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(i) * p.HKV * HD) = out[u];
       }
