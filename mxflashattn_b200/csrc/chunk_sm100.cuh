@@ -892,7 +892,8 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         v_exp = static_cast<float>(static_cast<int>(e.y));
         v_inv = pow2_f32(-static_cast<int>(e.y));
       }
-      const bool all_full = __all_sync(0xffffffffu, key0 + kTcKeys <= vis_end);
+      // (a negative scale, which looks for the least score, takes the masked loops)
+      const bool all_full = __all_sync(0xffffffffu, key0 + kTcKeys <= vis_end) && pos_scale;
       const float ext0 = pos_scale ? -INFINITY : INFINITY;
       float ext = ext0;
       uint32_t ra[32], rb[32];
@@ -902,17 +903,17 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       // tile the kernel took 5% longer, the quantised one 20%).  Tiles with
       // masked columns take short loops of their own, for the same reason.
       if (all_full) {
-        float e[4] = {ext0, ext0, ext0, ext0};
+        float e[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
         for (int c = 0; c < kTcKeys; c += 64) {
           tmem_ld32_async(sbuf + c, ra);
           tmem_wait_ld(ra);
           tmem_ld32_async(sbuf + c + 32, rb);
-          ext_chunk32(ra, pos_scale, e);
+          ext_chunk32(ra, true, e);
           tmem_wait_ld(rb);
-          ext_chunk32(rb, pos_scale, e);
+          ext_chunk32(rb, true, e);
         }
-        ext = pos_scale ? fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) : fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
+        ext = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3]));
       } else {
 #pragma unroll 1
         for (int c = 0; c < kTcKeys; c += 16) {
