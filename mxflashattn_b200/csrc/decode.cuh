@@ -466,6 +466,9 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   uint64_t* empty = full + Cfg::kSlots;
   uint8_t* slot_scales = reinterpret_cast<uint8_t*>(empty + Cfg::kSlots);  // [slot][K|V][16] (row scales)
   static_assert(!kRowScale || (kFp8 && kTma), "row scales are for e4m3 tiles loaded by TMA");
+  // Packed queries are for 16-bit caches and row scales; the tensor-scale
+  // e4m3 kernel is at its register cap, where carrying them cost 1.6%.
+  constexpr bool kMayPack = !kFp8 || kRowScale;
 
   // Programmatic dependent launch: let the next kernel on the stream start
   // placing its blocks as soon as every block of this grid is running (they
@@ -552,16 +555,23 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   // chunk z then covers [z*c_len, (z+1)*c_len) exactly as the reference's split
   const int lo = p.ows != nullptr ? z * p.c_len : 0;
   const int tile0 = (lo / kTileTok) * kTileTok;
-  int q_row0 = b * p.Sq, q_n = p.Sq;  // this sequence's query rows
-  if (p.cu_q != nullptr) {
-    q_row0 = p.cu_q[b];
-    q_n = p.cu_q[b + 1] - q_row0;
+  int packed_row0 = 0, packed_n = 0;  // this sequence's query rows, where they are packed
+  if constexpr (kMayPack) {
+    packed_row0 = b * p.Sq;
+    packed_n = p.Sq;
+    if (p.cu_q != nullptr) {
+      packed_row0 = p.cu_q[b];
+      packed_n = p.cu_q[b + 1] - packed_row0;
+    }
   }
   if (!have_len) cached_len = p.seqlens[b];
   // every CTA of the sequence agrees, so none is counted on
-  if (p.cu_q != nullptr && (q_n <= 0 || q_n > p.Sq || q_row0 < 0 || q_row0 > p.q_rows - q_n)) return;
+  if (kMayPack && p.cu_q != nullptr &&
+      (packed_n <= 0 || packed_n > p.Sq || packed_row0 < 0 || packed_row0 > p.q_rows - packed_n))
+    return;
   const int total_len = cached_len + p.append_len;
-  const int hi = p.ows != nullptr && !(p.last_open && z == p.NP - 1) ? min(lo + p.c_len, total_len) : total_len;
+  const bool cut = p.ows != nullptr && !(kMayPack && p.last_open && z == p.NP - 1);
+  const int hi = cut ? min(lo + p.c_len, total_len) : total_len;
   const int ntiles = (hi > lo) ? (hi - tile0 + kTileTok - 1) / kTileTok : 0;
 
   // The producer's first block-table reads go out now, so their latency
@@ -770,6 +780,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   // ---------------------------------------------------------------- consumers
   const int g = lane >> 2;
   const int t4 = lane & 3;
+  const int q_n = kMayPack ? packed_n : p.Sq;
   const int rows_total = q_n * p.GQ;
   const int row_base = rg * 8 * NT;
   const T* qptr = static_cast<const T*>(p.q);
@@ -788,7 +799,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
     if (row < rows_total) {
       const int i = row / p.GQ;
       const int h = kvh * p.GQ + row % p.GQ;
-      qr = qptr + (static_cast<size_t>(q_row0 + i) * p.HQ + h) * HD;
+      qr = qptr + (static_cast<size_t>((kMayPack ? packed_row0 : b * p.Sq) + i) * p.HQ + h) * HD;
     }
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk) {
@@ -1151,7 +1162,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
     }
     const int i = rr / p.GQ;
     const int h = kvh * p.GQ + rr % p.GQ;
-    const size_t R = static_cast<size_t>(q_row0 + i) * p.HQ + h;
+    const size_t R = static_cast<size_t>((kMayPack ? packed_row0 : b * p.Sq) + i) * p.HQ + h;
     if (p.ows != nullptr) {
       *reinterpret_cast<float4*>(p.ows + (R * p.NP + z) * HD + d4) = acc;
       if (d4 == 0) {
@@ -1191,7 +1202,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         if (rr >= rows_total) break;
         const int i = rr / p.GQ;
         const int h = kvh * p.GQ + rr % p.GQ;
-        const int R = (q_row0 + i) * p.HQ + h;
+        const int R = ((kMayPack ? packed_row0 : b * p.Sq) + i) * p.HQ + h;
         if constexpr (kFp8) {
           // the e4m3 kernel runs at its register cap: the loop form, inline
           if (p.cp_bufs != nullptr)
@@ -1218,7 +1229,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
             const int rr = row_base + col;
             if (rr >= rows_total) break;
             const int h = kvh * p.GQ + rr % p.GQ;
-            const int R = (q_row0 + rr / p.GQ) * p.HQ + h;
+            const int R = ((kMayPack ? packed_row0 : b * p.Sq) + rr / p.GQ) * p.HQ + h;
             cp_merge_row_call<T, HD>(recs, rows_all, R, p.cp_world, lane, static_cast<T*>(p.out), p.lse, tag, t0);
           }
           __syncwarp();  // lanes leave their per-word waits at different times
