@@ -233,6 +233,62 @@ def test_append_and_gather_pass_each_argument_in_its_slot(rec):
     assert c == dict(want, k_out=ko.data_ptr(), v_out=vo.data_ptr(), bf16=0)
 
 
+def _attend_call(rec, a, max_q, plan, **kw):
+    backend.flash_attn_varlen_with_kvcache(a["q"], a["k_cache"], a["v_cache"], a["cu"], a["lens"], a["table"], max_q, 48,
+                                           0.5, True, a["k_scales"], a["v_scales"], plan, None, True, **kw)
+    return rec.calls[-1]
+
+
+def _common(a, **over):
+    want = dict(q=a["q"].data_ptr(), k_cache=a["k_cache"].data_ptr(), v_cache=a["v_cache"].data_ptr(),
+                k_scales=a["k_scales"].data_ptr(), v_scales=a["v_scales"].data_ptr(), cu_seqlens_q=a["cu"].data_ptr(),
+                seqlens=a["lens"].data_ptr(), block_table=a["table"].data_ptr(), total_q=6, B=2, HQ=8, HKV=2, D=128,
+                PS=16, BTW=3, num_pages=7, causal=1, bf16=1, scale=0.5, stream=STREAM)
+    want.update(over)
+    return want
+
+
+def test_attention_passes_each_argument_in_its_slot(rec):
+    a = _args(quant=True)
+    table = torch.zeros(4096, dtype=torch.int32)
+    plan = fa.KvChunkPlan(6, 2, 4, 8, 2, True, table, None, torch.device("cpu"))
+    name, c = _attend_call(rec, a, 4, plan)
+    assert name == "mxfa_kvcache_varlen_attention_launch" and set(c) == set(NAMES[name])
+    want = _common(a, plan=table.data_ptr(), plan_bytes=4096 * 4, q_token_stride=1024, q_head_stride=128,
+                   workspace_bytes=5000)
+    assert {k: c[k] for k in want} == want
+    assert len({c["out"], c["lse"], c["workspace"], c["counters"]} - {None}) == 4
+
+
+def test_a_decode_step_passes_each_argument_in_its_slot(rec):
+    a = _args(quant=True)
+    order = torch.zeros(2, dtype=torch.int32)
+    plan = fa.KvChunkPlan(6, 2, 1, 8, 2, True, None, order, torch.device("cpu"))
+    name, c = _attend_call(rec, a, 1, plan)
+    assert name == "mxfa_kvcache_step_attention_launch" and set(c) == set(NAMES[name])
+    want = _common(a, length_order=order.data_ptr(), max_q=1, num_splits=1, chunk_len=48)
+    assert {k: c[k] for k in want} == want
+
+
+def test_unpacking_hands_the_attention_its_scratch_as_a_cache(rec, monkeypatch):
+    monkeypatch.setattr(backend, "unpack_pays", lambda *a: True)
+    a = _args(quant=True)
+    plan = fa.KvChunkPlan(6, 2, 4, 8, 2, True, torch.zeros(4096, dtype=torch.int32), None, torch.device("cpu"))
+    name, c = _attend_call(rec, a, 4, plan)
+    unpack, u = rec.calls[-2]
+    assert unpack == "mxfa_kvcache_unpack_launch" and set(u) == set(NAMES[unpack])
+    want = {k: v for k, v in _common(a, rows=128).items() if k in NAMES[unpack]}
+    assert {k: u[k] for k in want} == want
+    assert c["k_scales"] is None and c["v_scales"] is None and c["PS"] == 128 and c["num_pages"] == 2 and c["BTW"] == 1
+    assert (c["k_cache"], c["v_cache"], c["block_table"]) == (u["k_out"], u["v_out"], u["table_out"])
+    assert u["v_out"] - u["k_out"] == 2 * 128 * 2 * 128 * 2
+
+
+@pytest.fixture(autouse=True)
+def _fixed_chunk_sizes(monkeypatch):
+    monkeypatch.setattr(backend, "_chunk_sizes", lambda kv_heads, head_dim: (5000, 256))
+
+
 # ------------------------------------------------------------------------------------------- host guards of the C ABI
 
 @pytest.fixture(scope="module")
@@ -289,6 +345,18 @@ def test_step_entry_refuses_what_the_decode_kernel_does_not_take(lib):
                  dict(num_splits=3, workspace=None)):
         assert call(**over) == _lib.MXFA_ERR_INVALID, over
     assert call(max_q=0, q=None) == _lib.MXFA_OK
+
+
+def test_unpack_entry_refuses(lib):
+    name = "mxfa_kvcache_unpack_launch"
+    base = dict(k_scales=4096, v_scales=4096, rows=128, table_out=4096)
+    call = lambda **over: getattr(lib, name)(*_guard_args(name, **{**base, **over}))  # noqa: E731
+    assert call(D=96) == _lib.MXFA_ERR_UNSUPPORTED
+    assert call(B=70000) == _lib.MXFA_ERR_UNSUPPORTED
+    for over in (dict(k_scales=None, v_scales=None), dict(k_out=None), dict(table_out=None), dict(v_out=4104),
+                 dict(seqlens=None), dict(rows=-1), dict(k_scales=4098, v_scales=4096)):
+        assert call(**over) == _lib.MXFA_ERR_INVALID, over
+    assert call(rows=0, k_out=None) == _lib.MXFA_OK
 
 
 def test_plan_entry_refuses_and_sizes_are_host_only(lib):

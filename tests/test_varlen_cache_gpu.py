@@ -463,3 +463,161 @@ def test_a_nan_in_a_visible_key_reaches_the_output(quant, new, cuda_device):
     dirty = 3 * new
     assert np.isnan(out[:dirty]).all() and np.isnan(lse[:dirty]).all()
     assert np.isfinite(out[dirty:]).all() and np.isfinite(lse[dirty:]).all()
+
+
+@pytest.mark.parametrize("unpack", [True, False])
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 64)])
+def test_quantised_pieces_unpacked_or_converted_in_the_kernel(unpack, dtype, d, cuda_device, monkeypatch):
+    """Both ways through a quantised cache, on the same batch, whatever the rule would choose."""
+    from mxflashattn_b200 import backend
+
+    monkeypatch.setattr(backend, "unpack_pays", lambda *a: unpack)
+    b = make_batch(970, [130, 1, 40, 0], [700, 300, 40, 129], hq=8, hkv=2, d=d, dtype=dtype, quant=True, poison=np.nan)
+    out, lse, scale = _attend(b, cuda_device, True)
+    assert_attention(out, lse, b, scale, True, f"unpack {unpack}")
+
+
+def test_the_unpacking_rule_takes_long_pieces_and_bounded_memory():
+    from mxflashattn_b200.backend import unpack_pays
+
+    assert unpack_pays(1024, 1, 4, 8, 128, 16384)            # 32 tiles of one sequence
+    assert not unpack_pays(64, 1, 4, 8, 128, 16384)          # two tiles
+    assert not unpack_pays(543, 32, 4, 8, 128, 4608)         # one piece among decodes
+    assert not unpack_pays(1 << 17, 64, 4, 8, 128, 1 << 17)  # scratch of 34 GB
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("new,total,hq,hkv", [
+    ([600] * 5, [600] * 5, 4, 4),                    # whole waves and a split remainder
+    ([33] * 40, [200] * 40, 8, 2),                   # many tiles of a few keys
+    ([5, 1, 1], [6000, 30, 700], 16, 1),             # one long sequence among short ones
+    ([1] * 30 + [2], [3] * 30 + [9000], 2, 1),
+])
+def test_plans_that_split_tiles(quant, new, total, hq, hkv, cuda_device):
+    b = make_batch(980 + len(new), new, total, hq=hq, hkv=hkv, d=64, dtype="fp16", quant=quant)
+    out, lse, scale = _attend(b, cuda_device, True, plan=True)
+    assert_attention(out, lse, b, scale, True, "split plan")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("batch,hq,hkv", [(1, 8, 2), (40, 32, 8), (1500, 4, 4), (3000, 16, 1)])
+def test_a_plan_covers_every_tile_once(causal, batch, hq, hkv, cuda_device):
+    """Items of each tile: the parts 0 .. nsplit-1 cover its key tiles without gap or overlap."""
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    rng = np.random.default_rng(batch)
+    new = rng.integers(0, 3 if batch > 100 else 400, size=batch)
+    new[0] += 1
+    total = np.where(rng.random(batch) < 0.1, new // 2, new + rng.integers(0, 3000, size=batch))
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    plan = fa.kvcache_chunk_plan(torch.from_numpy(cu).to(cuda_device), torch.from_numpy(total).to(cuda_device),
+                                 int(cu[-1]), int(new.max()), q_heads=hq, kv_heads=hkv, causal=causal)
+    table = plan.table.cpu().numpy()
+    items = table[16:16 + 12 * table[0]].reshape(-1, 12)
+    tok = 128 // (hq // hkv)
+    seen = {}
+    for b, row0, ntok, pos0, length, kt0, kt1, nsplit, split, part0, group, _ in items.tolist():
+        seen.setdefault((b, row0), []).append((split, kt0, kt1, nsplit, ntok, pos0, length, part0, group))
+    want = [(b, int(cu[b]) + t, min(tok, int(new[b]) - t)) for b in range(batch) for t in range(0, int(new[b]), tok)]
+    assert sorted(seen) == [(b, r) for b, r, _ in want]
+    used = []
+    for b, row0, ntok in want:
+        parts = sorted(seen[(b, row0)])
+        pos = int(total[b]) - int(new[b]) + row0 - int(cu[b])
+        end = max(min(pos + ntok, int(total[b])), 0) if causal else int(total[b])
+        tiles = max(1, -(-end // 128))
+        assert [p[0] for p in parts] == list(range(parts[0][3])) and len(parts) == parts[0][3]
+        edges = [0] + [p[2] for p in parts]
+        assert [p[1] for p in parts] == edges[:-1] and edges[-1] == tiles
+        assert all(p[4:7] == (ntok, pos, int(total[b])) for p in parts)
+        if len(parts) > 1:
+            assert len({p[7:] for p in parts}) == 1
+            used += range(parts[0][7], parts[0][7] + len(parts))
+    assert len(used) == len(set(used))
+
+
+def test_query_offsets_that_decrease_make_an_empty_plan(cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+    from mxflashattn_b200 import _lib
+
+    cu = torch.tensor([0, 60, 0, 60, 0, 60], dtype=torch.int32, device=cuda_device)
+    lens = torch.full((5,), 100, dtype=torch.int32, device=cuda_device)
+    plan = fa.kvcache_chunk_plan(cu, lens, 60, 60, q_heads=128, kv_heads=1, causal=True)
+    assert int(plan.table[0]) == 0
+    assert _lib.read_error_flags() == _lib.FLAG_BAD_ORDER
+
+
+def test_a_plan_of_another_batch_of_the_same_counts_stays_in_bounds(cuda_device):
+    """A stale plan gives wrong numbers, but nothing outside the tensors is touched and no tile is waited for."""
+    import torch
+
+    import mxflashattn_b200 as fa
+    from mxflashattn_b200 import _lib
+
+    b = make_batch(990, [60, 4], [300, 400], quant=True)
+    t = b.device(cuda_device)
+    stale = fa.kvcache_chunk_plan(torch.tensor([0, 4, 64], device=cuda_device), torch.tensor([9000, 70], device=cuda_device),
+                                  64, 60, q_heads=b.hq, kv_heads=b.hkv, causal=True)
+    kw = dict(causal=True, k_scales=t["ks"], v_scales=t["vs"])
+    args = (t["q"], t["kc"], t["vc"], t["cu"], t["lens"], t["table"], 60)
+    good = fa.flash_attn_varlen_with_kvcache(*args, **kw)
+    fa.flash_attn_varlen_with_kvcache(*args, plan=stale, **kw)
+    torch.cuda.synchronize()
+    assert _lib.read_error_flags() & ~(_lib.FLAG_TABLE_TOO_NARROW | _lib.FLAG_PAGE_OUT_OF_RANGE) == 0
+    assert torch.equal(fa.flash_attn_varlen_with_kvcache(*args, **kw), good)
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("new", [1, 20])
+def test_offsets_past_32_bits(quant, new, cuda_device):
+    """A cache of more than 2^31 elements, the sequence in its last pages."""
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    b = make_batch(1000, [new], [150], hq=8, hkv=8, quant=quant, spare_pages=0)
+    t = b.device(cuda_device)
+    pages = (1 << 31) // (16 * 8 * 128) + 40
+    shift = pages - b.k.shape[0]
+    big = {}
+    for n in ("kc", "vc", "ks", "vs"):
+        if t[n] is not None:
+            x = torch.zeros((pages,) + t[n].shape[1:], device=cuda_device, dtype=torch.uint8 if quant else t[n].dtype)
+            x[shift:] = t[n].view(torch.uint8) if quant else t[n]
+            big[n] = x.view(t[n].dtype)
+    table = torch.where(t["table"] >= 0, t["table"] + shift, t["table"])
+    kw = dict(k_scales=big.get("ks"), v_scales=big.get("vs"))
+    out, lse = fa.flash_attn_varlen_with_kvcache(t["q"], big["kc"], big["vc"], t["cu"], t["lens"], table, new, 150,
+                                                 causal=True, return_softmax_lse=True, **kw)
+    assert_attention(host(out), host(lse), b, b.d ** -0.5, True, "large cache")
+    x = torch.randn((new, 8, 128), device=cuda_device, dtype=torch.bfloat16)
+    fa.kvcache_append_varlen(x, 2 * x, big["kc"], big["vc"], t["cu"], t["lens"], table, **kw)
+    k, v = fa.kvcache_gather_varlen(big["kc"], big["vc"], t["cu"], t["lens"], table, new, **kw)
+    for got, src in ((k, x), (v, 2 * x)):
+        codes, scale = quantise64(host(src))
+        assert np.array_equal(host(got).astype(np.float64), codes * scale[..., None] if quant else host(src))
+
+
+def test_two_streams_at_once_keep_their_workspaces_apart(cuda_device):
+    import torch
+
+    import mxflashattn_b200 as fa
+
+    b = make_batch(1010, [1, 3], [6000, 5000], hq=4, hkv=1, d=64, dtype="fp16", quant=True)
+    t = b.device(cuda_device)
+    run = lambda: fa.flash_attn_varlen_with_kvcache(t["q"], t["kc"], t["vc"], t["cu"], t["lens"], t["table"], 3,  # noqa: E731
+                                                    causal=True, k_scales=t["ks"], v_scales=t["vs"])
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
