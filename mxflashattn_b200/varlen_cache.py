@@ -345,7 +345,8 @@ def flash_attn_varlen_with_kvcache(
     ``causal`` the query at position ``p`` sees keys ``0 .. p``.  Pieces of
     prompts and single decode tokens may be mixed.  ``max_seqlen_q`` bounds
     the queries of one sequence, ``max_seqlen_k`` (default: what the table
-    can hold) the cached tokens.  A row that sees no key is 0 with LSE -inf;
+    can hold) the cached tokens: no sequence may be longer (a longer one may be
+    cut and flagged).  A row that sees no key is 0 with LSE -inf;
     rows past ``cu_seqlens_q[-1]`` are padding and are not written.
 
     The cache is 16-bit in ``q``'s dtype, or quantised with ``k_scales`` and
