@@ -125,6 +125,12 @@ int mxfa_kvcache_attention_launch(const void* q, const void* k_cache, const void
  * allocating; every launch leaves it zero again. */
 size_t mxfa_split_counter_bytes(int B, int Sq, int HQ, int HKV);
 
+/* Id of the graph capture that `stream` is part of (never the same for two
+ * captures of a process), 0 when it is not capturing.  A captured launch
+ * replays on any stream, so its counters belong to its graph: zeroed by a
+ * node of it, shared with no other graph and no eager launch. */
+int mxfa_stream_capture_id(void* stream, unsigned long long* id);
+
 /* mxfa_kvcache_attention_launch in ONE kernel launch when the plan splits:
  * each split CTA publishes its partial state, counts itself on its unit's
  * counter, and the last one merges the unit's partials into out / lse (the

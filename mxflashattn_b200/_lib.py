@@ -44,6 +44,7 @@ SIGNATURES = {
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i,
              _f, _vp]),
     "mxfa_split_counter_bytes": (_sz, [_i, _i, _i, _i]),
+    "mxfa_stream_capture_id": (_i, [_vp, ctypes.POINTER(ctypes.c_ulonglong)]),
     "mxfa_kvcache_attention_counted_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i,
              _i, _f, _vp]),

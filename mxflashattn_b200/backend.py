@@ -157,7 +157,18 @@ def kvcache_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, head_dim: 
 
 
 _COUNTERS: dict[tuple, "torch.Tensor"] = {}
-_OUTGROWN: list["torch.Tensor"] = []
+_CAPTURE_COUNTERS: dict[tuple, tuple[int, "torch.Tensor"]] = {}
+
+
+def _capture_id(device, stream_handle: int) -> int:
+    """Id of the graph capture that the stream is part of (ids are never used twice), 0 without one."""
+    import ctypes
+
+    if device.type != "cuda" or not _capturing():
+        return 0
+    out = ctypes.c_ulonglong(0)
+    _lib.check(_L().mxfa_stream_capture_id(stream_handle, ctypes.byref(out)), "mxfa_stream_capture_id")
+    return int(out.value)
 
 
 def split_counters(device, stream_handle: int, nbytes: int):
@@ -165,13 +176,24 @@ def split_counters(device, stream_handle: int, nbytes: int):
 
     Every counted launch leaves its counters at zero again, so one array per
     stream is reused by all launches ordered on that stream; it only grows.
+
+    A captured launch replays on any stream, next to other graphs and to eager
+    launches, so a graph shares its counters with nobody: the first launch of a
+    capture allocates them in the graph's own memory, and their zeroing is a
+    node of that graph, which the launches captured after it follow.
     """
     key = (device, stream_handle)
-    buf = _COUNTERS.get(key)
     n = max(nbytes // 4, 1)
+    capture = _capture_id(device, stream_handle)
+    if capture:
+        # kept until the stream's next capture: while this one runs, nothing else may get the memory
+        held, buf = _CAPTURE_COUNTERS.get(key, (0, None))
+        if held != capture or buf.numel() < n:
+            buf = torch.zeros((max(n, 4096),), device=device, dtype=torch.int32)
+            _CAPTURE_COUNTERS[key] = (capture, buf)
+        return buf
+    buf = _COUNTERS.get(key)
     if buf is None or buf.numel() < n:
-        if buf is not None:
-            _OUTGROWN.append(buf)  # a captured graph may still replay with it
         buf = _COUNTERS[key] = torch.zeros((max(n, 4096),), device=device, dtype=torch.int32)
     return buf
 

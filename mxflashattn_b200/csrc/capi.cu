@@ -593,6 +593,17 @@ size_t mxfa_split_counter_bytes(int B, int Sq, int HQ, int HKV) {
   return static_cast<size_t>(B) * HKV * groups * sizeof(unsigned);
 }
 
+int mxfa_stream_capture_id(void* stream, unsigned long long* id) {
+  if (id == nullptr) return fail(MXFA_ERR_INVALID, "id is NULL");
+  *id = 0;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long seq = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &seq);
+  if (e != cudaSuccess) return fail(MXFA_ERR_CUDA, "cudaStreamGetCaptureInfo: %s", cudaGetErrorString(e));
+  if (status == cudaStreamCaptureStatusActive) *id = seq;
+  return MXFA_OK;
+}
+
 int mxfa_kvcache_attention_counted_launch(const void* q, const void* k_cache, const void* v_cache,
                                           const int32_t* block_table, const int32_t* seqlens, void* out, float* lse,
                                           void* workspace, size_t workspace_bytes, unsigned* counters, int B, int Sq,
