@@ -946,6 +946,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
     // kept from -60 up, for the range of the row sum; a V row under that
     // counts with 2^-60, an error below 2^-51 in an output.
     float kf[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f}, iv[2] = {1.f, 1.f};
+    uint32_t vb[2] = {127u, 127u};
     if constexpr (kRowScale) {
       const uint32_t* words = reinterpret_cast<const uint32_t*>(slot_scales + slot * Cfg::kScaleBytes);
       const uint32_t kw = words[g >> 1], vw = words[kTileTok / 4 + (g >> 1)];
@@ -953,15 +954,17 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
       for (int c = 0; c < 2; ++c) {
         // the token's byte of the word, as the exponent field of a float
         const int byte = (g & 1) + 2 * c;
-        kf[c] = __uint_as_float(__funnelshift_l(kw, kw, 23 - 8 * byte) & 0x7f800000u);
-        uint32_t vb = (vw >> (8 * byte)) & 255u;
+        // (byte 255, NaN, comes out as infinity, which times zero is NaN)
+        const float field = __uint_as_float(__funnelshift_l(kw, kw, 23 - 8 * byte) & 0x7f800000u);
+        kf[c] = fmaf(field, 0.f, field);
+        vb[c] = (vw >> (8 * byte)) & 255u;
         if (partial) {  // bytes of positions outside [lo, hi) may be anything
           const int pos = pos0 + fp8_tok(g + 8 * c);
-          if (pos < lo || pos >= hi) vb = 127u;
+          if (pos < lo || pos >= hi) vb[c] = 127u;
         }
-        const uint32_t e = max(vb, 67u);
-        ve[c] = vb == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(0x4b000000u | e) - 8388735.f;  // e - 127
-        iv[c] = __uint_as_float(0x7f000000u - (e << 23));                                                // 2^(127 - e)
+        const uint32_t e = vb[c] == 255u ? 127u : max(vb[c], 67u);
+        ve[c] = __uint_as_float(0x4b000000u | e) - 8388735.f;  // e - 127
+        iv[c] = __uint_as_float(0x7f000000u - (e << 23));      // 2^(127 - e)
       }
     }
 
@@ -1026,6 +1029,17 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         s[nt][c] = p0;
         s[nt][c + 2] = p1;
       }
+    if constexpr (kRowScale) {
+      // a NaN V scale: the outputs of the rows that see the token, not their sums
+      if (__any_sync(0xffffffffu, max(vb[0], vb[1]) == 255u)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (vb[e >> 1] == 255u && pos0 + fp8_tok(g + 8 * (e >> 1)) <= lim[nt][e & 1])
+              s[nt][e] = __uint_as_float(0x7fffffffu);
+      }
+    }
     // the running max rarely moves after the first tiles: rescale O only when it did
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
