@@ -366,7 +366,7 @@ int mxfa_varlen_fwd_exact_launch(const void* q, const void* k, const void* v, co
  * Packed tokens [T, heads, D]: sequence b owns rows cu[b] .. cu[b+1] (int32
  * [B + 1] on the device), the LAST of the seqlens[b] tokens its cache holds
  * once the call's tokens are in it: packed row t is position
- * seqlens[b] - cu[b+1] + t.  Rows past cu[B] are padding and left alone.
+ * seqlens[b] - cu[b+1] + t.  Rows before cu[0] or past cu[B] are padding and left alone.
  * Caches are paged [P, PS, HKV, D] with a block table int32 [B, BTW]; D in
  * {64, 128}.  Quantised caches (k_scales and v_scales given) hold e4m3 codes
  * and one e8m0 byte per token and KV head, [P, HKV, PS]: value = code *

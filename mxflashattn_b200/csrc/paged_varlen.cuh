@@ -22,7 +22,8 @@
 namespace mxfa {
 
 // Sequence of packed token t (one warp): the number of entries cu[1..B] that
-// are <= t, every lane comparing its own; B when no sequence holds t.
+// are <= t, every lane comparing its own; B when every sequence ends before t.
+// (A token before cu[0] comes out as one of the first sequence: callers ask.)
 __device__ __forceinline__ int token_sequence(const int* __restrict__ cu, int B, int t, int lane) {
   int n = 0;
   for (int i = 0; i < B; i += 32) {
@@ -86,7 +87,8 @@ __device__ __forceinline__ void cta_token_rows(const PagedVarlenParams& p, int t
     int b = token_sequence(p.cu, p.B, t0, lane);
     if (lane < n) {
       while (b < p.B && p.cu[b + 1] <= t) ++b;
-      slots[lane] = b < p.B ? paged_slot(p.bt, b, p.seqlens[b] - p.cu[b + 1] + t, p.PS, p.BTW, p.P) : make_int2(-1, 0);
+      const bool owned = b < p.B && t >= p.cu[0];
+      slots[lane] = owned ? paged_slot(p.bt, b, p.seqlens[b] - p.cu[b + 1] + t, p.PS, p.BTW, p.P) : make_int2(-1, 0);
     }
   }
   __syncthreads();
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(128) varlen_rows_kernel(const VarlenAttnParams
   const int h = static_cast<int>(r - static_cast<long long>(t) * p.HQ);
   const int hk = h / p.GQ;
   const int b = token_sequence(p.cu, p.B, t, lane);
-  if (b >= p.B) return;  // a padding row: nothing is written
+  if (b >= p.B || t < p.cu[0]) return;  // a padding row: nothing is written
   const T* qr = static_cast<const T*>(p.q) + static_cast<size_t>(t) * p.q_tok + h * p.q_head;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) s_q[warp][j * 32 + lane] = static_cast<float>(qr[j * 32 + lane]);

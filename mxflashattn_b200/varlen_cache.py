@@ -178,7 +178,8 @@ def kvcache_append_varlen(
     power of two (at least 2^-126) with ``max |x| <= 448 s`` over the row's
     finite values; an infinity saturates to ``448 s`` and a NaN stays NaN.
     ``k`` and ``v`` may be strided views (slices of a fused projection); rows
-    past ``cu_seqlens[-1]`` are padding and are not written.
+    before ``cu_seqlens[0]`` or past ``cu_seqlens[-1]`` belong to no sequence and
+    are not written.
     """
     if not _quick(lambda: _plain_caches(k_cache, v_cache, k_scales, v_scales)
                   and _plain_batch(cu_seqlens, cache_seqlens, block_table, k_cache.device)
@@ -347,7 +348,8 @@ def flash_attn_varlen_with_kvcache(
     the queries of one sequence, ``max_seqlen_k`` (default: what the table
     can hold) the cached tokens: no sequence may be longer (a longer one may be
     cut and flagged).  A row that sees no key is 0 with LSE -inf;
-    rows past ``cu_seqlens_q[-1]`` are padding and are not written.
+    rows before ``cu_seqlens_q[0]`` or past ``cu_seqlens_q[-1]`` are padding and
+    are not written.
 
     The cache is 16-bit in ``q``'s dtype, or quantised with ``k_scales`` and
     ``v_scales``.  ``plan`` comes from ``kvcache_chunk_plan`` for the same
