@@ -41,8 +41,10 @@ extern "C" {
 #define MXFA_FLAG_WAIT_TIMEOUT 0x4u       /* a bounded pipeline wait gave up */
 #define MXFA_FLAG_DENSE_OVERFLOW 0x8u     /* dense-cache append past the cache capacity */
 #define MXFA_FLAG_BAD_ORDER 0x10u         /* a length order entry outside [0, B) (that row ran its own index), or
-                                           * query offsets that decrease (the chunk plan is then empty) or
-                                           * a plan made for another batch (its item is skipped) */
+                                           * query offsets that decrease or leave the packed rows (the
+                                           * chunk plan is then empty; a decode step leaves such a sequence
+                                           * out, and one with more rows than max_q), or a plan made for
+                                           * another batch (its item is skipped) */
 
 /* Library identity.  No reference counterpart (the reference's pybind
  * modules expose no version); used by the ctypes loader. */

@@ -131,19 +131,21 @@ __device__ __forceinline__ int block_sum(int x, int* s) {
 // to the atomics, since the order only schedules.
 __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const ChunkPlanParams p) {
   __shared__ int s_scan[kPlanThreads / 32];
-  __shared__ int s_sum, s_max, s_parts, s_groups, s_tail, s_hist[kPlanBuckets];
+  __shared__ int s_sum, s_max, s_parts, s_groups, s_tail, s_bad, s_hist[kPlanBuckets];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   ChunkItem* items = reinterpret_cast<ChunkItem*>(p.plan + kPlanHeader);
   int* off = p.plan + kPlanHeader + p.items_cap * static_cast<int>(sizeof(ChunkItem) / 4);
-  if (tid == 0) s_max = s_parts = s_groups = s_tail = 0;
+  if (tid == 0) s_max = s_parts = s_groups = s_tail = s_bad = 0;
   for (int i = tid; i < kPlanBuckets; i += kPlanThreads) s_hist[i] = 0;
+  __syncthreads();
   // tile offsets: block-wide exclusive scan over the sequences
   int base = 0;
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     const int n = b < p.B ? chunk_tiles_of(p, b) : 0;
+    if (b < p.B && (p.cu[b] < 0 || p.cu[b + 1] < p.cu[b] || p.cu[b + 1] > p.T)) s_bad = 1;
     int x = n;
 #pragma unroll
     for (int sh = 1; sh < 32; sh <<= 1) {
@@ -167,7 +169,8 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const ChunkPla
     __syncthreads();
   }
   int tiles = base;
-  if (tiles > p.T / p.tok + min(p.B, p.T)) {  // more than any cu_seqlens that never decreases has
+  // (offsets that never decrease have p.T / p.tok + min(p.B, p.T) tiles at most, which the plan has room for)
+  if (s_bad) {
     if (tid == 0) raise_flag(MXFA_FLAG_BAD_ORDER);
     tiles = 0;
   }

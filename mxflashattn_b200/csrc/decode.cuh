@@ -86,7 +86,7 @@ struct DecodeParams {
   const uint8_t* v_scales;
   // Packed queries (optional): sequence b owns rows cu_q[b] .. cu_q[b+1] of
   // q [q_rows, HQ, D] and of the outputs, Sq at most; a sequence without rows
-  // (or with more) is left alone.
+  // is left alone, one with more or with rows outside q is flagged as well.
   const int* cu_q;
   int q_rows;
   // The last split runs to the end of its sequence, however long: NP * c_len
@@ -568,9 +568,13 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
   }
   if (!have_len) cached_len = p.seqlens[b];
   // every CTA of the sequence agrees, so none is counted on
-  if (kMayPack && p.cu_q != nullptr &&
-      (packed_n <= 0 || packed_n > p.Sq || packed_row0 < 0 || packed_row0 > p.q_rows - packed_n))
-    return;
+  if (kMayPack && p.cu_q != nullptr) {
+    if (packed_n == 0) return;  // an idle sequence
+    if (packed_n < 0 || packed_n > p.Sq || packed_row0 < 0 || packed_row0 > p.q_rows - packed_n) {
+      if (threadIdx.x == 0) raise_flag(MXFA_FLAG_BAD_ORDER);
+      return;
+    }
+  }
   const int total_len = cached_len + p.append_len;
   const bool cut = p.ows != nullptr && !(kMayPack && p.last_open && z == p.NP - 1);
   const int hi = cut ? min(lo + p.c_len, total_len) : total_len;
