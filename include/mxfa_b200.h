@@ -390,7 +390,8 @@ int mxfa_kvcache_append_varlen_launch(const void* k, const void* v, void* k_cach
                                       void* stream);
 
 /* Read the packed tokens back: k_out, v_out [T, HKV, D] contiguous, code *
- * scale rounded once to the output type (16-bit caches are copied). */
+ * scale rounded once to the output type (16-bit caches are copied); rows that
+ * no sequence owns are zero, all of them where B = 0. */
 int mxfa_kvcache_gather_varlen_launch(const void* k_cache, const void* v_cache, const void* k_scales,
                                       const void* v_scales, const int32_t* cu_seqlens,
                                       const int32_t* seqlens, const int32_t* block_table, void* k_out,

@@ -9,8 +9,9 @@ int paged_varlen_checks(const void* k_cache, const void* v_cache, const void* k_
                                int total, int B, int HKV, int D, int PS, int BTW, int num_pages) {
   if (D != 64 && D != 128) return fail(MXFA_ERR_UNSUPPORTED, "head dim %d not in {64, 128}", D);
   if (total < 0 || B < 0 || HKV <= 0) return fail(MXFA_ERR_INVALID, "bad ragged batch geometry");
-  if (PS <= 0 || num_pages <= 0 || BTW <= 0) return fail(MXFA_ERR_INVALID, "bad cache geometry");
+  if (PS <= 0 || num_pages <= 0 || BTW < 0) return fail(MXFA_ERR_INVALID, "bad cache geometry");
   if (total == 0 || B == 0) return MXFA_OK;
+  if (BTW == 0) return fail(MXFA_ERR_INVALID, "bad cache geometry");
   if (!k_cache || !v_cache || !cu_seqlens || !seqlens || !block_table)
     return fail(MXFA_ERR_INVALID, "null tensor pointer");
   if ((k_scales == nullptr) != (v_scales == nullptr))
@@ -264,7 +265,7 @@ int mxfa_kvcache_gather_varlen_launch(const void* k_cache, const void* v_cache, 
   if (int rc = paged_varlen_checks(k_cache, v_cache, k_scales, v_scales, cu_seqlens, seqlens, block_table, total, B,
                                    HKV, D, PS, BTW, num_pages))
     return rc;
-  if (total == 0 || B == 0) return MXFA_OK;
+  if (total == 0) return MXFA_OK;  // (without sequences every row is one that nobody owns, and becomes zero)
   if (!k_out || !v_out) return fail(MXFA_ERR_INVALID, "null tensor pointer");
   if (!aligned16(k_out) || !aligned16(v_out)) return fail(MXFA_ERR_INVALID, "outputs must be 16-byte aligned");
   PagedVarlenParams p{};
