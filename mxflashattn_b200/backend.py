@@ -496,7 +496,7 @@ UNPACK_BYTES = 1 << 30
 
 def unpack_pays(total_q: int, batch: int, group: int, kv_heads: int, head_dim: int, max_len: int) -> bool:
     """Whether a quantised call first unpacks its sequences to 16 bits."""
-    return (total_q * group >= UNPACK_TILES * 128 * batch
+    return (total_q * group >= UNPACK_TILES * 128 * batch and max_len > 0  # (empty caches have no rows to unpack)
             and 4 * batch * max_len * kv_heads * head_dim <= UNPACK_BYTES)
 
 
