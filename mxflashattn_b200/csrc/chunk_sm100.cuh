@@ -326,11 +326,12 @@ struct ChunkCfg {
   static constexpr int kMl = kQ;                          // epilogue exchange over Q once every product is done
   static constexpr int kMPub = kRaw + kRawBytes;  // [2][128] running maxima
   // quantised: [4 tiles][K|V][128] row factors (f16 pairs), [8] (K, V)
-  // exponents of a tile, [128] factors of the query rows
+  // exponents of a tile (kWideTile: see there), [128] factors of the query rows
   static constexpr int kScale = kMPub + 2 * kTcRows * 4;
   static constexpr int kTileExp = kScale + (kQuant ? 4 * 2 * 128 * 4 : 0);
   static constexpr int kExpBytes = kTileExp + (kQuant ? 8 * 8 : 0);  // [8 tiles][K|V][128] exponent bytes
-  static constexpr int kQScale = kExpBytes + (kQuant ? 8 * 256 : 0);
+  static constexpr int kWide = kExpBytes + (kQuant ? 8 * 256 : 0);  // [8 tiles][128] (K factor, V exponent) of wide tiles
+  static constexpr int kQScale = kWide + (kQuant ? 8 * 128 * 8 : 0);
   static constexpr int kBad = kQScale + (kQuant ? 128 * 4 : 0);  // [HD] first keys with a non-finite V
   static constexpr int kBar = kBad + HD * 4;
   static constexpr int kNumBars = 52;
@@ -394,11 +395,26 @@ __device__ __noinline__ uint4 strip_nonfinite(uint4 v, unsigned rel, unsigned* b
 
 // Exponent bytes (e8m0) of a tile are taken relative to the tile's largest
 // one, ref: a 16-bit operand is code * 2^(byte - ref + 7), at most 448 * 2^7
-// < 65504, and exact in f16 for rows down to 2^-22 of the tile's largest
-// (smaller ones round at 2^-25 of a value of 2^15.8).  2^(ref - 127 - 7)
-// multiplies the products in 32 bits.  ref is kept from 2^-60 up, so that
-// 2^-ref and sums of it stay in range; values under 2^-75 vanish.
+// < 65504, and exact in f16 for rows down to 2^-22 of the tile's largest.
+// 2^(ref - 127 - 7) multiplies the products in 32 bits.  ref is kept from
+// 2^-60 up, so that 2^-ref and sums of it stay in range; values under 2^-75
+// vanish.
+//
+// The largest row may be one that a query does not see, or weighs with next
+// to nothing, and must not cost the others bits.  K has none to lose down to
+// 2^-22.  P is relative to max(score) * 2^ref, which overstates the largest
+// contribution by up to the spread of V's scales, and f16 has P's full 11
+// bits only down to 2^-14: P is scaled up by 2^kPShift (with the lazy maximum
+// at most 2^15), which makes up for a spread of as much.  A tile whose K
+// scales are further apart than 2^kWideK or whose V scales are than 2^kWideV
+// is *wide*: its operands are the codes as they are, the factors of each key
+// are applied to its scores in 32 bits, and V's exponent joins the score key by
+// key, as in the decode kernel (slower, on such tiles only).  Rows of zeros (byte 0 or 1, the smallest) have
+// no part in this.
 constexpr int kRefShift = 7, kRefMin = 127 - 60;
+constexpr int kPShift = 7, kWideK = 22, kWideV = kPShift;
+constexpr int kWideTile = 1 << 20;  // in place of a tile's K exponent
+static_assert(kPShift + kRescaleThreshold <= 15.f, "P in f16");
 
 // 2^e as an f16 pair for e <= 15; under 2^-24 it is 0.
 __device__ __forceinline__ uint32_t pow2_f16x2(int e) {
@@ -418,6 +434,17 @@ __device__ __forceinline__ uint4 codes_to_f16(uint2 codes, uint32_t factor) {
   e4m3x4_to_f16x2x2(codes.x, h.x, h.y);
   e4m3x4_to_f16x2x2(codes.y, h.z, h.w);
   return make_uint4(mul_f16x2(h.x, factor), mul_f16x2(h.y, factor), mul_f16x2(h.z, factor), mul_f16x2(h.w, factor));
+}
+
+// What a key of a wide tile puts on its scores: K's factor, and V's exponent,
+// from the scales' bytes.  (A NaN V scale is in the operand, and takes no part in the
+// row sum.)
+__device__ __forceinline__ float2 wide_key(int kb, int vb) {
+  return make_float2(e8m0_to_float(kb), vb == 255 ? 0.f : static_cast<float>(max(vb, kRefMin) - 127));
+}
+// 2^-e for a whole e: its bits come out of the sum with 1.5 * 2^23.
+__device__ __forceinline__ float pow2_inverse(float e) {
+  return __uint_as_float(0x3f800000u - (__float_as_uint(e + 12582912.f) << 23));
 }
 
 // Register shares of the quantised kernel's eight warpgroups (launched with 64
@@ -701,6 +728,7 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     uint32_t* factors = reinterpret_cast<uint32_t*>(sm + Cfg::kScale);
     int2* tile_exp = reinterpret_cast<int2*>(sm + Cfg::kTileExp);
     uint32_t* ring = reinterpret_cast<uint32_t*>(sm + Cfg::kExpBytes);  // [8][K|V][32]
+    float4* wide_keys = reinterpret_cast<float4*>(sm + Cfg::kWide);  // [8][128 / 2]
     const int nbox = kTcKeys / p.box;
     // box g's first byte in units of 8, ~0u without a page
     auto box_bytes = [&](int g, int phys) -> unsigned {
@@ -734,12 +762,22 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       m = __vmaxu4(m, m >> 8) & 255u;
       return max(static_cast<int>(__reduce_max_sync(0xffffffffu, m)), kRefMin);
     };
-    auto factor4 = [&](uint32_t w, int ref) -> uint4 {
+    // whether some row of the tile lies more than `most` under the largest; rows under `floor` count as that,
+    // bytes 0, 1 and 255 do not
+    auto spread_over = [&](uint32_t w, int ref, int floor, int most) -> bool {
+      uint32_t m = w | __vcmpltu4(w, 0x02020202u);
+      m = __vminu4(m, m >> 16);
+      m = __vminu4(m, m >> 8) & 255u;
+      return ref - max(static_cast<int>(__reduce_min_sync(0xffffffffu, m)), floor) > most;
+    };
+    // f16 factors of the rows relative to 2^ref, or of a wide tile: 1 for K, and for V what a byte lacks to kRefMin
+    auto factor4 = [&](uint32_t w, int ref, bool wide, bool v) -> uint4 {
       uint32_t f[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int byte = (w >> (8 * i)) & 255;
-        f[i] = byte == 255 ? 0x7fff7fffu : pow2_f16x2(byte - ref + kRefShift);
+        const int e = !wide ? byte - ref + kRefShift : v ? min(byte - kRefMin, 0) : 0;
+        f[i] = byte == 255 ? 0x7fff7fffu : pow2_f16x2(e);
       }
       return make_uint4(f[0], f[1], f[2], f[3]);
     };
@@ -751,13 +789,22 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       cp_async_wait<4>();  // tile t's group
       const uint32_t kw = cut(ring[(t & 7) * 64 + lane], t), vw = cut(ring[(t & 7) * 64 + 32 + lane], t);
       const int rk = largest(kw), rv = largest(vw);
+      const bool wide = spread_over(kw, rk, kRefMin - kWideK, kWideK) || spread_over(vw, rv, kRefMin, kWideV);
       // slot t % 4 is free once tile t-4's K and V are converted
       const bool ok = t < 4 || tc_wait(&bars->scale_free[t & 3], (t / 4 - 1) & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) break;
       uint4* f = reinterpret_cast<uint4*>(factors + (t & 3) * 256);
-      f[lane] = factor4(kw, rk);
-      f[32 + lane] = factor4(vw, rv);
-      if (lane == 0) tile_exp[t & 7] = make_int2(rk - 127 - kRefShift, rv - 127 - kRefShift);
+      f[lane] = factor4(kw, rk, wide, false);
+      f[32 + lane] = factor4(vw, rv, wide, true);
+      if (wide) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float2 a = wide_key((kw >> (8 * i)) & 255, (vw >> (8 * i)) & 255);
+          const float2 b = wide_key((kw >> (8 * i + 8)) & 255, (vw >> (8 * i + 8)) & 255);
+          wide_keys[(t & 7) * 64 + lane * 2 + i / 2] = make_float4(a.x, a.y, b.x, b.y);
+        }
+      }
+      if (lane == 0) tile_exp[t & 7] = make_int2(wide ? kWideTile : rk - 127 - kRefShift, rv - 127 - kRefShift);
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->scale_ready[t & 3]);
     }
@@ -878,7 +925,8 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
     // Quantised: scores count in units of the query row's and the tile's K
     // factor, so each tile has its own scale.  V counts in units of 2^v_exp:
     // the exponent joins the score before the maximum, so P is relative to
-    // the largest contribution to O, and leaves the row sum again.
+    // the largest contribution to O, and leaves the row sum again.  In a wide
+    // tile both belong to the key.
     float sc = p.scale_log2;
     float v_exp = 0.f, v_inv = 1.f;
     const bool pos_scale = sc >= 0.f;
@@ -903,14 +951,17 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       tc_fence_after();
       const uint32_t sbuf = lane_base + buf * kTcKeys;
       const int key0 = key_base + j * kTcKeys;
+      bool wide = false;
       if constexpr (kQuant) {
         const uint2 e = lds_v2(smem_u32(sm + Cfg::kTileExp) + (j & 7) * 8);
+        wide = e.x == kWideTile;
         sc = row_scale * pow2_f32(static_cast<int>(e.x));
         v_exp = static_cast<float>(static_cast<int>(e.y));
-        v_inv = pow2_f32(-static_cast<int>(e.y));
+        v_inv = wide ? 1.f : pow2_f32(-static_cast<int>(e.y));
       }
+      const uint32_t wide_keys = smem_u32(sm + Cfg::kWide) + (j & 7) * 1024;
       // (a negative scale, which looks for the least score, takes the masked loops)
-      const bool all_full = __all_sync(0xffffffffu, key0 + kTcKeys <= vis_end) && pos_scale;
+      const bool all_full = __all_sync(0xffffffffu, key0 + kTcKeys <= vis_end) && pos_scale && !wide;
       const float ext0 = pos_scale ? -INFINITY : INFINITY;
       float ext = ext0;
       uint32_t ra[32], rb[32];
@@ -931,6 +982,21 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
           ext_chunk32(rb, true, e);
         }
         ext = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3]));
+      } else if (kQuant && wide) {
+        ext = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < kTcKeys; c += 16) {
+          uint32_t raw[16];
+          tmem_ld16(sbuf + c, raw);
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float4 w = lds_f32x4(wide_keys + (c + i) * 8);
+            const float a = fmaf(__uint_as_float(raw[i]) * row_scale, w.x, w.y);
+            const float b = fmaf(__uint_as_float(raw[i + 1]) * row_scale, w.z, w.w);
+            ext = key0 + c + i < vis_end ? fmaxf(ext, a) : ext;
+            ext = key0 + c + i + 1 < vis_end ? fmaxf(ext, b) : ext;
+          }
+        }
       } else {
 #pragma unroll 1
         for (int c = 0; c < kTcKeys; c += 16) {
@@ -944,7 +1010,8 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
           }
         }
       }
-      const float mx = (ext == INFINITY || ext == -INFINITY) ? -INFINITY : kQuant ? fmaf(ext, sc, v_exp) : ext * sc;
+      float mx = kQuant ? (wide ? ext : fmaf(ext, sc, v_exp)) - kPShift : ext * sc;
+      mx = (ext == INFINITY || ext == -INFINITY) ? -INFINITY : mx;
       float m_in = -INFINITY;
       if (j > 0) {
         const int pj = j - 1;
@@ -1000,6 +1067,24 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
         float a, bb;
         f2_unpack(f2_add(acc0, acc1), a, bb);
         rs = a + bb;
+      } else if (kQuant && wide) {
+#pragma unroll 1
+        for (int c = 0; c < kTcKeys; c += 16) {
+          uint32_t raw[16];
+          tmem_ld16(sbuf + c, raw);
+          uint32_t packed[8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float4 w = lds_f32x4(wide_keys + (c + i) * 8);
+            const float a = fmaf(__uint_as_float(raw[i]) * row_scale, w.x, w.y - m_j);
+            const float b = fmaf(__uint_as_float(raw[i + 1]) * row_scale, w.z, w.w - m_j);
+            const float p0 = key0 + c + i < vis_end ? fast_exp2(a) : 0.f;
+            const float p1 = key0 + c + i + 1 < vis_end ? fast_exp2(b) : 0.f;
+            rs = fmaf(p0, pow2_inverse(w.y), fmaf(p1, pow2_inverse(w.w), rs));
+            packed[i >> 1] = Elem<MT>::pack(p0, p1);
+          }
+          tmem_st8(sbuf + (c >> 1), packed);
+        }
       } else {
 #pragma unroll 1
         for (int c = 0; c < kTcKeys; c += 16) {
