@@ -401,7 +401,7 @@ int mxfa_kvcache_gather_varlen_launch(const void* k_cache, const void* v_cache, 
 /* Quantised caches to 16-bit ones for one attention call: sequence b's tokens
  * 0 .. seqlens[b] to rows b * rows .. of k_out, v_out [B, rows, HKV, D], and
  * table_out [B] = 0 .. B-1, the block table that reads them as B pages of
- * `rows` tokens.  fp16 saturates at 65504. */
+ * `rows` tokens.  fp16 saturates at 65504 and rounds under 2^-24. */
 int mxfa_kvcache_unpack_launch(const void* k_cache, const void* v_cache, const void* k_scales,
                                const void* v_scales, const int32_t* seqlens, const int32_t* block_table,
                                void* k_out, void* v_out, int32_t* table_out, int B, int rows, int HKV,
@@ -438,6 +438,24 @@ int mxfa_kvcache_varlen_attention_launch(const void* q, const void* k_cache, con
                                          int PS, int BTW, int num_pages,
                                          size_t q_token_stride, size_t q_head_stride, int causal,
                                          int bf16, float scale, void* stream);
+
+/* The same for fp16 queries over a quantised cache by way of unpacked rows
+ * (k_rows, v_rows fp16 [B, rows, HKV, D], table_out [B], as
+ * mxfa_kvcache_unpack_launch writes them): tiles whose rows fp16 holds exactly
+ * run on them, tiles with a value past 65,504 or with bits under 2^-24 on the
+ * cache itself, so the result does not depend on which.  `inexact`
+ * (mxfa_unpack_flag_bytes) is scratch that says which are which.  Page sizes
+ * that are multiples of 8 and up to 128 query heads per KV head. */
+size_t mxfa_unpack_flag_bytes(int B, int rows);
+int mxfa_kvcache_varlen_attention_half_launch(const void* q, const void* k_cache, const void* v_cache,
+                                              const void* k_scales, const void* v_scales,
+                                              const int32_t* cu_seqlens_q, const int32_t* seqlens,
+                                              const int32_t* block_table, const void* plan, size_t plan_bytes,
+                                              void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                              unsigned* counters, void* k_rows, void* v_rows, int32_t* table_out,
+                                              int32_t* inexact, int total_q, int B, int HQ, int HKV, int D, int PS,
+                                              int BTW, int num_pages, int rows, size_t q_token_stride,
+                                              size_t q_head_stride, int causal, float scale, void* stream);
 
 /* The same attention for a decode step: every sequence has at most max_q
  * packed queries (one, usually; more query rows than 16 per KV head re-read

@@ -93,6 +93,10 @@ SIGNATURES = {
     "mxfa_kvcache_varlen_attention_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _sz, _sz, _i, _i, _f,
              _vp]),
+    "mxfa_unpack_flag_bytes": (_sz, [_i, _i]),
+    "mxfa_kvcache_varlen_attention_half_launch": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i,
+             _i, _i, _i, _i, _i, _sz, _sz, _i, _f, _vp]),
     "mxfa_kvcache_step_attention_launch": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i,
              _i, _i, _i, _i, _f, _vp]),

@@ -563,6 +563,17 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
                 rows = -(-max_seqlen_k // 128) * 128
                 kv = q.new_empty((2, B, rows, HKV, D))
                 pages_of = q.new_empty((B, 1), dtype=torch.int32)
+                if q.dtype == torch.float16:
+                    # fp16 does not hold every code * scale: tiles with such a value run on the cache itself
+                    inexact = q.new_empty((int(lib.mxfa_unpack_flag_bytes(B, rows)) // 4,), dtype=torch.int32)
+                    rc = lib.mxfa_kvcache_varlen_attention_half_launch(
+                        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                        cu.data_ptr(), seq.data_ptr(), bt.data_ptr(), table.data_ptr(), table.numel() * 4,
+                        out.data_ptr(), _lib.ptr(lse), ws.data_ptr(), ws_bytes, counters.data_ptr(), kv.data_ptr(),
+                        kv[1].data_ptr(), pages_of.data_ptr(), inexact.data_ptr(), Tq, B, HQ, HKV, D, PS, bt.shape[1],
+                        pages, rows, q.stride(0), q.stride(1), int(causal), float(softmax_scale), stream)
+                    _lib.check(rc, "mxfa_kvcache_varlen_attention_half_launch")
+                    return (out, lse) if return_lse else out
                 rc = lib.mxfa_kvcache_unpack_launch(
                     k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), seq.data_ptr(),
                     bt.data_ptr(), kv.data_ptr(), kv[1].data_ptr(), pages_of.data_ptr(), B, rows, HKV, D, PS,

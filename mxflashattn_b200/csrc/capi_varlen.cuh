@@ -148,7 +148,8 @@ int launch_chunk(const ChunkParams& p, int D, bool quant, dim3 grid, const CUten
 }
 
 int run_chunk(const VarlenAttnParams& a, int D, const void* plan, size_t plan_bytes, void* workspace,
-              size_t workspace_bytes, unsigned* counters, bool bf16, cudaStream_t st) {
+              size_t workspace_bytes, unsigned* counters, bool bf16, cudaStream_t st, const int* inexact = nullptr,
+              int unpacked = 0) {
   const bool quant = a.k_scales != nullptr;
   if (plan == nullptr || plan_bytes < mxfa_chunk_plan_bytes(a.T, a.B, a.HQ, a.HKV) || !aligned16(plan))
     return fail(MXFA_ERR_INVALID, "plan missing, too small or unaligned (%zu < %zu bytes)", plan_bytes,
@@ -166,6 +167,8 @@ int run_chunk(const VarlenAttnParams& a, int D, const void* plan, size_t plan_by
   p.lse = a.lse;
   p.k_scales = a.k_scales;
   p.v_scales = a.v_scales;
+  p.inexact = inexact;
+  p.unpacked = unpacked;
   p.parts_cap = chunk_parts_cap(a.HKV);
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<size_t>(a.HKV) * p.parts_cap * kTcRows * D;
@@ -207,6 +210,90 @@ int run_chunk(const VarlenAttnParams& a, int D, const void* plan, size_t plan_by
   if (grid.y > 65535) return fail(MXFA_ERR_UNSUPPORTED, "%u items exceed the grid", grid.y);
   return bf16 ? launch_chunk<__nv_bfloat16>(p, D, quant, grid, mq, maps, st)
               : launch_chunk<__half>(p, D, quant, grid, mq, maps, st);
+}
+
+// Checks of a ragged attention call, and its parameters (T = 0 where there is nothing to do).
+int varlen_params(VarlenAttnParams* params, const void* q, const void* k_cache, const void* v_cache,
+                  const void* k_scales, const void* v_scales, const int32_t* cu_seqlens_q, const int32_t* seqlens,
+                  const int32_t* block_table, void* out, float* lse, int total_q, int B, int HQ, int HKV, int D, int PS,
+                  int BTW, int num_pages, size_t q_token_stride, size_t q_head_stride, int causal, float scale) {
+  VarlenAttnParams& p = *params;
+  if (HKV <= 0 || HQ <= 0 || HQ % HKV != 0)
+    return fail(MXFA_ERR_INVALID, "bad head geometry (HQ=%d HKV=%d)", HQ, HKV);
+  if (int rc = paged_varlen_checks(k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqlens, block_table, total_q,
+                                   B, HKV, D, PS, BTW, num_pages))
+    return rc;
+  if (total_q == 0 || B == 0) return MXFA_OK;
+  if (!q || !out) return fail(MXFA_ERR_INVALID, "null tensor pointer");
+  if (!aligned16(q) || !aligned16(out) || (q_token_stride | q_head_stride) % 8 != 0)
+    return fail(MXFA_ERR_INVALID, "q rows and out must be 16-byte aligned");
+  const long long rows = static_cast<long long>(total_q) * HQ;
+  if (rows > INT_MAX) return fail(MXFA_ERR_UNSUPPORTED, "%lld query rows above 2^31-1", rows);
+  p.q = q;
+  p.q_tok = q_token_stride;
+  p.q_head = q_head_stride;
+  p.k = static_cast<const uint8_t*>(k_cache);
+  p.v = static_cast<const uint8_t*>(v_cache);
+  p.k_scales = static_cast<const uint8_t*>(k_scales);
+  p.v_scales = static_cast<const uint8_t*>(v_scales);
+  p.cu = cu_seqlens_q;
+  p.seqlens = seqlens;
+  p.bt = block_table;
+  p.out = out;
+  p.lse = lse;
+  p.T = total_q;
+  p.B = B;
+  p.HQ = HQ;
+  p.HKV = HKV;
+  p.GQ = HQ / HKV;
+  p.PS = PS;
+  p.BTW = BTW;
+  p.P = num_pages;
+  p.causal = causal ? 1 : 0;
+  p.scale_log2 = scale * kLog2e;
+  return MXFA_OK;
+}
+
+// Unpacks a quantised cache's sequences (mxfa_kvcache_unpack_launch); inexact: see PagedVarlenParams.
+int unpack_impl(const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
+                const int32_t* seqlens, const int32_t* block_table, void* k_out, void* v_out,
+                int32_t* table_out, int B, int rows, int HKV, int D, int PS, int BTW, int num_pages,
+                int bf16, int32_t* inexact, cudaStream_t st) {
+  // (the lengths stand in for the offsets, which this call has none of)
+  if (int rc = paged_varlen_checks(k_cache, v_cache, k_scales, v_scales, seqlens, seqlens, block_table, rows, B, HKV,
+                                   D, PS, BTW, num_pages))
+    return rc;
+  if (rows == 0 || B == 0) return MXFA_OK;
+  if (k_scales == nullptr) return fail(MXFA_ERR_INVALID, "unpacking is for quantised caches");
+  if (!k_out || !v_out || !table_out) return fail(MXFA_ERR_INVALID, "null tensor pointer");
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(MXFA_ERR_INVALID, "outputs must be 16-byte aligned");
+  if (B > 65535) return fail(MXFA_ERR_UNSUPPORTED, "%d sequences exceed the grid", B);
+  PagedVarlenParams p{};
+  p.k = k_out;
+  p.v = v_out;
+  p.k_cache = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  p.v_cache = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  p.k_scales = static_cast<uint8_t*>(const_cast<void*>(k_scales));
+  p.v_scales = static_cast<uint8_t*>(const_cast<void*>(v_scales));
+  p.seqlens = seqlens;
+  p.bt = block_table;
+  p.T = rows;
+  p.B = B;
+  p.HKV = HKV;
+  p.PS = PS;
+  p.BTW = BTW;
+  p.P = num_pages;
+  p.tok_per_cta = kPvMaxTok;
+  p.table = table_out;
+  p.inexact = inexact;
+  const dim3 grid(unpacked_blocks(rows), B);
+  if (bf16)
+    D == 128 ? gather_varlen_kernel<__nv_bfloat16, 128, true, true><<<grid, kPvThreads, 0, st>>>(p)
+             : gather_varlen_kernel<__nv_bfloat16, 64, true, true><<<grid, kPvThreads, 0, st>>>(p);
+  else
+    D == 128 ? gather_varlen_kernel<__half, 128, true, true><<<grid, kPvThreads, 0, st>>>(p)
+             : gather_varlen_kernel<__half, 64, true, true><<<grid, kPvThreads, 0, st>>>(p);
+  return check_launch("gather_varlen_kernel(dense)");
 }
 
 }  // namespace
@@ -343,40 +430,11 @@ int mxfa_kvcache_varlen_attention_launch(const void* q, const void* k_cache, con
                                          size_t workspace_bytes, unsigned* counters, int total_q, int B, int HQ, int HKV, int D, int PS, int BTW, int num_pages,
                                          size_t q_token_stride, size_t q_head_stride, int causal, int bf16,
                                          float scale, void* stream) {
-  if (HKV <= 0 || HQ <= 0 || HQ % HKV != 0)
-    return fail(MXFA_ERR_INVALID, "bad head geometry (HQ=%d HKV=%d)", HQ, HKV);
-  if (int rc = paged_varlen_checks(k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqlens, block_table, total_q,
-                                   B, HKV, D, PS, BTW, num_pages))
-    return rc;
-  if (total_q == 0 || B == 0) return MXFA_OK;
-  if (!q || !out) return fail(MXFA_ERR_INVALID, "null tensor pointer");
-  if (!aligned16(q) || !aligned16(out) || (q_token_stride | q_head_stride) % 8 != 0)
-    return fail(MXFA_ERR_INVALID, "q rows and out must be 16-byte aligned");
-  const long long rows = static_cast<long long>(total_q) * HQ;
-  if (rows > INT_MAX) return fail(MXFA_ERR_UNSUPPORTED, "%lld query rows above 2^31-1", rows);
   VarlenAttnParams p{};
-  p.q = q;
-  p.q_tok = q_token_stride;
-  p.q_head = q_head_stride;
-  p.k = static_cast<const uint8_t*>(k_cache);
-  p.v = static_cast<const uint8_t*>(v_cache);
-  p.k_scales = static_cast<const uint8_t*>(k_scales);
-  p.v_scales = static_cast<const uint8_t*>(v_scales);
-  p.cu = cu_seqlens_q;
-  p.seqlens = seqlens;
-  p.bt = block_table;
-  p.out = out;
-  p.lse = lse;
-  p.T = total_q;
-  p.B = B;
-  p.HQ = HQ;
-  p.HKV = HKV;
-  p.GQ = HQ / HKV;
-  p.PS = PS;
-  p.BTW = BTW;
-  p.P = num_pages;
-  p.causal = causal ? 1 : 0;
-  p.scale_log2 = scale * kLog2e;
+  if (int rc = varlen_params(&p, q, k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqlens, block_table, out, lse,
+                             total_q, B, HQ, HKV, D, PS, BTW, num_pages, q_token_stride, q_head_stride, causal, scale))
+    return rc;
+  if (p.T == 0) return MXFA_OK;
   const bool quant = k_scales != nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (chunk_tiled(HQ, HKV, PS))
@@ -417,41 +475,45 @@ int mxfa_kvcache_unpack_launch(const void* k_cache, const void* v_cache, const v
                                const int32_t* seqlens, const int32_t* block_table, void* k_out, void* v_out,
                                int32_t* table_out, int B, int rows, int HKV, int D, int PS, int BTW, int num_pages,
                                int bf16, void* stream) {
-  // (the lengths stand in for the offsets, which this call has none of)
-  if (int rc = paged_varlen_checks(k_cache, v_cache, k_scales, v_scales, seqlens, seqlens, block_table, rows, B, HKV,
-                                   D, PS, BTW, num_pages))
+  return unpack_impl(k_cache, v_cache, k_scales, v_scales, seqlens, block_table, k_out, v_out, table_out, B, rows, HKV,
+                     D, PS, BTW, num_pages, bf16, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+size_t mxfa_unpack_flag_bytes(int B, int rows) {
+  return B <= 0 || rows <= 0 ? 0 : static_cast<size_t>(B) * unpacked_blocks(rows) * sizeof(int32_t);
+}
+
+int mxfa_kvcache_varlen_attention_half_launch(const void* q, const void* k_cache, const void* v_cache,
+                                              const void* k_scales, const void* v_scales,
+                                              const int32_t* cu_seqlens_q, const int32_t* seqlens,
+                                              const int32_t* block_table, const void* plan, size_t plan_bytes,
+                                              void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                              unsigned* counters, void* k_rows, void* v_rows, int32_t* table_out,
+                                              int32_t* inexact, int total_q, int B, int HQ, int HKV, int D, int PS,
+                                              int BTW, int num_pages, int rows, size_t q_token_stride,
+                                              size_t q_head_stride, int causal, float scale, void* stream) {
+  VarlenAttnParams p{};
+  if (int rc = varlen_params(&p, q, k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqlens, block_table, out, lse,
+                             total_q, B, HQ, HKV, D, PS, BTW, num_pages, q_token_stride, q_head_stride, causal, scale))
     return rc;
-  if (rows == 0 || B == 0) return MXFA_OK;
-  if (k_scales == nullptr) return fail(MXFA_ERR_INVALID, "unpacking is for quantised caches");
-  if (!k_out || !v_out || !table_out) return fail(MXFA_ERR_INVALID, "null tensor pointer");
-  if (!aligned16(k_out) || !aligned16(v_out)) return fail(MXFA_ERR_INVALID, "outputs must be 16-byte aligned");
-  if (B > 65535) return fail(MXFA_ERR_UNSUPPORTED, "%d sequences exceed the grid", B);
-  PagedVarlenParams p{};
-  p.k = k_out;
-  p.v = v_out;
-  p.k_cache = static_cast<uint8_t*>(const_cast<void*>(k_cache));
-  p.v_cache = static_cast<uint8_t*>(const_cast<void*>(v_cache));
-  p.k_scales = static_cast<uint8_t*>(const_cast<void*>(k_scales));
-  p.v_scales = static_cast<uint8_t*>(const_cast<void*>(v_scales));
-  p.seqlens = seqlens;
-  p.bt = block_table;
-  p.T = rows;
-  p.B = B;
-  p.HKV = HKV;
-  p.PS = PS;
-  p.BTW = BTW;
-  p.P = num_pages;
-  p.tok_per_cta = kPvMaxTok;
-  p.table = table_out;
-  const dim3 grid((rows + kPvMaxTok - 1) / kPvMaxTok, B);
+  if (p.T == 0) return MXFA_OK;
+  if (!chunk_tiled(HQ, HKV, PS)) return fail(MXFA_ERR_UNSUPPORTED, "not a call of the tiled kernel (page size %d)", PS);
+  if (rows <= 0 || inexact == nullptr) return fail(MXFA_ERR_INVALID, "unpacked rows or their flags missing");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (bf16)
-    D == 128 ? gather_varlen_kernel<__nv_bfloat16, 128, true, true><<<grid, kPvThreads, 0, st>>>(p)
-             : gather_varlen_kernel<__nv_bfloat16, 64, true, true><<<grid, kPvThreads, 0, st>>>(p);
-  else
-    D == 128 ? gather_varlen_kernel<__half, 128, true, true><<<grid, kPvThreads, 0, st>>>(p)
-             : gather_varlen_kernel<__half, 64, true, true><<<grid, kPvThreads, 0, st>>>(p);
-  return check_launch("gather_varlen_kernel(dense)");
+  if (int rc = unpack_impl(k_cache, v_cache, k_scales, v_scales, seqlens, block_table, k_rows, v_rows, table_out, B, rows,
+                           HKV, D, PS, BTW, num_pages, 0, inexact, st))
+    return rc;
+  VarlenAttnParams unpacked = p;
+  unpacked.k = static_cast<const uint8_t*>(k_rows);
+  unpacked.v = static_cast<const uint8_t*>(v_rows);
+  unpacked.k_scales = unpacked.v_scales = nullptr;
+  unpacked.bt = table_out;
+  unpacked.PS = rows;
+  unpacked.BTW = 1;
+  unpacked.P = B;
+  if (int rc = run_chunk(unpacked, D, plan, plan_bytes, workspace, workspace_bytes, counters, false, st, inexact, rows))
+    return rc;
+  return run_chunk(p, D, plan, plan_bytes, workspace, workspace_bytes, counters, false, st, inexact, rows);
 }
 
 }  // extern "C"

@@ -297,6 +297,12 @@ struct ChunkParams {
   float* part_ml;   // [HKV][parts_cap][128][2]
   unsigned* counters;  // [HKV][parts_cap / 2 + 1], zero on entry and on exit
   int parts_cap;
+  // fp16 queries over unpacked rows (optional): which blocks of kPvMaxTok
+  // tokens of the first `unpacked` of a sequence fp16 does not hold exactly.
+  // Items with such a token are left to the converting kernel, which is
+  // launched behind the 16-bit one and takes no others.
+  const int* inexact;
+  int unpacked;
   int T, B, HQ, HKV, GQ, PS, BTW, P;
   int box;       // rows of one TMA box: divides PS and 128, a multiple of 8
   int causal;
@@ -495,6 +501,14 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
       (it.nsplit > 1 && (it.part0 < 0 || it.part0 > p.parts_cap - it.nsplit || it.group < 0 || it.group > p.parts_cap / 2))) {
     if (threadIdx.x == 0) raise_flag(MXFA_FLAG_BAD_ORDER);
     return;
+  }
+  if (p.inexact != nullptr) {
+    constexpr int kPer = kTcKeys / kPvMaxTok;  // blocks of a key tile
+    const int end = min(min(it.kt1, (p.unpacked + kTcKeys - 1) / kTcKeys) * kPer, unpacked_blocks(min(it.total, p.unpacked)));
+    const int* f = p.inexact + static_cast<size_t>(it.b) * unpacked_blocks(p.unpacked);
+    int lost = 0;
+    for (int i = it.kt0 * kPer + threadIdx.x; i < end; i += Cfg::kThreads) lost |= f[i];
+    if ((__syncthreads_or(lost) != 0) != kQuant) return;
   }
   // keys the block table can hold; a longer sequence is flagged and cut
   const int k_lim = min(it.total, p.BTW * p.PS);

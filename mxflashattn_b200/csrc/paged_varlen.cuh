@@ -72,10 +72,13 @@ struct PagedVarlenParams {
   int T, B, HKV, PS, BTW, P;
   int tok_per_cta;
   int* table;  // dense read-back: [B], written
+  int* inexact;  // dense read-back to fp16, optional: [B][unpacked_blocks(T)], written for the tokens that exist
 };
 
 constexpr int kPvThreads = 256;
 constexpr int kPvMaxTok = 16;  // tokens of one CTA (8 to 32 differ by 7%)
+// CTAs of a sequence of `rows` unpacked tokens.
+__host__ __device__ __forceinline__ int unpacked_blocks(int rows) { return (rows + kPvMaxTok - 1) / kPvMaxTok; }
 
 // The cache slots of this CTA's tokens (page -1: not mapped), a token per lane of
 // the first warp: one search for the first token, then each lane walks on to
@@ -263,7 +266,9 @@ __device__ __forceinline__ uint32_t pack_sat(float lo, float hi) {
 // kDense: every sequence's tokens from position 0 on, sequence b (blockIdx.y)
 // to rows b * T .. of the output, T rows a sequence, with the table
 // (sequence b: page b) that reads the output as a cache of pages of T tokens.
-// Rows past a sequence's length are left alone.
+// Rows past a sequence's length are left alone.  To fp16, p.inexact says of
+// each CTA's tokens whether some value is not one of fp16's: past 65,504 (it
+// saturates) or with bits under 2^-24.
 template <typename T, int HD, bool kQuant, bool kDense = false>
 __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVarlenParams p) {
   constexpr int kGroup = HD / 8;
@@ -284,8 +289,9 @@ __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVa
   }
   const int sub = threadIdx.x % kGroup;
   const RowWalk walk = row_walk<kGroup>(2 * p.HKV);
-  if (!walk.live) return;
-  for (int pair = walk.pair; pair < 2 * p.HKV; pair += kPvThreads / kGroup) {
+  constexpr bool kCheck = kDense && std::is_same_v<T, __half>;
+  int lost = 0;
+  for (int pair = walk.live ? walk.pair : 2 * p.HKV; pair < 2 * p.HKV; pair += kPvThreads / kGroup) {
     const int kv = pair >= p.HKV, h = pair - kv * p.HKV;
     const uint8_t* cache = kv ? p.v_cache : p.k_cache;
     const uint8_t* scales = kv ? p.v_scales : p.k_scales;
@@ -320,10 +326,24 @@ __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVa
           // read back, a value past fp16's largest is its infinity; as an operand it saturates
           auto pack = [](float lo, float hi) { return kDense ? pack_sat<T>(lo, hi) : Elem<T>::pack(lo, hi); };
           out[u] = make_uint4(pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7]));
+          if (kCheck && byte[u] - 112u > 22u) {  // (448 * 2^7 fits, and so does 2^-9, the codes' last place, times 2^-15)
+            const uint32_t w[4] = {out[u].x, out[u].y, out[u].z, out[u].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = Elem<T>::unpack(w[j]);
+              lost |= f.x != x[2 * j] && x[2 * j] == x[2 * j];
+              lost |= f.y != x[2 * j + 1] && x[2 * j + 1] == x[2 * j + 1];
+            }
+          }
         }
         if (i < n) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(i) * p.HKV * HD) = out[u];
       }
     }
+  }
+  if constexpr (kCheck) {
+    lost = __syncthreads_or(lost);
+    if (threadIdx.x == 0 && p.inexact != nullptr)
+      p.inexact[static_cast<size_t>(blockIdx.y) * unpacked_blocks(p.T) + blockIdx.x] = lost;
   }
 }
 

@@ -16,7 +16,7 @@ from varlen_oracle import attention64, make_batch
 pytestmark = pytest.mark.gpu
 
 
-@pytest.fixture(params=["converted"])
+@pytest.fixture(params=["converted", "unpacked", "by the rule"])
 def path(request, monkeypatch):
     """Sets the way that the quantised calls go, and tells it for a batch: True where its rows are unpacked first."""
     from mxflashattn_b200 import backend
