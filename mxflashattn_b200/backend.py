@@ -17,6 +17,7 @@ stream and reads nothing back to the host.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 
 import torch
 
@@ -28,7 +29,7 @@ SUPPORTED_DTYPES = (torch.float16, torch.bfloat16)
 # torch's own unwrapped queries of the current device and stream: a tenth of the time of the public
 # functions, which build a context check or a Stream object around them
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_capturing = torch.cuda.is_current_stream_capturing
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -143,8 +144,6 @@ _PLANS: dict[tuple, tuple[int, int]] = {}
 
 def kvcache_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, head_dim: int, max_len: int):
     """(num_splits, chunk_len) the library picks for this shape on the current device (cached)."""
-    import ctypes
-
     key = (_current_device() if (_CUDA_OK or torch.cuda.is_available()) else -1, batch, q_len, q_heads,
            kv_heads, head_dim, max_len)
     plan = _PLANS.get(key)
@@ -162,8 +161,6 @@ _CAPTURE_COUNTERS: dict[tuple, tuple[int, "torch.Tensor"]] = {}
 
 def _capture_id(device, stream_handle: int) -> int:
     """Id of the graph capture that the stream is part of (ids are never used twice), 0 without one."""
-    import ctypes
-
     if device.type != "cuda" or not _capturing():
         return 0
     out = ctypes.c_ulonglong(0)
