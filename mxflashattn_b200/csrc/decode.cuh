@@ -947,8 +947,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
 
     // row scales: K's factor, V's exponent and its inverse for the two tokens
     // (rows g and g + 8 of the product) this thread holds.  V's exponents are
-    // kept from -60 up, for the range of the row sum; a V row under that
-    // counts with 2^-60, an error below 2^-51 in an output.
+    // kept from -60 up, for the range of the row sum; for a V row under that
+    // P takes the rest before it meets V (f16: values under 2^-75 vanish).
     float kf[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f}, iv[2] = {1.f, 1.f};
     uint32_t vb[2] = {127u, 127u};
     if constexpr (kRowScale) {
@@ -1034,14 +1034,18 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPer
         s[nt][c + 2] = p1;
       }
     if constexpr (kRowScale) {
-      // a NaN V scale: the outputs of the rows that see the token, not their sums
-      if (__any_sync(0xffffffffu, max(vb[0], vb[1]) == 255u)) {
+      // V scales of NaN: the outputs of the rows that see the token, not their
+      // sums; under 2^-60: what the exponent lacks.
+      const bool odd = max(vb[0], vb[1]) == 255u || min(vb[0], vb[1]) < 67u;
+      if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (vb[e >> 1] == 255u && pos0 + fp8_tok(g + 8 * (e >> 1)) <= lim[nt][e & 1])
-              s[nt][e] = __uint_as_float(0x7fffffffu);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t v = vb[e >> 1];
+            if (v < 67u) s[nt][e] *= __uint_as_float((v + 60u) << 23);  // 2^(v - 67)
+            if (v == 255u && pos0 + fp8_tok(g + 8 * (e >> 1)) <= lim[nt][e & 1]) s[nt][e] = __uint_as_float(0x7fffffffu);
+          }
       }
     }
     // the running max rarely moves after the first tiles: rescale O only when it did
