@@ -202,6 +202,10 @@ __device__ __forceinline__ void load_partial(const float* src, float (&o)[HD / 3
   }
 }
 
+// Whether a split's (m, d) takes part in a merge: not when it saw no key.  A
+// NaN state does, so a NaN in a visible key reaches the output.
+__device__ __forceinline__ bool split_counts(float2 v) { return v.x != -INFINITY && !(v.y <= 0.f); }
+
 // The reduction behind merge_split_row and merge_split_row_publish: M, L and
 // the unnormalised sum of the weighted partial rows (this lane's columns).
 // For NP <= 64 every lane loads the (m, d) pairs of splits lane and lane+32
@@ -212,10 +216,6 @@ __device__ __forceinline__ void load_partial(const float* src, float (&o)[HD / 3
 // pairs.  The arithmetic and its order are those of the loop form below
 // (used for NP > 64, and always when kChunked is false): the same M, L and
 // accumulation, bit for bit.
-// Whether a split's (m, d) takes part in a merge: not when it saw no key.  A
-// NaN state does, so a NaN in a visible key reaches the output.
-__device__ __forceinline__ bool split_counts(float2 v) { return v.x != -INFINITY && !(v.y <= 0.f); }
-
 template <int HD, bool kChunked = true>
 __device__ __forceinline__ void merge_split_core(const float* ows, const float* mdws, int r, int NP, int lane,
                                                  float (&acc)[HD / 32], float& M_out, float& L_out) {
@@ -347,7 +347,7 @@ __device__ __forceinline__ void merge_split_row_publish(const float* ows, const 
   float acc[kPer], M, L;
   merge_split_core<HD, kChunked>(ows, mdws, r, NP, lane, acc, M, L);
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  const float lse = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+  const float lse = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
   for (int dst = 0; dst < world; ++dst) {
     uint64_t* rec = reinterpret_cast<uint64_t*>(bufs[dst] + rec_off) + (static_cast<size_t>(rank) * rows + r) * (HD + 2);
 #pragma unroll
@@ -378,7 +378,8 @@ __device__ __noinline__ void merge_split_row_publish_call(const float* ows, cons
 // order, once each lane has seen step tag `tag` on its words (bounded wait:
 // after kWaitLimitNs from t0 the lane stops waiting, raises the timeout flag
 // and merges what it has), and write the output row and its LSE.  A record
-// (O, lse) is the partial (o = O, m = lse * log2 e, d = 1).
+// (O, lse) is the partial (o = O, m = lse * log2 e, d = 1).  A rank without
+// keys (-inf) takes no part, one of NaN makes the row NaN.
 template <typename T, int HD>
 __device__ __forceinline__ void cp_merge_row(const uint64_t* recs, int rows, int r, int world, int lane, T* out,
                                              float* lse, unsigned tag, unsigned long long t0) {
@@ -407,8 +408,8 @@ __device__ __forceinline__ void cp_merge_row(const uint64_t* recs, int rows, int
       }
     }
     const float mz = __uint_as_float(static_cast<uint32_t>(wl)) * kLog2e;
-    if (!(mz > -INFINITY)) continue;
-    const float mn = fmaxf(M, mz);
+    if (mz == -INFINITY) continue;
+    const float mn = fmax_nan(M, mz);
     const float f1 = fast_exp2(M - mn);
     const float f2 = fast_exp2(mz - mn);
 #pragma unroll
@@ -421,7 +422,7 @@ __device__ __forceinline__ void cp_merge_row(const uint64_t* recs, int rows, int
 #pragma unroll
   for (int j = 0; j < kPer; j += 2)
     *reinterpret_cast<uint32_t*>(op + j) = Elem<T>::pack(acc[j] * inv, acc[j + 1] * inv);
-  if (lse != nullptr && lane == 0) lse[r] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+  if (lse != nullptr && lane == 0) lse[r] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
 }
 template <typename T, int HD>
 __device__ __noinline__ void cp_merge_row_call(const uint64_t* recs, int rows, int r, int world, int lane, T* out,
@@ -1312,8 +1313,8 @@ __global__ void __launch_bounds__(128) split_combine_kernel(const float* __restr
       dz = mdws[pi * 2 + 1];
       src = ows + pi * HD;
     }
-    if (!(mz > -INFINITY) || !(dz > 0.f)) continue;
-    const float mn = fmaxf(M, mz);
+    if (!split_counts(make_float2(mz, dz))) continue;
+    const float mn = fmax_nan(M, mz);
     const float f1 = fast_exp2(M - mn);
     const float f2 = fast_exp2(mz - mn);
     float vals[kPer];
@@ -1339,13 +1340,13 @@ __global__ void __launch_bounds__(128) split_combine_kernel(const float* __restr
     float* row = out_f32 + static_cast<size_t>(r) * (HD + 1);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) row[lane * kPer + j] = acc[j] * inv;
-    if (lane == 0) row[HD] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+    if (lane == 0) row[HD] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
   } else {
     if (out_f32 != nullptr) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) out_f32[static_cast<size_t>(r) * HD + lane * kPer + j] = acc[j] * inv;
     }
-    if (lse != nullptr && lane == 0) lse[r] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+    if (lse != nullptr && lane == 0) lse[r] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
   }
 }
 
