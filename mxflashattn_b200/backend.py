@@ -140,10 +140,11 @@ def flash_attn_func(q, k, v, causal, softmax_scale, *, return_lse: bool = False,
 # ------------------------------------------------------------------ decode
 
 _PLANS: dict[tuple, tuple[int, int]] = {}
+_PLANS_KEPT = 4096  # a serving loop may ask for another length every step
 
 
 def kvcache_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, head_dim: int, max_len: int):
-    """(num_splits, chunk_len) the library picks for this shape on the current device (cached)."""
+    """(num_splits, chunk_len) the library picks for this shape on the current device (cached, the latest ones)."""
     key = (_current_device() if (_CUDA_OK or torch.cuda.is_available()) else -1, batch, q_len, q_heads,
            kv_heads, head_dim, max_len)
     plan = _PLANS.get(key)
@@ -151,6 +152,8 @@ def kvcache_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, head_dim: 
         np_, cl = ctypes.c_int(0), ctypes.c_int(0)
         _lib.check(_L().mxfa_kvcache_plan(batch, q_len, q_heads, kv_heads, head_dim, max_len,
                                                   ctypes.byref(np_), ctypes.byref(cl)), "mxfa_kvcache_plan")
+        if len(_PLANS) >= _PLANS_KEPT:
+            _PLANS.clear()
         plan = _PLANS[key] = (int(np_.value), int(cl.value))
     return plan
 
