@@ -206,8 +206,9 @@ int run_chunk(const VarlenAttnParams& a, int D, const void* plan, size_t plan_by
       return fail(MXFA_ERR_UNSUPPORTED, "TMA descriptor encoding failed for the queries");
     g_chunk_q_maps.put(qkey, mq);
   }
-  const dim3 grid(a.HKV, chunk_items_cap(a.T, a.B, a.HQ, a.HKV));
-  if (grid.y > 65535) return fail(MXFA_ERR_UNSUPPORTED, "%u items exceed the grid", grid.y);
+  const long long blocks = static_cast<long long>(a.HKV) * chunk_items_cap(a.T, a.B, a.HQ, a.HKV);
+  if (blocks > INT_MAX) return fail(MXFA_ERR_UNSUPPORTED, "%lld items exceed the grid", blocks);
+  const dim3 grid(static_cast<unsigned>(blocks));
   return bf16 ? launch_chunk<__nv_bfloat16>(p, D, quant, grid, mq, maps, st)
               : launch_chunk<__half>(p, D, quant, grid, mq, maps, st);
 }

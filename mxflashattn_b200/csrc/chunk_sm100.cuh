@@ -492,9 +492,10 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   int* s_last = reinterpret_cast<int*>(tmem_slot + 3);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = blockIdx.x;
-  if (static_cast<int>(blockIdx.y) >= p.plan[0]) return;
-  const ChunkItem it = reinterpret_cast<const ChunkItem*>(p.plan + kPlanHeader)[blockIdx.y];
+  // block: KV head, then item (one dimension, which alone has room for more than 65,535)
+  const int hk = blockIdx.x % p.HKV, item = blockIdx.x / p.HKV;
+  if (item >= p.plan[0]) return;
+  const ChunkItem it = reinterpret_cast<const ChunkItem*>(p.plan + kPlanHeader)[item];
   // a plan made for another batch reaches nothing outside this one's tensors
   if (it.b < 0 || it.b >= p.B || it.row0 < 0 || it.ntok < 1 || it.ntok * p.GQ > kTcRows || it.row0 > p.T - it.ntok ||
       it.kt0 < 0 || it.nsplit < 1 || it.nsplit > kChunkMaxParts || it.split < 0 || it.split >= it.nsplit ||
