@@ -492,12 +492,13 @@ def _chunk_sizes(kv_heads: int, head_dim: int) -> tuple[int, int]:
 # 1,024 (32) 470 / 257.
 UNPACK_TILES = 4
 UNPACK_BYTES = 1 << 30
+UNPACK_BATCH = 65535  # sequences of one unpacking launch
 
 
 def unpack_pays(total_q: int, batch: int, group: int, kv_heads: int, head_dim: int, max_len: int) -> bool:
     """Whether a quantised call first unpacks its sequences to 16 bits."""
     return (total_q * group >= UNPACK_TILES * 128 * batch and max_len > 0  # (empty caches have no rows to unpack)
-            and 4 * batch * max_len * kv_heads * head_dim <= UNPACK_BYTES)
+            and batch <= UNPACK_BATCH and 4 * batch * max_len * kv_heads * head_dim <= UNPACK_BYTES)
 
 
 _MAX_GROUP = 128  # query heads of one KV head that the tiled kernel takes
