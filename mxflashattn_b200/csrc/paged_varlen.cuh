@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(kPvThreads) gather_varlen_kernel(const PagedVa
   const RowWalk walk = row_walk<kGroup>(2 * p.HKV);
   constexpr bool kCheck = kDense && std::is_same_v<T, __half>;
   int lost = 0;
-  for (int pair = walk.live ? walk.pair : 2 * p.HKV; pair < 2 * p.HKV; pair += kPvThreads / kGroup) {
+  if (!kCheck && !walk.live) return;
+  for (int pair = walk.pair; (!kCheck || walk.live) && pair < 2 * p.HKV; pair += kPvThreads / kGroup) {
     const int kv = pair >= p.HKV, h = pair - kv * p.HKV;
     const uint8_t* cache = kv ? p.v_cache : p.k_cache;
     const uint8_t* scales = kv ? p.v_scales : p.k_scales;
