@@ -372,7 +372,9 @@ int mxfa_varlen_fwd_exact_launch(const void* q, const void* k, const void* v, co
  * Caches are paged [P, PS, HKV, D] with a block table int32 [B, BTW]; D in
  * {64, 128}.  Quantised caches (k_scales and v_scales given) hold e4m3 codes
  * and one e8m0 byte per token and KV head, [P, HKV, PS]: value = code *
- * 2^(byte - 127).  Out-of-range pages and positions are skipped and flagged.
+ * 2^(byte - 127).  Out-of-range pages and positions are flagged; nothing is
+ * written there, and what is read from them is zero (in attention a key of
+ * score 0, or none on the row kernel).
  * No reference counterpart: the reference appends and attends uniform
  * blocks (mxflashattn/reference.py:88-139) and has no quantised cache. */
 

@@ -487,9 +487,13 @@ def _chunk_sizes(kv_heads: int, head_dim: int) -> tuple[int, int]:
 
 
 # Unpacking costs a pass over the cached rows and then runs the faster 16-bit kernel; converting in the
-# kernel repeats its work for every tile of a sequence. Device us, converted against unpacked, 15,360 cached tokens
-# and 4 heads per KV head: 32 new tokens (1 tile) 64 / 76, 64 (2) 60 / 65, 128 (4) 82 / 70, 256 (8) 136 / 95,
-# 1,024 (32) 470 / 257.
+# kernel repeats its work for every tile of a sequence. Device us, converted / unpacked, bf16, 8 KV heads, 4 heads each:
+#   one sequence of 15,360 cached tokens: 32 new ones (1 tile) 65 / 76, 64 (2) 60 / 64, 96 (3) 67 / 65,
+#     128 (4) 80 / 68, 256 (8) 133 / 93, 1,024 (32) 468 / 248
+#   8 sequences of 2,000: 64 each 43 / 51, 128 (4) 81 / 71, 256 159 / 122
+#   512 tokens on 4,096 and 31 decodes on as many (2 tiles a sequence): 207 / 251
+# fp16 (with the converting launch behind): 128 on 15,360 84 / 75, 8 x 128 on 2,000 83 / 85, 1,024 495 / 262.
+# bf16 P is rounded to 8 bits on unpacked rows, as on a 16-bit cache, and to f16's 11 in the converting kernel.
 UNPACK_TILES = 4
 UNPACK_BYTES = 1 << 30
 UNPACK_BATCH = 65535  # sequences of one unpacking launch

@@ -25,7 +25,7 @@ int paged_varlen_checks(const void* k_cache, const void* v_cache, const void* k_
 // Tokens a CTA takes: one while that still fills the GPU's CTA slots (8 of
 // 256 threads per SM), so a decode step's few tokens spread over every SM,
 // and up to 16 for long prompts, where a CTA's token lookups overlap (read-back of
-// 8 x 16,384 tokens: 91 us at 16, 97 at 32, 93 at 8; the append 78, 78, 81).
+// 8 x 16,384 tokens: 91 us at 16, 97 at 32, 93 at 8; the append, 69 now, was at 78, 78, 81 then).
 int tokens_per_cta(int total) {
   const int n = (total + 8 * sm_count() - 1) / (8 * sm_count());
   return n > kPvMaxTok ? kPvMaxTok : n;

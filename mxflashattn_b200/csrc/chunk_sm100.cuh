@@ -34,14 +34,15 @@
 //    two instructions per pair of codes; widening to bf16 took five.  The scale
 //    bytes come by a warp of their own.
 //
-// Measured (HQ 32, HKV 8, D 128, bf16): 2,048 tokens on 14,336 cached take 443 us
-// in a burst (1,162 TFLOP/s) and 517 back to back under the power cap, 1,920
+// Measured (HQ 32, HKV 8, D 128, bf16): 2,048 tokens on 14,336 cached take 445 us
+// in a burst (1,157 TFLOP/s) and 521 back to back under the power cap, 1,920
 // cycles per key tile and SM, all included, against 1,024 of tensor work.  On 512
 // tokens issue is active 0.44 per scheduler and the tensor pipe 46%: what remains
 // is taken to be the latency from one score buffer's product to its next.  The loops stay
 // rolled because all warps' code has to fit the instruction cache (541 -> 515 us).
-// Converting e4m3 in the kernel takes 470 us for 1,024 tokens on 15,360, against
-// 257 with the rows unpacked first, so only short pieces convert.
+// Converting e4m3 in the kernel takes 468 us for 1,024 tokens on 15,360, against
+// 248 with the rows unpacked first, so only short pieces convert; 722 where every
+// tile is wide (see kWideTile).
 #pragma once
 
 #include "paged_varlen.cuh"
@@ -312,8 +313,8 @@ struct ChunkParams {
 template <int HD, bool kQuant>
 struct ChunkCfg {
   // softmax groups of four warps; group g takes tiles j % kGroups == g.  At D = 64 the products
-  // of a tile are short and a third group pays (46.2 -> 43.4 us on ragged pieces); at D = 128 it
-  // costs (477 -> 494 us on a long one).
+  // of a tile are short and a third group pays (46.2 -> 43.4 us on ragged pieces, the one case it was
+  // tried on; later steps brought them to 32-36); at D = 128 it costs (477 -> 494 us on a long one).
   static constexpr int kGroups = !kQuant && HD == 64 ? 3 : 2;
   static constexpr int kThreads = kQuant ? 1024 : 128 + 128 * kGroups;
   static constexpr int kDBlk = HD / 64;

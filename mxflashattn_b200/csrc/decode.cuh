@@ -334,8 +334,6 @@ __device__ __forceinline__ void merge_split_row(const float* ows, const float* m
   if (lse != nullptr && lane == 0) lse[r] = L != 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
 }
 
-// kFp8: e4m3 caches.  Tiles are dequantised in registers (cvt e4m3x2 ->
-// f16x2, exact) and both products run in f16; q is converted to f16 once.
 // merge_split_row for the exchange: the normalised f32 row and its LSE,
 // tagged with step tag, are written to the record slot [rank][r] of every
 // rank's exchange buffer (16-byte stores of two tagged words).
@@ -448,14 +446,17 @@ __device__ __forceinline__ void ldsm_b8_x2_trans(uint32_t addr, uint32_t& r0, ui
                : "r"(addr));
 }
 
+// kFp8: e4m3 caches.  Tiles are dequantised in registers (cvt e4m3x2 ->
+// f16x2, exact) and both products run in f16; q is converted to f16 once.
 // kRowScale (with kFp8 and kTma): each token of a KV head has its own
 // power-of-two scales.  The K scale multiplies the token's scores; V's
 // exponent joins the score before the maximum, so the stored state counts O
 // and d in units of 2^m with P relative to the largest p * |scale| (P never
-// leaves f16's range whatever the scales are), and is taken out of the row
-// sum again: d = sum P 2^-e.  The merge algebra is unchanged.  128 sequences of up
-// to 1,281 tokens (8 KV heads of 128) take 39.8 us on the device, 0.66 of the copy
-// bandwidth; one scale per tensor takes 34 on the same cache.
+// leaves f16's range), and is taken out of the row sum again: d = sum P 2^-e.
+// e runs from -60, and V scales within 2^100 of one another lose no term of d
+// that counts.  The merge algebra is unchanged.  128 sequences of up to 1,281 tokens (8 KV heads of
+// 128) take 38.5 us on the device, 0.68 of the copy bandwidth (39.8 where one scale per
+// tensor took 34 on the same cache).
 template <typename T, int HD, int NT, bool kTma, bool kFp8 = false, bool kRowScale = false>
 __global__ void __launch_bounds__(kDecThreads, DecodeCfg<HD, NT, kFp8>::kCtasPerSm)
     paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap tmk,

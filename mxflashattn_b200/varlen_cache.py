@@ -14,7 +14,9 @@ and every layer; no call changes them.
 
 A quantised cache is a pair of ``torch.float8_e4m3fn`` tensors [P, PS, HKV, D]
 with a pair of ``torch.float8_e8m0fnu`` scale tensors [P, HKV, PS]: one
-power-of-two scale per token and KV head, value = code * scale.
+power-of-two scale per token and KV head, value = code * scale.  Scales of one
+sequence may lie as far apart as they like for K, within 2^100 of one another
+for V; values under 2^-75 count as zero.
 
 Calls validate on the host without reading device memory;
 ``MXFLASHATTN_STRICT_VALIDATION=1`` adds checks of the lengths and the table
