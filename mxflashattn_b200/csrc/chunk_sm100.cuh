@@ -506,10 +506,11 @@ __global__ void __launch_bounds__(ChunkCfg<HD, kQuant>::kThreads, 1)
   }
   if (p.inexact != nullptr) {
     constexpr int kPer = kTcKeys / kPvMaxTok;  // blocks of a key tile
-    const int end = min(min(it.kt1, (p.unpacked + kTcKeys - 1) / kTcKeys) * kPer, unpacked_blocks(min(it.total, p.unpacked)));
+    const int tiles = (p.unpacked + kTcKeys - 1) / kTcKeys;
+    const int end = min(min(it.kt1, tiles) * kPer, unpacked_blocks(min(it.total, p.unpacked)));
     const int* f = p.inexact + static_cast<size_t>(it.b) * unpacked_blocks(p.unpacked);
     int lost = 0;
-    for (int i = it.kt0 * kPer + threadIdx.x; i < end; i += Cfg::kThreads) lost |= f[i];
+    for (int i = min(it.kt0, tiles) * kPer + threadIdx.x; i < end; i += Cfg::kThreads) lost |= f[i];
     if ((__syncthreads_or(lost) != 0) != kQuant) return;
   }
   // keys the block table can hold; a longer sequence is flagged and cut
