@@ -506,6 +506,7 @@ def unpack_pays(total_q: int, batch: int, group: int, kv_heads: int, head_dim: i
 
 
 _MAX_GROUP = 128  # query heads of one KV head that the tiled kernel takes
+_MAX_STEP_BATCH = 65535  # sequences that the split-KV kernel takes
 
 
 def kvcache_chunk_plan(cu_seqlens_q, cache_seqlens, total_q: int, q_heads: int, kv_heads: int, causal: bool):
@@ -539,7 +540,7 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, cu_seqlens_q, cache_seql
     lib = _L()
     with _on(q):
         stream = _stream(q)
-        if max_seqlen_q <= 1 and Tq and B and (k_scales is None or (D == 128 and PS % 16 == 0)):
+        if max_seqlen_q <= 1 and Tq and 0 < B <= _MAX_STEP_BATCH and (k_scales is None or (D == 128 and PS % 16 == 0)):
             # a decode step: the split-KV kernel reads K/V once for the query heads of a KV head
             # without a 128-row tile to fill
             q = _contig(q)
